@@ -243,6 +243,43 @@ int opmx_rms_norm(const void *X, const void *weight, const void *SkipIn, int64_t
 int opmx_moe_reduce(const void *Y, const void *expert_weights, const int64_t *invert_permutation,
                     int64_t T, int k, int64_t N, int dtype, void *out, void *stream);
 
+/* Activations kept in 8 bits for a backward pass (no counterpart in the reference, which only runs forward).
+ * Blocks of 32 consecutive values of a row (the last one of a row may be shorter) share a power-of-two step:
+ * with m the largest magnitude of a block, 2^e the largest power of two not above m (one more if
+ * m >= 1.9921875 * 2^e, but never beyond the type's largest exponent), the step is 2^max(e - 6, -126) and a
+ * value x is held as q = round-half-even(x / step) in [-127, 127]; code = the step's biased exponent.  A block
+ * with an infinity or a NaN has code 255 and q = 0 and stands for NaN throughout.
+ *   X [R,D] (dtype), q [R,D] int8, code [R, ceil(D/32)] uint8; X may start at any address its type allows.
+ * pack writes q and code, unpack writes the values q * step rounded to dtype (exact in float32 and bfloat16,
+ * and in float16 down to its smallest magnitudes). */
+#define OPMX_CHECKPOINT8_BLOCK 32
+int opmx_checkpoint8_pack(const void *X, int64_t R, int64_t D, int dtype, int8_t *q, uint8_t *code, void *stream);
+int opmx_checkpoint8_unpack(const int8_t *q, const uint8_t *code, int64_t R, int64_t D, int dtype, void *X, void *stream);
+
+/* SwiGLU for training: opmx_swiglu and, in the same pass, its input in 8 bits; both halves of a row have their
+ * own blocks: q [R,2,D], code [R,2,ceil(D/32)].  The backward pass takes the gradient at the held values a, g:
+ *   dX[r, D+i] = dY a s(beta a),   dX[r, i] = dY g s(beta a) (1 + beta a (1 - s(beta a))).
+ * X, dX [R,2D]; Y, dY [R,D] (dtype); fp32 arithmetic, one rounding. */
+int opmx_swiglu_checkpoint8(const void *X, int64_t R, int64_t D, float beta, int dtype, void *Y, int8_t *q, uint8_t *code,
+                            void *stream);
+int opmx_swiglu_checkpoint8_backward(const void *dY, const int8_t *q, const uint8_t *code, int64_t R, int64_t D,
+                                     float beta, int dtype, void *dX, void *stream);
+
+/* Balance loss of the router and tokens per expert (no counterpart in the reference).
+ *   p[t,:] = softmax(scores[t,:]) (0 for a row of -inf alone), count[e] = kept tokens with e among their k
+ *   largest scores (the picks of opmx_moe_select), f = count / (k n), n = kept tokens,
+ *   loss = E sum_e f_e (1/n) sum_t p[t,e]: 1 for a router that spreads evenly; 0 when no token is kept.
+ * scores [T,E] (dtype); token_mask [T] bytes, 0 = the token does not count (NULL: all count);
+ * loss: one float; expert_count [E] int64; weight [E] float: w_e = E f_e / n, what the backward pass needs;
+ * workspace: opmx_moe_balance_loss_workspace_bytes(), 16-byte aligned, not shared with a call running at the same time.
+ * backward, f held constant:  dscores[t,e] = dloss p[t,e] (w_e - sum_j w_j p[t,j]), 0 for tokens that do not
+ * count; dloss: one float on the device.  E and k limits are those of opmx_moe_select. */
+size_t opmx_moe_balance_loss_workspace_bytes(int64_t T, int E);
+int opmx_moe_balance_loss(const void *scores, const uint8_t *token_mask, int64_t T, int E, int k, int dtype, float *loss,
+                          int64_t *expert_count, float *weight, void *workspace, size_t workspace_bytes, void *stream);
+int opmx_moe_balance_loss_backward(const void *scores, const uint8_t *token_mask, const float *weight, const float *dloss,
+                                   int64_t T, int E, int dtype, void *dscores, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

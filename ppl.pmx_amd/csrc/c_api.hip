@@ -352,4 +352,66 @@ int opmx_moe_reduce(const void *Y, const void *expert_weights, const int64_t *in
     return launch_moe_reduce(Y, expert_weights, invert_permutation, T, k, N, dtype, out, st(stream));
 }
 
+int opmx_checkpoint8_pack(const void *X, int64_t R, int64_t D, int dtype, int8_t *q, uint8_t *code, void *stream)
+{
+    if (R < 0 || D < 0) return OPMX_ERR_BAD_ARGUMENT;
+    if (!dtype_ok(dtype)) return OPMX_ERR_UNSUPPORTED;
+    if (R == 0 || D == 0) return OPMX_OK;
+    if (!X || !q || !code) return OPMX_ERR_BAD_ARGUMENT;
+    return launch_checkpoint8_pack(X, R, D, dtype, q, code, st(stream));
+}
+
+int opmx_checkpoint8_unpack(const int8_t *q, const uint8_t *code, int64_t R, int64_t D, int dtype, void *X, void *stream)
+{
+    if (R < 0 || D < 0) return OPMX_ERR_BAD_ARGUMENT;
+    if (!dtype_ok(dtype)) return OPMX_ERR_UNSUPPORTED;
+    if (R == 0 || D == 0) return OPMX_OK;
+    if (!X || !q || !code) return OPMX_ERR_BAD_ARGUMENT;
+    return launch_checkpoint8_unpack(q, code, R, D, dtype, X, st(stream));
+}
+
+int opmx_swiglu_checkpoint8(const void *X, int64_t R, int64_t D, float beta, int dtype, void *Y, int8_t *q, uint8_t *code,
+                            void *stream)
+{
+    if (R < 0 || D < 0) return OPMX_ERR_BAD_ARGUMENT;
+    if (!dtype_ok(dtype)) return OPMX_ERR_UNSUPPORTED;
+    if (R == 0 || D == 0) return OPMX_OK;
+    if (!X || !Y || !q || !code) return OPMX_ERR_BAD_ARGUMENT;
+    return launch_swiglu_checkpoint8(X, R, D, beta, dtype, Y, q, code, st(stream));
+}
+
+int opmx_swiglu_checkpoint8_backward(const void *dY, const int8_t *q, const uint8_t *code, int64_t R, int64_t D,
+                                     float beta, int dtype, void *dX, void *stream)
+{
+    if (R < 0 || D < 0) return OPMX_ERR_BAD_ARGUMENT;
+    if (!dtype_ok(dtype)) return OPMX_ERR_UNSUPPORTED;
+    if (R == 0 || D == 0) return OPMX_OK;
+    if (!dY || !q || !code || !dX) return OPMX_ERR_BAD_ARGUMENT;
+    return launch_swiglu_checkpoint8_backward(dY, q, code, R, D, beta, dtype, dX, st(stream));
+}
+
+size_t opmx_moe_balance_loss_workspace_bytes(int64_t T, int E) { return moe_balance_loss_workspace_bytes(T, E); }
+
+int opmx_moe_balance_loss(const void *scores, const uint8_t *token_mask, int64_t T, int E, int k, int dtype, float *loss,
+                          int64_t *expert_count, float *weight, void *workspace, size_t workspace_bytes, void *stream)
+{
+    if (T < 0 || E <= 0 || k <= 0 || k > E) return OPMX_ERR_BAD_ARGUMENT;
+    if (!dtype_ok(dtype) || E > OPMX_MOE_MAX_EXPERTS || k > OPMX_MOE_MAX_EXPERTS_PER_TOKEN) return OPMX_ERR_UNSUPPORTED;
+    if (T > (int64_t{1} << 31) / k) return OPMX_ERR_UNSUPPORTED;
+    if (!loss || !expert_count || !weight || (T > 0 && !scores)) return OPMX_ERR_BAD_ARGUMENT;
+    if (T > 0 && (!workspace || workspace_bytes < moe_balance_loss_workspace_bytes(T, E))) return OPMX_ERR_WORKSPACE;
+    if (workspace && !aligned16(workspace)) return OPMX_ERR_ALIGNMENT;
+    return launch_moe_balance_loss(scores, token_mask, T, E, k, dtype, loss, expert_count, weight, workspace, st(stream));
+}
+
+int opmx_moe_balance_loss_backward(const void *scores, const uint8_t *token_mask, const float *weight, const float *dloss,
+                                   int64_t T, int E, int dtype, void *dscores, void *stream)
+{
+    if (T < 0 || E <= 0) return OPMX_ERR_BAD_ARGUMENT;
+    if (!dtype_ok(dtype) || E > OPMX_MOE_MAX_EXPERTS) return OPMX_ERR_UNSUPPORTED;
+    if (T == 0) return OPMX_OK;
+    if (!scores || !weight || !dloss || !dscores) return OPMX_ERR_BAD_ARGUMENT;
+    return launch_moe_balance_loss_backward(scores, token_mask, weight, dloss, T, E, dtype, dscores, st(stream));
+}
+
 }  // extern "C"

@@ -8,7 +8,9 @@ the seven operators of the MoE layer and the RMSNorm pair in front of it, plus f
 are not ONNX nodes (gate/up GEMM with SwiGLU, router gate with MoeSelect, and MoeSelect as an
 index that the gate/up GEMM reads the tokens through, without the expanded copy).
 """
+from .Checkpoint8 import checkpoint8_pack, checkpoint8_unpack, swiglu_checkpoint8
 from .Linear import linear
+from .MoeBalanceLoss import moe_balance_loss
 from .MoeColumnParallelLinear import (moe_column_parallel_linear, moe_column_parallel_linear_indexed,
                                       moe_column_parallel_linear_swiglu)
 from .MoeReduce import moe_reduce
@@ -18,6 +20,7 @@ from .RMSNorm import rms_norm, skip_rms_norm
 from .SiLU import silu
 from .SwiGLU import swiglu
 
-__all__ = ["linear", "moe_column_parallel_linear", "moe_column_parallel_linear_indexed",
+__all__ = ["checkpoint8_pack", "checkpoint8_unpack", "linear", "moe_balance_loss", "moe_column_parallel_linear", "moe_column_parallel_linear_indexed",
            "moe_column_parallel_linear_swiglu", "moe_reduce", "moe_route_select", "moe_route_select_index",
-           "moe_row_parallel_linear", "moe_select", "moe_select_index", "rms_norm", "silu", "skip_rms_norm", "swiglu"]
+           "moe_row_parallel_linear", "moe_select", "moe_select_index", "rms_norm", "silu", "skip_rms_norm", "swiglu",
+           "swiglu_checkpoint8"]

@@ -49,6 +49,13 @@ _SIGNATURES = {
     "opmx_swiglu": (_int, [_vp, _i64, _i64, _f, _int, _vp, _vp]),
     "opmx_silu": (_int, [_vp, _vp, _i64, _int, _vp, _vp]),
     "opmx_rms_norm": (_int, [_vp, _vp, _vp, _i64, _i64, _f, _int, _vp, _vp, _vp]),
+    "opmx_checkpoint8_pack": (_int, [_vp, _i64, _i64, _int, _vp, _vp, _vp]),
+    "opmx_checkpoint8_unpack": (_int, [_vp, _vp, _i64, _i64, _int, _vp, _vp]),
+    "opmx_swiglu_checkpoint8": (_int, [_vp, _i64, _i64, _f, _int, _vp, _vp, _vp, _vp]),
+    "opmx_swiglu_checkpoint8_backward": (_int, [_vp, _vp, _vp, _i64, _i64, _f, _int, _vp, _vp]),
+    "opmx_moe_balance_loss_workspace_bytes": (_sz, [_i64, _int]),
+    "opmx_moe_balance_loss": (_int, [_vp, _vp, _i64, _int, _int, _int, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "opmx_moe_balance_loss_backward": (_int, [_vp, _vp, _vp, _vp, _i64, _int, _int, _vp, _vp]),
     "opmx_moe_reduce": (_int, [_vp, _vp, _vp, _i64, _int, _i64, _int, _vp, _vp]),
 }
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
@@ -105,6 +112,23 @@ def require_gpu(what: str, *tensors: Optional[torch.Tensor]) -> torch.device:
             raise RuntimeError("{}: tensors are on different devices".format(what))
         dev = t.device
     return dev
+
+
+class on_device:
+    """Makes ``dev`` the current GPU for the calls inside (the library launches on the current one); nothing to do,
+    and nothing spent, when it already is."""
+
+    def __init__(self, dev: torch.device):
+        self.want = dev.index
+
+    def __enter__(self):
+        self.had = torch.cuda.current_device()
+        if self.want is not None and self.want != self.had:
+            torch.cuda.set_device(self.want)
+
+    def __exit__(self, *exc):
+        if self.want is not None and self.want != self.had:
+            torch.cuda.set_device(self.had)
 
 
 def ptr(t: Optional[torch.Tensor]):

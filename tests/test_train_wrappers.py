@@ -1,0 +1,108 @@
+"""CPU: what the training operators refuse, in the package and at the C interface, before anything runs on a device."""
+import ctypes
+
+import pytest
+import torch
+
+import torch_function as OPMX
+from torch_function import _lib
+
+ONE = ctypes.c_void_p(256)      # never dereferenced on these paths
+
+
+def test_no_cpu_path():
+    x = torch.randn(4, 16)
+    for call in (lambda: OPMX.checkpoint8_pack(x), lambda: OPMX.swiglu_checkpoint8(x),
+                 lambda: OPMX.checkpoint8_unpack(torch.zeros(4, 16, dtype=torch.int8),
+                                                 torch.zeros(4, 1, dtype=torch.uint8), torch.float32),
+                 lambda: OPMX.moe_balance_loss(x, 16, 2)):
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            call()
+
+
+def test_public_names_and_signatures():
+    import inspect
+    sig = lambda f: list(inspect.signature(f).parameters)
+    assert sig(OPMX.swiglu_checkpoint8) == ["X", "beta"]
+    assert sig(OPMX.checkpoint8_pack) == ["X"] and sig(OPMX.checkpoint8_unpack) == ["q", "code", "dtype"]
+    assert sig(OPMX.moe_balance_loss) == ["scores", "num_experts", "num_experts_per_token", "token_mask"]
+
+
+def test_checkpoint8_c_interface():
+    L = _lib.lib()
+    assert L.opmx_checkpoint8_pack(ONE, -1, 8, 1, ONE, ONE, None) == -1
+    assert L.opmx_checkpoint8_pack(ONE, 4, 8, 7, ONE, ONE, None) == -2
+    for i in (0, 4, 5):
+        a = [ONE, 4, 8, 1, ONE, ONE, None]
+        a[i] = None
+        assert L.opmx_checkpoint8_pack(*a) == -1
+    assert L.opmx_checkpoint8_pack(None, 0, 8, 1, None, None, None) == 0
+    assert L.opmx_checkpoint8_unpack(ONE, ONE, 4, -8, 1, ONE, None) == -1
+    assert L.opmx_checkpoint8_unpack(ONE, ONE, 4, 8, 3, ONE, None) == -2
+    assert L.opmx_checkpoint8_unpack(ONE, None, 4, 8, 1, ONE, None) == -1
+    assert L.opmx_checkpoint8_unpack(None, None, 4, 0, 1, None, None) == 0
+    assert L.opmx_swiglu_checkpoint8(ONE, 4, 8, 1.0, 9, ONE, ONE, ONE, None) == -2
+    for i in (0, 5, 6, 7):
+        a = [ONE, 4, 8, 1.0, 1, ONE, ONE, ONE, None]
+        a[i] = None
+        assert L.opmx_swiglu_checkpoint8(*a) == -1
+    assert L.opmx_swiglu_checkpoint8(None, 0, 8, 1.0, 1, None, None, None, None) == 0
+    for i in (0, 1, 2, 7):
+        a = [ONE, ONE, ONE, 4, 8, 1.0, 1, ONE, None]
+        a[i] = None
+        assert L.opmx_swiglu_checkpoint8_backward(*a) == -1
+    assert L.opmx_swiglu_checkpoint8_backward(ONE, ONE, ONE, 4, 8, 1.0, -1, ONE, None) == -2
+    assert L.opmx_swiglu_checkpoint8_backward(None, None, None, 4, 0, 1.0, 1, None, None) == 0
+
+
+def test_balance_loss_c_interface():
+    L = _lib.lib()
+    need = L.opmx_moe_balance_loss_workspace_bytes(4096, 64)
+    assert need % 256 == 0 and need >= 256
+
+    def call(scores=ONE, mask=None, T=4096, E=64, k=8, dtype=1, loss=ONE, count=ONE, w=ONE, ws=ONE, bytes_=need):
+        return L.opmx_moe_balance_loss(scores, mask, T, E, k, dtype, loss, count, w, ws, bytes_, None)
+
+    assert call(T=-1) == -1 and call(E=0) == -1 and call(k=0) == -1 and call(k=65) == -1
+    assert call(E=257) == -2 and call(k=33) == -2 and call(dtype=4) == -2 and call(T=1 << 40) == -2
+    assert call(scores=None) == -1 and call(loss=None) == -1 and call(count=None) == -1 and call(w=None) == -1
+    assert call(ws=None) == -3 and call(bytes_=need - 1) == -3 and call(ws=ctypes.c_void_p(264)) == -4
+
+    def back(scores=ONE, w=ONE, d=ONE, T=8, E=8, dtype=1, out=ONE):
+        return L.opmx_moe_balance_loss_backward(scores, None, w, d, T, E, dtype, out, None)
+
+    assert back(T=-1) == -1 and back(E=0) == -1 and back(E=300) == -2 and back(dtype=9) == -2
+    assert back(scores=None) == -1 and back(w=None) == -1 and back(d=None) == -1 and back(out=None) == -1
+    assert back(None, None, None, 0, 8, 1, None) == 0
+
+
+@pytest.mark.gpu
+def test_package_refusals():
+    d = torch.device("cuda:0")
+    x = torch.randn(4, 15, device=d)
+    with pytest.raises(ValueError, match="even"):
+        OPMX.swiglu_checkpoint8(x)
+    with pytest.raises(TypeError):
+        OPMX.swiglu_checkpoint8(x[:, :14].double())
+    with pytest.raises(TypeError):
+        OPMX.checkpoint8_pack(x.int())
+    q, code = OPMX.checkpoint8_pack(x)
+    with pytest.raises(TypeError):
+        OPMX.checkpoint8_unpack(q.int(), code, torch.float32)
+    with pytest.raises(TypeError):
+        OPMX.checkpoint8_unpack(q, code, torch.int32)
+    with pytest.raises(ValueError):
+        OPMX.checkpoint8_unpack(q, code[:3], torch.float32)
+    for a in ((x, 8, 2), (x, 15, 0), (x, 15, 16), (x, 15, 2, torch.ones(4, device=d)),
+              (x, 15, 2, torch.ones(3, dtype=torch.bool, device=d))):
+        with pytest.raises(ValueError):
+            OPMX.moe_balance_loss(*a)
+    with pytest.raises(TypeError):
+        OPMX.moe_balance_loss(x.double(), 15, 2)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        OPMX.moe_balance_loss(x, 15, 2, torch.ones(4, dtype=torch.bool))
+    leaf = x[:, :14].clone().requires_grad_(True)
+    y = OPMX.swiglu_checkpoint8(leaf)
+    g, = torch.autograd.grad(y, leaf, torch.ones_like(y).requires_grad_(True), create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
