@@ -65,6 +65,15 @@ typedef enum opmx_epilogue {
     OPMX_EPILOGUE_SWIGLU = 1
 } opmx_epilogue;
 
+/* Activations of opmx_linear_epilogue. */
+typedef enum opmx_activation {
+    OPMX_ACTIVATION_NONE = 0,
+    OPMX_ACTIVATION_SILU = 1,       /* h s(h), s the logistic function */
+    OPMX_ACTIVATION_GELU = 2,       /* h Phi(h), Phi the normal distribution function */
+    OPMX_ACTIVATION_GELU_TANH = 3,  /* h/2 (1 + tanh(sqrt(2/pi) (h + 0.044715 h^3))) */
+    OPMX_ACTIVATION_SWIGLU = 4      /* h[D+i] h[i] s(h[i]), D = N/2: Y is [T, N/2] */
+} opmx_activation;
+
 /* Limits of the routing kernels. */
 #define OPMX_MOE_MAX_EXPERTS 256
 #define OPMX_MOE_MAX_EXPERTS_PER_TOKEN 32
@@ -264,6 +273,27 @@ int opmx_swiglu_checkpoint8(const void *X, int64_t R, int64_t D, float beta, int
                             void *stream);
 int opmx_swiglu_checkpoint8_backward(const void *dY, const int8_t *q, const uint8_t *code, int64_t R, int64_t D,
                                      float beta, int dtype, void *dX, void *stream);
+
+/* Linear with bias, activation and residual in its epilogue, and its gradients (the reference has the parts:
+ * Linear.forward torch_function/Linear.py:25-33, and SiLU, GELU, SwiGLU as operators of their own):
+ *   H = X W^T + B,  Y = act(H) + R         sums and epilogue in fp32, one rounding
+ * X [T,K], W [N,K], B [N] or NULL, R (residual) [T,M] or NULL, Y [T,M]; M = N, or N/2 with OPMX_ACTIVATION_SWIGLU.
+ * H: NULL, or [T,N], receives H rounded to dtype for the backward pass.
+ * backward: from dY [T,M]
+ *   dH = dY * act'(H) (rounded to dtype),  dX = dH W [T,K],  dW = dH^T X [N,K],  dB = sum_t dH [N] (summed unrounded)
+ * each of dX, dW, dB may be NULL (not wanted).  dX needs W; dW needs X, or its 8-bit form x_q, x_code (see
+ * opmx_checkpoint8_pack; then X is ignored); every activation but NONE needs H.  The gradient of R is dY.
+ * X, W, dY start at multiples of 16 bytes where K (dY: N, without an activation) is a multiple of 16 bytes
+ * (OPMX_ERR_ALIGNMENT otherwise), the others anywhere their type allows.
+ * workspace: opmx_linear_epilogue[_backward]_workspace_bytes(), 256-byte aligned, contents arbitrary, not shared with
+ * a call running at the same time.  Results do not vary from call to call.  K < 2^21. */
+size_t opmx_linear_epilogue_workspace_bytes(int64_t T, int64_t K, int64_t N, int dtype, int activation);
+int opmx_linear_epilogue(const void *X, const void *W, const void *B, const void *R, int64_t T, int64_t K, int64_t N,
+                         int dtype, int activation, void *Y, void *H, void *workspace, size_t workspace_bytes, void *stream);
+size_t opmx_linear_epilogue_backward_workspace_bytes(int64_t T, int64_t K, int64_t N, int dtype, int activation);
+int opmx_linear_epilogue_backward(const void *dY, const void *X, const int8_t *x_q, const uint8_t *x_code, const void *W,
+                                  const void *H, int64_t T, int64_t K, int64_t N, int dtype, int activation, void *dX,
+                                  void *dW, void *dB, void *workspace, size_t workspace_bytes, void *stream);
 
 /* Balance loss of the router and tokens per expert (no counterpart in the reference).
  *   p[t,:] = softmax(scores[t,:]) (0 for a row of -inf alone), count[e] = kept tokens with e among their k

@@ -390,6 +390,67 @@ int opmx_swiglu_checkpoint8_backward(const void *dY, const int8_t *q, const uint
     return launch_swiglu_checkpoint8_backward(dY, q, code, R, D, beta, dtype, dX, st(stream));
 }
 
+// Sizes whose offsets inside a tile (256 rows) and whose counts of tiles and values stay in range.
+static bool linear_sizes_ok(int64_t T, int64_t K, int64_t N)
+{
+    constexpr int64_t most = int64_t{1} << 21, rows = int64_t{1} << 31;
+    return K < most && N < most && T < rows;
+}
+
+size_t opmx_linear_epilogue_workspace_bytes(int64_t T, int64_t K, int64_t N, int dtype, int activation)
+{
+    if (T <= 0 || K <= 0 || N <= 0 || !dtype_ok(dtype) || !linear_sizes_ok(T, K, N)) return 256;
+    return linear_epilogue_workspace_bytes(T, K, N, dtype, activation);
+}
+
+int opmx_linear_epilogue(const void *X, const void *W, const void *B, const void *R, int64_t T, int64_t K, int64_t N,
+                         int dtype, int activation, void *Y, void *H, void *workspace, size_t workspace_bytes, void *stream)
+{
+    if (T < 0 || K < 0 || N < 0 || activation < OPMX_ACTIVATION_NONE || activation > OPMX_ACTIVATION_SWIGLU)
+        return OPMX_ERR_BAD_ARGUMENT;
+    if (activation == OPMX_ACTIVATION_SWIGLU && N % 2) return OPMX_ERR_BAD_ARGUMENT;
+    if (!dtype_ok(dtype) || !linear_sizes_ok(T, K, N)) return OPMX_ERR_UNSUPPORTED;
+    if (T == 0 || N == 0) return OPMX_OK;
+    if (!X || !W || !Y || K == 0) return OPMX_ERR_BAD_ARGUMENT;
+    if (K * static_cast<int64_t>(elt(dtype)) % 16 == 0 && !(aligned16(X) && aligned16(W))) return OPMX_ERR_ALIGNMENT;
+    const size_t need = linear_epilogue_workspace_bytes(T, K, N, dtype, activation);
+    if (need > 256 && (!workspace || workspace_bytes < need)) return OPMX_ERR_WORKSPACE;
+    if (workspace && (reinterpret_cast<uintptr_t>(workspace) & 255u)) return OPMX_ERR_ALIGNMENT;
+    return launch_linear_epilogue(X, W, B, R, T, K, N, dtype, activation, Y, H, workspace, st(stream));
+}
+
+size_t opmx_linear_epilogue_backward_workspace_bytes(int64_t T, int64_t K, int64_t N, int dtype, int activation)
+{
+    if (T < 0 || K <= 0 || N <= 0 || !dtype_ok(dtype) || !linear_sizes_ok(T, K, N)) return 256;
+    return linear_epilogue_backward_workspace_bytes(T, K, N, dtype, activation);
+}
+
+int opmx_linear_epilogue_backward(const void *dY, const void *X, const int8_t *x_q, const uint8_t *x_code, const void *W,
+                                  const void *H, int64_t T, int64_t K, int64_t N, int dtype, int activation, void *dX,
+                                  void *dW, void *dB, void *workspace, size_t workspace_bytes, void *stream)
+{
+    if (T < 0 || K < 0 || N < 0 || activation < OPMX_ACTIVATION_NONE || activation > OPMX_ACTIVATION_SWIGLU)
+        return OPMX_ERR_BAD_ARGUMENT;
+    if (activation == OPMX_ACTIVATION_SWIGLU && N % 2) return OPMX_ERR_BAD_ARGUMENT;
+    if (!dtype_ok(dtype) || !linear_sizes_ok(T, K, N)) return OPMX_ERR_UNSUPPORTED;
+    if (K == 0 || N == 0) return OPMX_ERR_BAD_ARGUMENT;
+    if (!dX && !dW && !dB) return OPMX_OK;
+    if (T > 0) {
+        if (!dY || (activation != OPMX_ACTIVATION_NONE && !H) || (dX && !W)) return OPMX_ERR_BAD_ARGUMENT;
+        if (dW && !(x_q && x_code) && !X) return OPMX_ERR_BAD_ARGUMENT;
+    }
+    if ((x_q == nullptr) != (x_code == nullptr)) return OPMX_ERR_BAD_ARGUMENT;
+    const int64_t size = static_cast<int64_t>(elt(dtype));
+    if (K * size % 16 == 0 && ((dX && !aligned16(W)) || (dW && !x_q && !aligned16(X)))) return OPMX_ERR_ALIGNMENT;
+    if (activation == OPMX_ACTIVATION_NONE && N * size % 16 == 0 && !aligned16(dY)) return OPMX_ERR_ALIGNMENT;
+    const size_t need = linear_epilogue_backward_workspace_bytes(T, K, N, dtype, activation);
+    if (need > 256 && (!workspace || workspace_bytes < need)) return OPMX_ERR_WORKSPACE;
+    if (workspace && (reinterpret_cast<uintptr_t>(workspace) & 255u)) return OPMX_ERR_ALIGNMENT;
+    if (T == 0) dX = nullptr;
+    return launch_linear_epilogue_backward(dY, X, x_q, x_code, W, H, T, K, N, dtype, activation, dX, dW, dB, workspace,
+                                           st(stream));
+}
+
 size_t opmx_moe_balance_loss_workspace_bytes(int64_t T, int E) { return moe_balance_loss_workspace_bytes(T, E); }
 
 int opmx_moe_balance_loss(const void *scores, const uint8_t *token_mask, int64_t T, int E, int k, int dtype, float *loss,

@@ -114,7 +114,8 @@ __global__ __launch_bounds__(256) void pack8_kernel(const T *__restrict__ X, int
 
 template <typename T>
 __global__ __launch_bounds__(256) void unpack8_kernel(const int8_t *__restrict__ q, const uint8_t *__restrict__ codes,
-                                                      int64_t R, int64_t D, int64_t blocks, T *__restrict__ X)
+                                                      int64_t R, int64_t D, int64_t blocks, int64_t pitch,
+                                                      T *__restrict__ X)
 {
     constexpr int n = Chunk<T>::n;
     const int64_t c = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) * n, left = D - c;
@@ -126,7 +127,7 @@ __global__ __launch_bounds__(256) void unpack8_kernel(const int8_t *__restrict__
         Chunk<T> x;
 #pragma unroll
         for (int j = 0; j < n; ++j) x.v[j] = from_f32<T>(from_steps(b.v[j], code));
-        store_chunk(X + r * D + c, x, left);
+        store_chunk(X + r * pitch + c, x, left);
     }
 }
 
@@ -211,11 +212,12 @@ template <typename T> int pack8_impl(const void *X, int64_t R, int64_t D, void *
     OPMX_LAUNCH_CHECK();
     return OPMX_OK;
 }
-template <typename T> int unpack8_impl(const void *q, const void *codes, int64_t R, int64_t D, void *X, hipStream_t s)
+template <typename T>
+int unpack8_impl(const void *q, const void *codes, int64_t R, int64_t D, int64_t pitch, void *X, hipStream_t s)
 {
     const Shape g = shape_for<T>(R, D);
     unpack8_kernel<T><<<g.grid, g.block, 0, s>>>(static_cast<const int8_t *>(q), static_cast<const uint8_t *>(codes), R, D,
-                                                 ceil_div(D, kBlock8), static_cast<T *>(X));
+                                                 ceil_div(D, kBlock8), pitch, static_cast<T *>(X));
     OPMX_LAUNCH_CHECK();
     return OPMX_OK;
 }
@@ -253,12 +255,15 @@ int launch_checkpoint8_pack(const void *X, int64_t R, int64_t D, int dtype, void
     return OPMX_ERR_UNSUPPORTED;
 }
 
-int launch_checkpoint8_unpack(const void *q, const void *codes, int64_t R, int64_t D, int dtype, void *X, hipStream_t s)
+int launch_checkpoint8_unpack(const void *q, const void *codes, int64_t R, int64_t D, int dtype, void *X, hipStream_t s,
+                              int64_t pitch)
 {
+    if (R == 0 || D == 0) return OPMX_OK;
+    if (pitch == 0) pitch = D;
     switch (dtype) {
-        case OPMX_DTYPE_F32: return unpack8_impl<float>(q, codes, R, D, X, s);
-        case OPMX_DTYPE_F16: return unpack8_impl<f16>(q, codes, R, D, X, s);
-        case OPMX_DTYPE_BF16: return unpack8_impl<bf16>(q, codes, R, D, X, s);
+        case OPMX_DTYPE_F32: return unpack8_impl<float>(q, codes, R, D, pitch, X, s);
+        case OPMX_DTYPE_F16: return unpack8_impl<f16>(q, codes, R, D, pitch, X, s);
+        case OPMX_DTYPE_BF16: return unpack8_impl<bf16>(q, codes, R, D, pitch, X, s);
     }
     return OPMX_ERR_UNSUPPORTED;
 }

@@ -1,0 +1,401 @@
+// Linear with bias, activation and residual in its epilogue: Y = act(X W^T + B) + R, and its gradients
+//   dH = dY * act'(H),  dX = dH W,  dW = dH^T X,  dB = sum_t dH   (dR = dY).
+// The products run in linear_gemm.hip; here are the passes around them and the choice of tiles.
+//   pad         operands whose rows are not whole 16-byte chunks are copied to rows that are (the copy is
+//               (T + N) K values against 2 T N K operations)
+//   slope       dH from dY and the kept H in one pass, with the column sums for dB
+//   join        products with few tiles are cut along k; the fp32 sums of the ranges meet here, in order, and
+//               go through the epilogue
+// H is kept in the tensors' type: its rounding moves act'(H) by at most |act''| |H| eps / 2, no more than the
+// rounding of dH to that type, which the matrix units need anyway, moves the products.
+#include "checkpoint8.h"
+#include "linear_epilogue.h"
+
+namespace opmx {
+namespace {
+
+inline int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+// X [R, C] dense -> [R][pitch], zeros behind the C values.
+template <typename T>
+__global__ __launch_bounds__(256) void pad_kernel(const T *__restrict__ X, int64_t R, int64_t C, int64_t pitch,
+                                                  T *__restrict__ out)
+{
+    const int64_t c = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) * 8;
+    if (c >= pitch) return;
+    const int64_t step = static_cast<int64_t>(gridDim.y) * blockDim.y;
+    for (int64_t r = static_cast<int64_t>(blockIdx.y) * blockDim.y + threadIdx.y; r < R; r += step) {
+        float v[8];
+        load8(X + r * C + c, C - c, v);
+        store8(out + r * pitch + c, pitch - c, v);
+    }
+}
+
+// dH [T][pitch] (zeros behind the N values) from dY [T, ncols] and H [T, N]; sums: per row chunk (blockIdx.y) the
+// column sums [chunks][N] in fp32, before dH is rounded.  Lanes go over columns, 8 each, blockDim.y rows at a time.
+template <typename T, bool GATED>
+__global__ __launch_bounds__(256) void slope_kernel(const T *__restrict__ dY, const T *__restrict__ H, int64_t Ttok,
+                                                    int64_t N, int64_t ncols, int64_t pitch, int64_t rows_per_chunk,
+                                                    int act, T *__restrict__ dH, float *__restrict__ sums)
+{
+    __shared__ float s_sum[256 * 8 * (GATED ? 2 : 1)];
+    const int64_t c = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) * 8;
+    const int64_t left = ncols - c;
+    const int64_t r0 = static_cast<int64_t>(blockIdx.y) * rows_per_chunk;
+    const int64_t r1 = r0 + rows_per_chunk < Ttok ? r0 + rows_per_chunk : Ttok;
+    float sum[2][8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum[0][j] = sum[1][j] = 0.0f;
+    if (left > 0) {
+        for (int64_t r = r0 + threadIdx.y; r < r1; r += blockDim.y) {
+            float d[8], h[8];
+            load8(dY + r * ncols + c, left, d);
+            if (GATED) {
+                float a[8], g[8];
+                load8(H + r * N + c, left, a);
+                load8(H + r * N + ncols + c, left, g);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float s = logistic_for<T>(a[j]);
+                    h[j] = d[j] * a[j] * s;                                            // of the second half
+                    d[j] = d[j] * g[j] * (s + a[j] * s * (1.0f - s));
+                    sum[0][j] += d[j];
+                    sum[1][j] += h[j];
+                }
+                if (dH) {
+                    store8(dH + r * pitch + c, left, d);
+                    store8(dH + r * pitch + ncols + c, left < 8 ? left : pitch - ncols - c, h);
+                }
+            } else {
+                if (act != OPMX_ACTIVATION_NONE) {
+                    load8(H + r * N + c, left, h);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) d[j] *= slope<T>(act, h[j]);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    if (j >= left) d[j] = 0.0f;
+                    sum[0][j] += d[j];
+                }
+                if (dH) store8(dH + r * pitch + c, pitch - c, d);
+            }
+        }
+        if (GATED && dH && left <= 8)                    // the row's pad, by the lane of its last columns
+            for (int64_t r = r0 + threadIdx.y; r < r1; r += blockDim.y)
+                for (int64_t p = N; p < pitch; ++p) dH[r * pitch + p] = from_f32<T>(0.0f);
+    }
+    if (sums == nullptr) return;
+    const int t = threadIdx.y * blockDim.x + threadIdx.x;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        s_sum[j * 256 + t] = sum[0][j];
+        if (GATED) s_sum[(8 + j) * 256 + t] = sum[1][j];
+    }
+    __syncthreads();
+    if (threadIdx.y == 0 && left > 0) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            float a = 0.0f, b = 0.0f;
+            for (unsigned y = 0; y < blockDim.y; ++y) {
+                a += s_sum[j * 256 + y * blockDim.x + threadIdx.x];
+                if (GATED) b += s_sum[(8 + j) * 256 + y * blockDim.x + threadIdx.x];
+            }
+            if (j < left) {
+                sums[blockIdx.y * N + c + j] = a;
+                if (GATED) sums[blockIdx.y * N + ncols + c + j] = b;
+            }
+        }
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void column_sum_kernel(const float *__restrict__ sums, int64_t chunks, int64_t N,
+                                                         T *__restrict__ dB)
+{
+    const int64_t c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (c >= N) return;
+    double v = 0.0;
+#pragma unroll 8
+    for (int64_t i = 0; i < chunks; ++i) v += sums[i * N + c];
+    dB[c] = from_f32<T>(static_cast<float>(v));
+}
+
+// The fp32 sums of the k ranges, added in order, through the epilogue.
+template <typename T, bool GATED>
+__global__ __launch_bounds__(256) void join_kernel(Epilogue e, int ranges)
+{
+    const int64_t chunks = (e.ncols + 7) / 8;
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (at >= chunks * e.rows) return;
+    const int64_t m = at / chunks, c = (at - m * chunks) * 8;
+    float h[8], g[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) h[j] = g[j] = 0.0f;
+    for (int i = 0; i < ranges; ++i) {
+        const float *p = e.part + (i * e.rows + m) * e.pitch + c;
+        float v[8];
+        load8(p, 8, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) h[j] += v[j];
+        if (GATED) {
+            load8(p + e.pitch / 2, 8, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) g[j] += v[j];
+        }
+    }
+    finish8<T, GATED>(e, m, c, h, g);
+}
+
+// Tile and k ranges of a product of `rows` x `ncols` outputs (gated: ncols pairs of them) over Kc.
+struct Cut {
+    int tile, ranges;
+    int64_t pitch;      // of the ranges' sums
+    size_t bytes;       // of the ranges' sums
+};
+Cut cut_for(int64_t rows, int64_t ncols, int64_t Kc, bool gated, int dtype)
+{
+    Cut c{128, 1, 0, 0};
+    const int64_t width = gated ? 2 * ncols : ncols;
+    const int64_t t256 = ceil_div(rows, 256) * ceil_div(width, 256);
+    if (dtype != OPMX_DTYPE_F32 && t256 >= 192) c.tile = 256;
+    if (c.tile == 128) {
+        const int64_t tiles = ceil_div(rows, 128) * ceil_div(width, 128);
+        const int64_t nk = ceil_div(Kc, dtype == OPMX_DTYPE_F32 ? 32 : 64);
+        int64_t r = tiles > 0 ? 512 / tiles : 1;
+        if (r > nk / 4) r = nk / 4;
+        if (r > 32) r = 32;
+        if (r > 1) {
+            const int64_t per = ceil_div(nk, r);
+            c.ranges = static_cast<int>(ceil_div(nk, per));
+        }
+    }
+    if (c.ranges > 1) {
+        c.pitch = gated ? 2 * up(ncols, 8) : up(ncols, 8);
+        c.bytes = static_cast<size_t>(c.ranges) * rows * c.pitch * 4;
+    }
+    return c;
+}
+
+template <typename T> int join(const Epilogue &e, int ranges, hipStream_t s)
+{
+    const int64_t blocks = ceil_div(ceil_div(e.ncols, 8) * e.rows, 256);
+    if (blocks >= (int64_t{1} << 31)) return OPMX_ERR_UNSUPPORTED;
+    if (e.act == OPMX_ACTIVATION_SWIGLU) join_kernel<T, true><<<static_cast<unsigned>(blocks), 256, 0, s>>>(e, ranges);
+    else join_kernel<T, false><<<static_cast<unsigned>(blocks), 256, 0, s>>>(e, ranges);
+    OPMX_LAUNCH_CHECK();
+    return OPMX_OK;
+}
+
+template <typename T>
+int product(const Operand &P, const Operand &Q, int64_t Kc, Epilogue e, void *ws, hipStream_t s)
+{
+    const bool gated = e.act == OPMX_ACTIVATION_SWIGLU;
+    const Cut c = cut_for(e.rows, e.ncols, Kc, gated, DType<T>::id);
+    if (c.ranges > 1) {
+        e.part = static_cast<float *>(ws);
+        e.pitch = c.pitch;
+    }
+    const int rc = launch_linear_gemm(P, Q, Kc, DType<T>::id, e, c.tile, c.ranges, s);
+    return rc != OPMX_OK || c.ranges == 1 ? rc : join<T>(e, c.ranges, s);
+}
+
+struct Lanes {
+    dim3 grid, block;
+};
+// 8 columns per lane, short rows several to a block.
+inline Lanes lanes_over(int64_t rows, int64_t cols)
+{
+    int bx = 8;
+    while (bx < 256 && bx * 8 < cols) bx <<= 1;
+    const int64_t y = ceil_div(rows, 256 / bx);
+    return {dim3(static_cast<unsigned>(ceil_div(cols, bx * 8)), static_cast<unsigned>(y < 65535 ? y : 65535)),
+            dim3(bx, 256 / bx)};
+}
+
+template <typename T> int pad(const void *X, int64_t R, int64_t C, int64_t pitch, void *out, hipStream_t s)
+{
+    if (R == 0) return OPMX_OK;
+    const Lanes l = lanes_over(R, pitch);
+    pad_kernel<T><<<l.grid, l.block, 0, s>>>(static_cast<const T *>(X), R, C, pitch, static_cast<T *>(out));
+    OPMX_LAUNCH_CHECK();
+    return OPMX_OK;
+}
+
+// What the workspace holds, in this order.
+struct ForwardPlan {
+    size_t x, w, part, total;
+};
+ForwardPlan forward_plan(int64_t Ttok, int64_t K, int64_t N, int dtype, int act)
+{
+    const int64_t esize = dtype == OPMX_DTYPE_F32 ? 4 : 2, n = 16 / esize, pitch = up(K, n);
+    const bool gated = act == OPMX_ACTIVATION_SWIGLU, padded = K % n != 0;
+    ForwardPlan p{};
+    p.x = 0;
+    p.w = p.x + (padded ? up(Ttok * pitch * esize, 256) : 0);
+    p.part = p.w + (padded ? up(N * pitch * esize, 256) : 0);
+    p.total = p.part + up(cut_for(Ttok, gated ? N / 2 : N, K, gated, dtype).bytes, 256);
+    return p;
+}
+
+// Rows per chunk of the column sums: a few thousand blocks at most, 16 rows a chunk at least.
+inline int64_t chunk_rows(int64_t Ttok, int64_t ncols)
+{
+    const int64_t strips = ceil_div(ncols, 2048);
+    int64_t rows = 16;
+    while (ceil_div(Ttok, rows) * strips > 4096 || ceil_div(Ttok, rows) > 512) rows <<= 1;
+    return rows;
+}
+
+struct BackwardPlan {
+    size_t dh, x, w, sums, part, total;
+    int64_t pitch_n, pitch_k, chunk;
+    bool own_dh, padded;
+};
+BackwardPlan backward_plan(int64_t Ttok, int64_t K, int64_t N, int dtype, int act)
+{
+    const int64_t esize = dtype == OPMX_DTYPE_F32 ? 4 : 2, n = 16 / esize;
+    BackwardPlan p{};
+    p.pitch_n = up(N, n);
+    p.pitch_k = up(K, n);
+    p.padded = K % n != 0;
+    p.own_dh = act != OPMX_ACTIVATION_NONE || N % n != 0;
+    p.chunk = chunk_rows(Ttok, act == OPMX_ACTIVATION_SWIGLU ? N / 2 : N);
+    p.dh = 0;
+    p.x = p.dh + (p.own_dh ? up(Ttok * p.pitch_n * esize, 256) : 0);
+    p.w = p.x + up(Ttok * p.pitch_k * esize, 256);          // padded, or unpacked from 8 bits
+    p.sums = p.w + (p.padded ? up(N * p.pitch_k * esize, 256) : 0);
+    p.part = p.sums + up(ceil_div(Ttok, p.chunk) * N * 4, 256);
+    const size_t a = cut_for(Ttok, K, N, false, dtype).bytes, b = cut_for(N, K, Ttok, false, dtype).bytes;
+    p.total = p.part + up(a > b ? a : b, 256);
+    return p;
+}
+
+template <typename T>
+int forward_impl(const void *X, const void *W, const void *B, const void *R, int64_t Ttok, int64_t K, int64_t N, int act,
+                 void *Y, void *H, char *ws, hipStream_t s)
+{
+    constexpr int64_t n = 16 / sizeof(T);
+    const ForwardPlan plan = forward_plan(Ttok, K, N, DType<T>::id, act);
+    int64_t pitch = K;
+    if (K % n != 0) {
+        pitch = up(K, n);
+        int rc = pad<T>(X, Ttok, K, pitch, ws + plan.x, s);
+        if (rc == OPMX_OK) rc = pad<T>(W, N, K, pitch, ws + plan.w, s);
+        if (rc != OPMX_OK) return rc;
+        X = ws + plan.x;
+        W = ws + plan.w;
+    }
+    Epilogue e;
+    e.bias = B;
+    e.residual = R;
+    e.Y = Y;
+    e.H = H;
+    e.rows = Ttok;
+    e.N = N;
+    e.ncols = act == OPMX_ACTIVATION_SWIGLU ? N / 2 : N;
+    e.act = act;
+    return product<T>({W, pitch, false}, {X, pitch, false}, K, e, ws + plan.part, s);
+}
+
+template <typename T>
+int backward_impl(const void *dY, const void *X, const void *xq, const void *xcode, const void *W, const void *H,
+                  int64_t Ttok, int64_t K, int64_t N, int act, void *dX, void *dW, void *dB, char *ws, hipStream_t s)
+{
+    const BackwardPlan plan = backward_plan(Ttok, K, N, DType<T>::id, act);
+    const bool gated = act == OPMX_ACTIVATION_SWIGLU;
+    const int64_t ncols = gated ? N / 2 : N;
+    const void *dH = dY;
+    int rc = OPMX_OK;
+    const bool want_dh = plan.own_dh && (dX || dW);
+    if (Ttok > 0 && (want_dh || dB)) {
+        T *out = want_dh ? reinterpret_cast<T *>(ws + plan.dh) : nullptr;
+        float *sums = dB ? reinterpret_cast<float *>(ws + plan.sums) : nullptr;
+        Lanes l = lanes_over(plan.chunk, gated ? ncols : plan.pitch_n);
+        l.grid.y = static_cast<unsigned>(ceil_div(Ttok, plan.chunk));
+        if (gated)
+            slope_kernel<T, true><<<l.grid, l.block, 0, s>>>(static_cast<const T *>(dY), static_cast<const T *>(H), Ttok, N, ncols,
+                                                             plan.pitch_n, plan.chunk, act, out, sums);
+        else
+            slope_kernel<T, false><<<l.grid, l.block, 0, s>>>(static_cast<const T *>(dY), static_cast<const T *>(H), Ttok, N, ncols,
+                                                              plan.pitch_n, plan.chunk, act, out, sums);
+        OPMX_LAUNCH_CHECK();
+    }
+    if (plan.own_dh) dH = ws + plan.dh;
+    if (dB) {
+        column_sum_kernel<T><<<static_cast<unsigned>(ceil_div(N, 256)), 256, 0, s>>>(
+            reinterpret_cast<const float *>(ws + plan.sums), ceil_div(Ttok, plan.chunk), N, static_cast<T *>(dB));
+        OPMX_LAUNCH_CHECK();
+    }
+    Epilogue e;
+    if (dX) {
+        int64_t pitch = K;
+        if (plan.padded) {
+            pitch = plan.pitch_k;
+            rc = pad<T>(W, N, K, pitch, ws + plan.w, s);
+            if (rc != OPMX_OK) return rc;
+            W = ws + plan.w;
+        }
+        e.Y = dX;
+        e.rows = Ttok;
+        e.N = e.ncols = K;
+        rc = product<T>({W, pitch, true}, {dH, plan.pitch_n, false}, N, e, ws + plan.part, s);
+        if (rc != OPMX_OK) return rc;
+    }
+    if (dW) {
+        int64_t pitch = K;
+        if (xq) {
+            pitch = plan.pitch_k;
+            rc = launch_checkpoint8_unpack(xq, xcode, Ttok, K, DType<T>::id, ws + plan.x, s, pitch);
+            X = ws + plan.x;
+        } else if (plan.padded) {
+            pitch = plan.pitch_k;
+            rc = pad<T>(X, Ttok, K, pitch, ws + plan.x, s);
+            X = ws + plan.x;
+        }
+        if (rc != OPMX_OK) return rc;
+        e.Y = dW;
+        e.rows = N;
+        e.N = e.ncols = K;
+        rc = product<T>({X, pitch, true}, {dH, plan.pitch_n, true}, Ttok, e, ws + plan.part, s);
+    }
+    return rc;
+}
+
+}  // namespace
+
+size_t linear_epilogue_workspace_bytes(int64_t T, int64_t K, int64_t N, int dtype, int act)
+{
+    const size_t b = forward_plan(T, K, N, dtype, act).total;
+    return b > 256 ? b : 256;
+}
+size_t linear_epilogue_backward_workspace_bytes(int64_t T, int64_t K, int64_t N, int dtype, int act)
+{
+    const size_t b = backward_plan(T, K, N, dtype, act).total;
+    return b > 256 ? b : 256;
+}
+
+int launch_linear_epilogue(const void *X, const void *W, const void *B, const void *R, int64_t T, int64_t K, int64_t N,
+                           int dtype, int act, void *Y, void *H, void *ws, hipStream_t s)
+{
+    switch (dtype) {
+        case OPMX_DTYPE_F32: return forward_impl<float>(X, W, B, R, T, K, N, act, Y, H, static_cast<char *>(ws), s);
+        case OPMX_DTYPE_F16: return forward_impl<f16>(X, W, B, R, T, K, N, act, Y, H, static_cast<char *>(ws), s);
+        case OPMX_DTYPE_BF16: return forward_impl<bf16>(X, W, B, R, T, K, N, act, Y, H, static_cast<char *>(ws), s);
+    }
+    return OPMX_ERR_UNSUPPORTED;
+}
+
+int launch_linear_epilogue_backward(const void *dY, const void *X, const void *xq, const void *xcode, const void *W,
+                                    const void *H, int64_t T, int64_t K, int64_t N, int dtype, int act, void *dX, void *dW,
+                                    void *dB, void *ws, hipStream_t s)
+{
+    char *w = static_cast<char *>(ws);
+    switch (dtype) {
+        case OPMX_DTYPE_F32: return backward_impl<float>(dY, X, xq, xcode, W, H, T, K, N, act, dX, dW, dB, w, s);
+        case OPMX_DTYPE_F16: return backward_impl<f16>(dY, X, xq, xcode, W, H, T, K, N, act, dX, dW, dB, w, s);
+        case OPMX_DTYPE_BF16: return backward_impl<bf16>(dY, X, xq, xcode, W, H, T, K, N, act, dX, dW, dB, w, s);
+    }
+    return OPMX_ERR_UNSUPPORTED;
+}
+
+}  // namespace opmx

@@ -1,0 +1,357 @@
+// Tile product of the linear with epilogue, for the forward pass and both gradients (gfx950, MFMA).
+//
+//   C[m, c] = sum_k Q(m, k) P(c, k)
+//     forward      Q = X  [T,K],  P = W [N,K]:  rows of both run along k
+//     gradient X   Q = dH [T,N],  P = W [N,K] read as (c = K, k = N): k runs over rows
+//     gradient W   Q = dH [T,N],  P = X [T,K], k = T: k runs over rows in both
+//
+// A workgroup owns a BM x BN tile of C and walks k in tiles of 128 bytes (64 values, 32 in fp32), two LDS buffers,
+// loaded straight into LDS.  P is the A operand of the MFMAs and Q the B operand, so a lane ends up with four
+// neighbouring columns of a row.
+//   rows along k:     LDS [row][8 chunks of 16 bytes], chunk c in slot c ^ (row / 2 % 8): a fragment is one
+//                     16-byte read, conflict free;
+//   k along rows:     LDS [k][row], 16-bit fragments through the transposing LDS read (four k of one column per
+//                     lane and read), fp32 ones value by value.  32-byte units (fp32: 64) are permuted within
+//                     256 bytes by k so that the k rows that one read meets lie in different banks.
+// What does not exist (rows, columns, k past the end) is loaded from an offset that the descriptor's range check
+// answers with zeros.  The k order of a fragment is the same in both layouts, whatever it is.
+#include "linear_epilogue.h"
+#include "moe_gemm.h"
+
+#include <type_traits>
+
+namespace opmx {
+namespace {
+
+constexpr int kTileBytes = 128;                 // of k per row
+constexpr uint32_t kNowhere = 0x80000000u;      // past every descriptor
+#define OPMX_LDS(p) ((void __attribute__((address_space(3))) *)(p))
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t descriptor(const char *base)
+{
+    const uint64_t b = reinterpret_cast<uint64_t>(base);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(b));
+    const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(b >> 32));
+    return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void *>((static_cast<uint64_t>(hi) << 32) | lo), 0,
+                                             0x7FFFFFFF, 0x00020000);
+}
+
+template <typename T> struct Step;
+template <> struct Step<f16> {
+    using frag = half8_t;
+    static __device__ __forceinline__ float4_t mma(frag p, frag q, float4_t c) { return Mfma<f16>::m16(p, q, c); }
+};
+template <> struct Step<bf16> {
+    using frag = bf16x8_t;
+    static __device__ __forceinline__ float4_t mma(frag p, frag q, float4_t c) { return Mfma<bf16>::m16(p, q, c); }
+};
+template <> struct Step<float> {
+    using frag = float4_t;
+    static __device__ __forceinline__ float4_t mma(frag p, frag q, float4_t c)
+    {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(p[j], q[j], c, 0, 0, 0);
+        return c;
+    }
+};
+
+// How k-major rows are permuted inside a k row of LDS: the index of a unit (32 bytes; fp32: 64) is xored with this.
+template <typename T> __device__ __forceinline__ int unit_swizzle(int k)
+{
+    if constexpr (sizeof(T) == 2) return (k & 3) | ((k >> 3 & 1) << 2);
+    else return (k >> 2) & 3;
+}
+
+// One operand's share of a thread: LOADS 16-byte pieces of a k-tile of ROWS rows.
+template <typename T, int ROWS, int THREADS, bool KM, bool GATED> struct Loader {
+    static constexpr int n = 16 / sizeof(T);
+    static constexpr int LOADS = ROWS * kTileBytes / 16 / THREADS;
+    const char *base, *base2;        // of the current k-tile (GATED: of the second half's rows)
+    int64_t step;                    // to the next one
+    uint32_t off[LOADS];
+    int first_k[LOADS];              // within the tile
+
+    // Rows [row0, row0 + ROWS) of `count`.  GATED: groups of 64 tile rows are 32 rows of the first half and the 32
+    // rows of the second half (count further on) that belong to the same columns.
+    __device__ __forceinline__ void init(const Operand &o, int64_t row0, int64_t count, int64_t k0)
+    {
+        const int64_t esize = sizeof(T);
+        const char *p = static_cast<const char *>(o.p);
+        if (KM) {
+            base = p + (k0 * o.pitch + row0) * esize;
+            base2 = base;
+            step = (kTileBytes / sizeof(T)) * o.pitch * esize;
+        } else {
+            base = p + (row0 * o.pitch + k0) * esize;
+            base2 = GATED ? base + count * o.pitch * esize : base;
+            step = kTileBytes;
+        }
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int piece = i * THREADS + threadIdx.x;
+            if (KM) {
+                constexpr int per_k = ROWS / n;                  // pieces of a k row
+                constexpr int per_unit = sizeof(T) == 2 ? 2 : 4;
+                const int k = piece / per_k, c = piece % per_k;
+                const int r = (((c / per_unit) ^ unit_swizzle<T>(k)) * per_unit + c % per_unit) * n;
+                first_k[i] = k;
+                off[i] = row0 + r < count ? static_cast<uint32_t>((k * o.pitch + r) * esize) : kNowhere;
+            } else {
+                const int row = piece >> 3, c = (piece & 7) ^ ((row >> 1) & 7);
+                const int r = GATED ? (row / 64) * 32 + row % 32 : row;
+                first_k[i] = c * n;
+                off[i] = row0 + r < count ? static_cast<uint32_t>(r * o.pitch * esize + c * 16) : kNowhere;
+            }
+        }
+    }
+    // Loads piece i of the current k-tile, of which k_left values exist, to lds + its place.
+    __device__ __forceinline__ void issue(int i, char *lds, int64_t k_left) const
+    {
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+        const int piece0 = i * THREADS + wave * kWave;                       // of the wave: uniform
+        const bool second = GATED && !KM && ((piece0 >> 3) % 64) >= 32;
+        const uint32_t v = first_k[i] < k_left ? off[i] : kNowhere;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(descriptor(second ? base2 : base), OPMX_LDS(lds + piece0 * 16), 16, v, 0, 0, 0);
+    }
+    __device__ __forceinline__ void next()
+    {
+        base += step;
+        base2 += step;
+    }
+};
+
+// Eight transposing reads, waited for: four fragments of a k-major tile.  Written as one block because the compiler
+// puts a wait for every outstanding global -> LDS load in front of the builtin (it takes it for a store), and the
+// next k-tile's loads are in flight by design.  a: LDS addresses of the fragments' lanes at k step 0.
+template <int KSTEP_BYTES, int HALF_BYTES, typename F>
+__device__ __forceinline__ void transposed4(F *f, const uint32_t *a)
+{
+    typedef uint32_t pair __attribute__((ext_vector_type(2)));
+    pair v[8];
+    asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%12\n\t"
+                 "ds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
+                 "ds_read_b64_tr_b16 %2, %9 offset:%12\n\t"
+                 "ds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
+                 "ds_read_b64_tr_b16 %4, %10 offset:%12\n\t"
+                 "ds_read_b64_tr_b16 %5, %10 offset:%13\n\t"
+                 "ds_read_b64_tr_b16 %6, %11 offset:%12\n\t"
+                 "ds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7])
+                 : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "n"(KSTEP_BYTES), "n"(KSTEP_BYTES + HALF_BYTES)
+                 : "memory");
+#pragma unroll
+    for (int j = 0; j < 4; ++j) __builtin_memcpy(&f[j], &v[2 * j], 16);
+}
+
+// The fragments of N groups of 16 rows from row 16 * row16 on, k step KS (0, 1), of an LDS tile of ROWS rows.
+template <typename T, int ROWS, bool KM, int KS, int N>
+__device__ __forceinline__ void fragments(const char *lds, int row16, int lane, typename Step<T>::frag (&f)[N])
+{
+    using frag = typename Step<T>::frag;
+    const int r = lane & 15, g = lane >> 4;
+    if constexpr (!KM) {
+        const int slot = (KS * 4 + g) ^ ((r >> 1) & 7);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            f[i] = *reinterpret_cast<const frag *>(lds + ((row16 + i) * 16 + r) * kTileBytes + slot * 16);
+    } else if constexpr (sizeof(T) == 2) {
+        // lane r of a group of 16 reads four columns of k row r / 4 and receives four k rows of column r
+        static_assert(N % 4 == 0, "four fragments per block of reads");
+        const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(OPMX_LDS(lds)));
+        const int k = g * 8 + (r >> 2);             // neither the second half (k + 4) nor KS (k + 32) changes the swizzle
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            uint32_t a[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                a[j] = base + k * (ROWS * 2) + (((row16 + i + j) ^ unit_swizzle<T>(k)) << 5) + (r & 3) * 8;
+            transposed4<KS * 32 * ROWS * 2, 4 * ROWS * 2>(f + i, a);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int k = KS * 16 + g * 4 + j;
+                f[i][j] = *reinterpret_cast<const float *>(lds + k * (ROWS * 4) + (((row16 + i) ^ unit_swizzle<T>(k)) << 6) + r * 4);
+            }
+    }
+}
+
+// Tile ids to tiles.  Ids go round the 8 XCDs; each XCD takes a contiguous eighth of the tiles, in bands of 8
+// row tiles walked column by column, so that the 32 workgroups an XCD runs share 8 + 4 operand tiles in its L2.
+__device__ __forceinline__ void place(int64_t id, int64_t mt, int64_t nt, int64_t &m, int64_t &c)
+{
+    const int64_t total = mt * nt, per = total / 8, rest = total % 8;
+    const int64_t x = id % 8;
+    const int64_t t = x * per + (x < rest ? x : rest) + id / 8;
+    const int64_t band = t / (8 * nt), first = band * 8;
+    const int64_t high = mt - first < 8 ? mt - first : 8;
+    const int64_t in = t - band * 8 * nt;
+    m = first + in % high;
+    c = in / high;
+}
+
+template <typename T, int BM, int BN, int WM, int WN, bool PK, bool QK, bool GATED>
+__global__ __launch_bounds__(WM *WN *kWave) void linear_gemm_kernel(Operand P, Operand Q, int64_t Kc, Epilogue e, int64_t mt,
+                                                                    int64_t nt, int64_t ktiles_per_range)
+{
+    constexpr int THREADS = WM * WN * kWave, WTM = BM / WM, WTN = BN / WN, TM = WTM / 16, TN = WTN / 16;
+    constexpr int STAGE = (BM + BN) * kTileBytes, BK = kTileBytes / sizeof(T);
+    constexpr int BNO = GATED ? BN / 2 : BN;
+    static_assert(WTN == 64 && (TM == 4 || TM == 8), "the epilogue stages 64 x 64 pieces");
+    using frag = typename Step<T>::frag;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+
+    int64_t tm, tc;
+    place(blockIdx.x, mt, nt, tm, tc);
+    const int64_t m0 = tm * BM, c0 = tc * BNO;
+    const int64_t kt0 = blockIdx.y * ktiles_per_range;
+    const int64_t k0 = kt0 * BK;
+    const int64_t klen = Kc - k0 < ktiles_per_range * BK ? Kc - k0 : ktiles_per_range * BK;   // > 0: see the launch
+    const int nk = static_cast<int>((klen + BK - 1) / BK);
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int wm = wave / WN, wn = wave % WN;
+
+    Loader<T, BN, THREADS, PK, GATED> lp;
+    Loader<T, BM, THREADS, QK, false> lq;
+    lp.init(P, c0, e.ncols, k0);
+    lq.init(Q, m0, e.rows, k0);
+
+    float4_t acc[TN][TM];
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int i = 0; i < TM; ++i) acc[j][i] = float4_t{0.f, 0.f, 0.f, 0.f};
+
+    auto load = [&](char *stage, int64_t left) {
+#pragma unroll
+        for (int i = 0; i < lq.LOADS; ++i) lq.issue(i, stage, left);
+#pragma unroll
+        for (int i = 0; i < lp.LOADS; ++i) lp.issue(i, stage + BM * kTileBytes, left);
+        lq.next();
+        lp.next();
+    };
+    auto half = [&](const char *cur, auto ks_tag, auto h_tag, const frag (&p)[TN]) {
+        constexpr int KS = decltype(ks_tag)::value, H = decltype(h_tag)::value;
+        frag q[4];
+        fragments<T, BM, QK, KS, 4>(cur, wm * TM + H * 4, lane, q);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[j][H * 4 + i] = Step<T>::mma(p[j], q[i], acc[j][H * 4 + i]);
+    };
+    auto multiply = [&](const char *cur, auto ks_tag) {
+        frag p[TN];
+        fragments<T, BN, PK, decltype(ks_tag)::value, TN>(cur + BM * kTileBytes, wn * TN, lane, p);
+        half(cur, ks_tag, std::integral_constant<int, 0>{}, p);
+        if constexpr (TM == 8) half(cur, ks_tag, std::integral_constant<int, 1>{}, p);
+    };
+    load(smem, klen);
+    __syncthreads();                                       // waits for the loads as well
+    for (int kt = 0; kt < nk; ++kt) {
+        const char *cur = smem + (kt & 1) * STAGE;
+        if (kt + 1 < nk) load(smem + ((kt + 1) & 1) * STAGE, klen - static_cast<int64_t>(kt + 1) * BK);
+        multiply(cur, std::integral_constant<int, 0>{});
+        multiply(cur, std::integral_constant<int, 1>{});
+        __syncthreads();
+    }
+
+    // The wave's columns go through LDS in pieces of 64 x 64 fp32 values of its own (16-byte chunks xored with the
+    // row), so that a lane then has eight neighbouring columns of a row.
+    char *mine = smem + wave * (64 * 256);
+    const int r = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int piece = 0; piece < WTM / 64; ++piece) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+                *reinterpret_cast<float4_t *>(mine + (i * 16 + r) * 256 + (((j * 4 + g) ^ r) << 4)) = acc[j][piece * 4 + i];
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_wave_barrier();
+        constexpr int PER_ROW = GATED ? 4 : 8, ROWS = kWave / PER_ROW;       // lanes per row, rows per trip
+#pragma unroll 1
+        for (int t = 0; t < 64 / ROWS; ++t) {
+            const int row = t * ROWS + lane / PER_ROW, c8 = lane % PER_ROW;
+            float h[8], gate[8];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const float4_t v = *reinterpret_cast<const float4_t *>(mine + row * 256 + (((c8 * 2 + x) ^ (row & 15)) << 4));
+#pragma unroll
+                for (int y = 0; y < 4; ++y) h[x * 4 + y] = v[y];
+                if (GATED) {
+                    const float4_t u = *reinterpret_cast<const float4_t *>(mine + row * 256 + (((8 + c8 * 2 + x) ^ (row & 15)) << 4));
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) gate[x * 4 + y] = u[y];
+                }
+            }
+            const int64_t m = m0 + wm * WTM + piece * 64 + row;
+            const int64_t c = c0 + wn * (GATED ? 32 : 64) + c8 * 8;
+            if (m < e.rows && c < e.ncols) {
+                if (e.part) {
+                    // whole chunks: the pitch holds them
+                    float *at = e.part + (blockIdx.y * e.rows + m) * e.pitch + c;
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        *reinterpret_cast<float4_any *>(at + x * 4) = float4_any{h[x * 4], h[x * 4 + 1], h[x * 4 + 2], h[x * 4 + 3]};
+                        if (GATED)
+                            *reinterpret_cast<float4_any *>(at + e.pitch / 2 + x * 4) =
+                                float4_any{gate[x * 4], gate[x * 4 + 1], gate[x * 4 + 2], gate[x * 4 + 3]};
+                    }
+                } else {
+                    finish8<T, GATED>(e, m, c, h, gate);
+                }
+            }
+        }
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+template <typename T, int BM, int BN, int WM, int WN, bool PK, bool QK, bool GATED>
+int launch(const Operand &P, const Operand &Q, int64_t Kc, const Epilogue &e, int ranges, hipStream_t s)
+{
+    constexpr int BNO = GATED ? BN / 2 : BN, BK = kTileBytes / sizeof(T), SMEM = 2 * (BM + BN) * kTileBytes;
+    const int64_t mt = ceil_div(e.rows, BM), nt = ceil_div(e.ncols, BNO), nk = ceil_div(Kc, BK);
+    const int64_t per = nk > 0 ? ceil_div(nk, ranges) : 1;
+    const int64_t used = nk > 0 ? ceil_div(nk, per) : 1;    // every range holds at least one k-tile
+    if (mt * nt == 0) return OPMX_OK;
+    if (mt * nt >= (int64_t{1} << 31) || used > 65535 || (ranges > 1 && used != ranges)) return OPMX_ERR_UNSUPPORTED;
+    static std::atomic<uint64_t> done{0};
+    const void *k = reinterpret_cast<const void *>(&linear_gemm_kernel<T, BM, BN, WM, WN, PK, QK, GATED>);
+    if (!ensure_dynamic_smem(k, SMEM, done)) return OPMX_ERR_LAUNCH;
+    linear_gemm_kernel<T, BM, BN, WM, WN, PK, QK, GATED>
+        <<<dim3(static_cast<unsigned>(mt * nt), static_cast<unsigned>(used)), WM * WN * kWave, SMEM, s>>>(P, Q, Kc, e, mt, nt, per);
+    OPMX_LAUNCH_CHECK();
+    return OPMX_OK;
+}
+
+template <typename T, int BM, int BN, int WM, int WN>
+int by_layout(const Operand &P, const Operand &Q, int64_t Kc, const Epilogue &e, int ranges, hipStream_t s)
+{
+    if (e.act == OPMX_ACTIVATION_SWIGLU) return launch<T, BM, BN, WM, WN, false, false, true>(P, Q, Kc, e, ranges, s);
+    if (!P.k_major) return launch<T, BM, BN, WM, WN, false, false, false>(P, Q, Kc, e, ranges, s);
+    if (!Q.k_major) return launch<T, BM, BN, WM, WN, true, false, false>(P, Q, Kc, e, ranges, s);
+    return launch<T, BM, BN, WM, WN, true, true, false>(P, Q, Kc, e, ranges, s);
+}
+
+}  // namespace
+
+int launch_linear_gemm(const Operand &P, const Operand &Q, int64_t Kc, int dtype, const Epilogue &e, int tile, int ranges,
+                       hipStream_t s)
+{
+    switch (dtype) {
+        case OPMX_DTYPE_F32: return by_layout<float, 128, 128, 2, 2>(P, Q, Kc, e, ranges, s);
+        case OPMX_DTYPE_F16:
+            return tile == 256 ? by_layout<f16, 256, 256, 2, 4>(P, Q, Kc, e, ranges, s)
+                               : by_layout<f16, 128, 128, 2, 2>(P, Q, Kc, e, ranges, s);
+        case OPMX_DTYPE_BF16:
+            return tile == 256 ? by_layout<bf16, 256, 256, 2, 4>(P, Q, Kc, e, ranges, s)
+                               : by_layout<bf16, 128, 128, 2, 2>(P, Q, Kc, e, ranges, s);
+    }
+    return OPMX_ERR_UNSUPPORTED;
+}
+
+}  // namespace opmx

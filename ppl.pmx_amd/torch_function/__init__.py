@@ -10,6 +10,7 @@ index that the gate/up GEMM reads the tokens through, without the expanded copy)
 """
 from .Checkpoint8 import checkpoint8_pack, checkpoint8_unpack, swiglu_checkpoint8
 from .Linear import linear
+from .LinearEpilogue import linear_epilogue
 from .MoeBalanceLoss import moe_balance_loss
 from .MoeColumnParallelLinear import (moe_column_parallel_linear, moe_column_parallel_linear_indexed,
                                       moe_column_parallel_linear_swiglu)
@@ -20,7 +21,7 @@ from .RMSNorm import rms_norm, skip_rms_norm
 from .SiLU import silu
 from .SwiGLU import swiglu
 
-__all__ = ["checkpoint8_pack", "checkpoint8_unpack", "linear", "moe_balance_loss", "moe_column_parallel_linear", "moe_column_parallel_linear_indexed",
+__all__ = ["checkpoint8_pack", "checkpoint8_unpack", "linear", "linear_epilogue", "moe_balance_loss", "moe_column_parallel_linear", "moe_column_parallel_linear_indexed",
            "moe_column_parallel_linear_swiglu", "moe_reduce", "moe_route_select", "moe_route_select_index",
            "moe_row_parallel_linear", "moe_select", "moe_select_index", "rms_norm", "silu", "skip_rms_norm", "swiglu",
            "swiglu_checkpoint8"]

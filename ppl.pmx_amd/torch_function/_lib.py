@@ -19,6 +19,7 @@ ABI_VERSION = 1
 
 F32, F16, BF16 = 0, 1, 2
 EPILOGUE_NONE, EPILOGUE_SWIGLU = 0, 1
+ACTIVATIONS = {"none": 0, "silu": 1, "gelu": 2, "gelu_tanh": 3, "swiglu": 4}
 MAX_EXPERTS, MAX_EXPERTS_PER_TOKEN = 256, 32
 SELECT_STATIC_SCRATCH_BYTES = 4 << 20
 
@@ -53,6 +54,11 @@ _SIGNATURES = {
     "opmx_checkpoint8_unpack": (_int, [_vp, _vp, _i64, _i64, _int, _vp, _vp]),
     "opmx_swiglu_checkpoint8": (_int, [_vp, _i64, _i64, _f, _int, _vp, _vp, _vp, _vp]),
     "opmx_swiglu_checkpoint8_backward": (_int, [_vp, _vp, _vp, _i64, _i64, _f, _int, _vp, _vp]),
+    "opmx_linear_epilogue_workspace_bytes": (_sz, [_i64, _i64, _i64, _int, _int]),
+    "opmx_linear_epilogue": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _int, _vp, _vp, _vp, _sz, _vp]),
+    "opmx_linear_epilogue_backward_workspace_bytes": (_sz, [_i64, _i64, _i64, _int, _int]),
+    "opmx_linear_epilogue_backward": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _int, _vp, _vp, _vp,
+                                             _vp, _sz, _vp]),
     "opmx_moe_balance_loss_workspace_bytes": (_sz, [_i64, _int]),
     "opmx_moe_balance_loss": (_int, [_vp, _vp, _i64, _int, _int, _int, _vp, _vp, _vp, _vp, _sz, _vp]),
     "opmx_moe_balance_loss_backward": (_int, [_vp, _vp, _vp, _vp, _i64, _int, _int, _vp, _vp]),

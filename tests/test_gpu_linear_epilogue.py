@@ -1,0 +1,272 @@
+"""GPU: the linear with bias, activation and residual in its epilogue, and its gradients, against the 64-bit oracle.
+
+Tolerances, u = eps / 2 of the type, f = 2^-24.
+  A sum of n products in fp32: every addition rounds by at most f times the partial sum.  Partial sums of random signs
+  grow like the root of their number, so the root mean square of the total is f sqrt(n) / 2.4 times the root of the
+  sum of squares q of the products; 4 f (8 + sqrt(n)) q is about ten of those.
+  Y: that times the largest slope of the activation, its own arithmetic (8 + 2 |exponent|) f, and one rounding u.
+  dH: H is kept with a rounding u, which moves act'(H) by u |H| max |act''| (1/2 silu, 0.8 gelu), and dH is rounded by u
+  (not in float32, whose u is f).  These errors are independent from value to value: their part of dX and dW is four
+  times the root of their sum of squares with each at its bound (about seven standard deviations)."""
+import pytest
+import torch
+
+from _util import dev
+from oracle import train_oracle as O
+
+pytestmark = pytest.mark.gpu
+DTYPES = [torch.float16, torch.bfloat16, torch.float32]
+ACTS = ["none", "silu", "gelu", "gelu_tanh", "swiglu"]
+CURVE = {"none": 0.0, "silu": 0.5, "gelu": 0.8, "gelu_tanh": 0.85}
+F = 2.0 ** -24
+
+
+def opmx():
+    import torch_function as OPMX
+    return OPMX
+
+
+def tensors(T, K, N, dtype, act, bias, residual, seed=0):
+    g = torch.Generator().manual_seed(seed + T * 7 + K * 3 + N)
+    r = lambda *s: torch.randn(*s, generator=g)
+    M = N // 2 if act == "swiglu" else N
+    X = r(T, K)
+    X[:, ::11] *= 4
+    return (X.to(dtype), (r(N, K) / K ** 0.5).to(dtype), r(N).to(dtype) if bias else None,
+            r(T, M).to(dtype) if residual else None, r(T, M).to(dtype))
+
+
+def allow(got, ref, tol, what):
+    got, ref = got.detach().double().cpu(), ref.double()
+    assert got.shape == ref.shape, (what, got.shape, ref.shape)
+    bad = ~((got - ref).abs() <= tol)
+    assert not bool(bad.any()), "{}: {} of {} off, worst {:.3e} where {:.3e} is allowed, at {}".format(
+        what, int(bad.sum()), bad.numel(), float((got - ref).abs()[bad].max()), float(tol.expand_as(bad)[bad].min()),
+        bad.nonzero()[0].tolist())
+
+
+def sum_error(A, B, n):
+    """Of fp32 sums over n of products of A [m, n] and B [n, c]."""
+    return 4 * F * (8 + n ** 0.5) * ((A.double() ** 2) @ (B.double() ** 2)).sqrt()
+
+
+def forward_tolerance(X, W, B, R, H, Y, act, dtype):
+    u = torch.finfo(dtype).eps / 2
+    eh = sum_error(X, W.t(), X.shape[1]) + (0 if B is None else 4 * F * B.double().abs())
+    own = 8 + 4 * H.abs()
+    if act == "swiglu":
+        a, g = H.chunk(2, -1)
+        ea, eg = eh.chunk(2, -1)
+        e = 1.1 * ea * g.abs() + eg * (a * O.logistic(a)).abs() + F * own.chunk(2, -1)[0] * (g * a * O.logistic(a)).abs()
+    else:
+        exponent = 1.6 * (H.abs() + 0.045 * H.abs() ** 3) if act == "gelu_tanh" else H.abs() + H ** 2 / 2
+        e = 1.2 * eh + (0 if act == "none" else F * (16 + 4 * exponent) * O.act(H, act)[0].abs())
+    tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    return e + (u + 2 * F) * Y.abs() + (0 if R is None else F * R.double().abs()) + tiny
+
+
+def backward_tolerances(Xh, W, H, dY, act, dtype, ref):
+    u = torch.finfo(dtype).eps / 2
+    d = dY.double().abs()
+    K, N, T = W.shape[1], W.shape[0], Xh.shape[0]
+    eh = sum_error(Xh, W.t(), K)                 # H itself is a sum
+    if act == "swiglu":
+        a, g = H.chunk(2, -1)
+        ra, rg = (u * a.abs() + eh.chunk(2, -1)[0]), (u * g.abs() + eh.chunk(2, -1)[1])
+        arith = F * (16 + 4 * a.abs())
+        e = torch.cat([d * (1.1 * rg + 0.5 * g.abs() * ra + arith * g.abs() * (1 + a.abs())),
+                       d * (1.1 * ra + arith * a.abs())], -1)
+    else:
+        arith = 0 if act == "none" else F * (16 + 4 * H.abs()) * (1 + H.abs())
+        e = d * (CURVE[act] * (u * H.abs() + eh) + arith)
+    dH = torch.cat([f * dY.double() for f in O.act(H, act)[1]], -1)
+    tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    ew = e + (0 if act == "none" else u * dH.abs() + tiny)      # rounded, too
+    rss = lambda A, B: 4 * ((A.double() ** 2) @ (B.double() ** 2)).sqrt()
+    dX, dW, dB = ref
+    return (u * 1.01 * dX.abs() + rss(ew, W) + sum_error(dH, W, N) + tiny,
+            u * 1.01 * dW.abs() + rss(ew.t(), Xh) + sum_error(dH.t(), Xh, T) + tiny,
+            u * 1.01 * dB.abs() + 4 * (e ** 2).sum(0).sqrt() + 4 * F * (8 + T ** 0.5) * (dH ** 2).sum(0).sqrt() + tiny)
+
+
+def check(T, K, N, dtype, act, bias=True, residual=True, train=True, checkpoint8=False, seed=0):
+    OPMX = opmx()
+    X, W, B, R, dY = tensors(T, K, N, dtype, act, bias, residual, seed)
+    leaves = [None if t is None else t.to(dev()).requires_grad_(train) for t in (X, W, B, R)]
+    Y = OPMX.linear_epilogue(*leaves, K, N, act, checkpoint8=checkpoint8)
+    Yr, H = O.linear_epilogue(X, W, B, R, act)
+    assert Y.dtype == dtype
+    allow(Y, Yr, forward_tolerance(X, W, B, R, H, Yr, act, dtype), "Y")
+    if not train:
+        return
+    wanted = [t for t in leaves if t is not None]
+    grads = dict(zip([i for i in range(4) if leaves[i] is not None], torch.autograd.grad(Y, wanted, dY.to(dev()))))
+    Xh = O.held8(X) if checkpoint8 else X
+    ref = O.linear_epilogue_backward(Xh, W, H, dY, act)
+    tols = backward_tolerances(X, W, H, dY, act, dtype, ref)
+    for i, what in ((0, "dX"), (1, "dW"), (2, "dB")):
+        if i in grads:
+            allow(grads[i], ref[i], tols[i], what)
+    if residual:
+        assert torch.equal(grads[3].cpu(), dY)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("T,K,N", [(1, 64, 64), (1, 256, 512), (3, 100, 36), (7, 33, 10), (64, 200, 130), (130, 129, 258)])
+def test_small_and_ragged(dtype, act, T, K, N):
+    check(T, K, N, dtype, act)
+    check(T, K, N, dtype, act, bias=False, residual=False, checkpoint8=True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("T,K,N", [(1, 4096, 512), (2, 1000, 1024), (16, 2048, 96), (17, 777, 514), (33, 2816, 1024),
+                                   (300, 1024, 2816), (513, 1001, 834)])
+def test_few_rows_and_long_sums(dtype, act, T, K, N):
+    check(T, K, N, dtype, act, train=T not in (1, 16))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("act,T,K,N", [("none", 3600, 136, 3400), ("swiglu", 3333, 200, 3600), ("gelu", 3500, 77, 3335)])
+def test_large_tiles(dtype, act, T, K, N):
+    check(T, K, N, dtype, act, checkpoint8=act == "swiglu")
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_large_tiles_in_both_gradients(dtype):
+    check(200, 3500, 3600, dtype, "silu")        # dW [3600, 3500]: k is the 200 rows
+    check(3500, 3600, 200, dtype, "none")        # dX [3500, 3600]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_only_what_is_asked_for(dtype):
+    OPMX = opmx()
+    X, W, B, R, dY = [t.to(dev()) for t in tensors(40, 72, 56, dtype, "silu", True, True)]
+    full = [t.clone().requires_grad_(True) for t in (X, W, B, R)]
+    want = torch.autograd.grad(OPMX.linear_epilogue(*full, 72, 56, "silu"), full, dY)
+    for i in range(4):
+        some = [t.clone().requires_grad_(i == j) for j, t in enumerate((X, W, B, R))]
+        got, = torch.autograd.grad(OPMX.linear_epilogue(*some, 72, 56, "silu"), some[i], dY)
+        assert torch.equal(got, want[i]), i
+    with torch.no_grad():
+        Y = OPMX.linear_epilogue(*full, 72, 56, "silu")
+    assert not Y.requires_grad and torch.equal(Y, OPMX.linear_epilogue(X, W, B, R, 72, 56, "silu"))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_empty_batches(dtype):
+    OPMX = opmx()
+    W = torch.randn(24, 16, device=dev()).to(dtype).requires_grad_(True)
+    B = torch.randn(24, device=dev()).to(dtype).requires_grad_(True)
+    for act, M in (("gelu", 24), ("swiglu", 12)):
+        X = torch.empty(0, 16, device=dev(), dtype=dtype, requires_grad=True)
+        Y = OPMX.linear_epilogue(X, W, B, None, 16, 24, act)
+        dX, dW, dB = torch.autograd.grad(Y, (X, W, B), torch.empty(0, M, device=dev(), dtype=dtype))
+        assert Y.shape == (0, M) and dX.shape == (0, 16) and not bool(dW.any()) and not bool(dB.any())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("K,N", [(64, 64), (61, 35)])
+def test_strides_views_and_leading_dimensions(dtype, K, N):
+    """Transposed operands, rows that start at odd addresses, an expanded gradient, batches of more dimensions."""
+    OPMX = opmx()
+    X, W, B, R, dY = tensors(12, K, N, dtype, "silu", True, True)
+    want = None
+    for form in range(3):
+        if form == 0:
+            lx, lw, lb, lr = [t.to(dev()).requires_grad_(True) for t in (X, W, B, R)]
+            x, w, b, r = lx, lw, lb, lr
+        elif form == 1:
+            lx, lw, lb, lr = [t.to(dev()) for t in (X.t().contiguous(), W.t().contiguous(), B, R.t().contiguous())]
+            for t in (lx, lw, lb, lr):
+                t.requires_grad_(True)
+            x, w, b, r = lx.t(), lw.t(), lb, lr.t()
+        else:
+            off = lambda t: torch.cat([t.new_zeros(1), t.flatten()]).to(dev())[1:].view(t.shape)
+            x, w, b, r = [off(t).requires_grad_(True) for t in (X, W, B, R)]
+        Y = OPMX.linear_epilogue(x.view(3, 4, K) if form != 1 else x, w, b, r.view(3, 4, N) if form != 1 else r, K, N, "silu")
+        g = torch.autograd.grad(Y, (x, w, b, r), torch.ones((), device=dev(), dtype=dtype).expand_as(Y))
+        Y = Y.reshape(12, N)
+        if want is None:
+            want = (Y, g)
+        else:
+            assert torch.equal(Y, want[0]) and all(torch.equal(p, q) for p, q in zip(g, want[1])), form
+
+
+def test_infinities_stay_in_their_rows():
+    """Rows and columns do not leak into others, nor what lies behind the tensors' ends into a tile."""
+    OPMX = opmx()
+    for dtype in DTYPES:
+        for K in (72, 70):
+            X, W, B, R, dY = [t.to(dev()) for t in tensors(70, K, 90, dtype, "none", True, True)]
+            clean = OPMX.linear_epilogue(X, W, B, R, K, 90)
+            Xb, Wb = X.clone(), W.clone()
+            Xb[5, 3] = float("inf")
+            Wb[11, 7] = float("nan")
+            Y = OPMX.linear_epilogue(Xb, Wb, B, R, K, 90)
+            keep = torch.ones_like(Y, dtype=torch.bool)
+            keep[5], keep[:, 11] = False, False
+            assert torch.equal(Y[keep], clean[keep]) and not bool(torch.isfinite(Y[~keep]).any())
+
+
+def test_difference_quotients_in_float32():
+    OPMX = opmx()
+    X, W, B, R, dY = tensors(6, 20, 12, torch.float32, "swiglu", True, True)
+    lx, lw, lb = [t.to(dev()).requires_grad_(True) for t in (X, W, B)]
+    Y = OPMX.linear_epilogue(lx, lw, lb, R.to(dev()), 20, 12, "swiglu")
+    g = torch.autograd.grad(Y, (lx, lw, lb), dY.to(dev()))
+    f = lambda x, w, b: float((O.linear_epilogue(x, w, b, R, "swiglu")[0] * dY.double()).sum())
+    h = 1e-5
+    for which, idx in ((0, (2, 3)), (0, (5, 19)), (1, (0, 0)), (1, (11, 7)), (2, (4,)), (2, (9,))):
+        args = [X.double(), W.double(), B.double()]
+        plus, minus = [a.clone() for a in args], [a.clone() for a in args]
+        plus[which][idx] += h
+        minus[which][idx] -= h
+        d = (f(*plus) - f(*minus)) / (2 * h)
+        assert abs(float(g[which][idx]) - d) <= 1e-4 * (1 + abs(d))
+
+
+def test_a_change_in_place_is_noticed():
+    OPMX = opmx()
+    X = torch.randn(8, 16, device=dev())
+    W = torch.randn(16, 16, device=dev(), requires_grad=True)
+    Y = OPMX.linear_epilogue(X, W, None, None, 16, 16, "silu")
+    X.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        Y.sum().backward()
+    Y = OPMX.linear_epilogue(X, W, None, None, 16, 16, "silu", checkpoint8=True)
+    X.add_(1.0)                                                      # only its 8 bits are used
+    Y.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("T,K,N", [(5, 128, 256), (200, 1001, 514)])
+def test_captured_step_replays(dtype, T, K, N):
+    """Two graphs of a training step, replayed in turn over new inputs with eager work in between: the same bits."""
+    OPMX = opmx()
+    X, W, B, R, dY = [t.to(dev()).requires_grad_(True) for t in tensors(T, K, N, dtype, "swiglu", True, True)]
+    dY = dY.detach()
+
+    def step():
+        Y = OPMX.linear_epilogue(X, W, B, R, K, N, "swiglu", checkpoint8=True)
+        return [Y.detach(), *torch.autograd.grad(Y, (X, W, B), dY)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        graphs.append((graph, out))
+    for i in range(4):
+        with torch.no_grad():
+            X.copy_(torch.randn(T, K, device=dev()))
+        graph, out = graphs[i % 2]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, step())), i

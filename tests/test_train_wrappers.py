@@ -15,7 +15,8 @@ def test_no_cpu_path():
     for call in (lambda: OPMX.checkpoint8_pack(x), lambda: OPMX.swiglu_checkpoint8(x),
                  lambda: OPMX.checkpoint8_unpack(torch.zeros(4, 16, dtype=torch.int8),
                                                  torch.zeros(4, 1, dtype=torch.uint8), torch.float32),
-                 lambda: OPMX.moe_balance_loss(x, 16, 2)):
+                 lambda: OPMX.moe_balance_loss(x, 16, 2),
+                 lambda: OPMX.linear_epilogue(x, torch.randn(8, 16), None, None, 16, 8)):
         with pytest.raises(RuntimeError, match="no CPU path"):
             call()
 
@@ -25,6 +26,8 @@ def test_public_names_and_signatures():
     sig = lambda f: list(inspect.signature(f).parameters)
     assert sig(OPMX.swiglu_checkpoint8) == ["X", "beta"]
     assert sig(OPMX.checkpoint8_pack) == ["X"] and sig(OPMX.checkpoint8_unpack) == ["q", "code", "dtype"]
+    assert sig(OPMX.linear_epilogue) == ["X", "W", "B", "residual", "in_features", "out_features", "activation",
+                                         "checkpoint8"]
     assert sig(OPMX.moe_balance_loss) == ["scores", "num_experts", "num_experts_per_token", "token_mask"]
 
 
@@ -76,6 +79,36 @@ def test_balance_loss_c_interface():
     assert back(None, None, None, 0, 8, 1, None) == 0
 
 
+def test_linear_epilogue_c_interface():
+    L = _lib.lib()
+    odd = ctypes.c_void_p(258)
+    need = L.opmx_linear_epilogue_workspace_bytes(64, 4000, 512, 1, 0)
+    assert need % 256 == 0 and need > 256            # cut along k
+
+    def call(X=ONE, W=ONE, T=64, K=4000, N=512, dtype=1, act=0, Y=ONE, ws=ONE, bytes_=need):
+        return L.opmx_linear_epilogue(X, W, None, None, T, K, N, dtype, act, Y, None, ws, bytes_, None)
+
+    assert call(T=-1) == -1 and call(K=-1) == -1 and call(K=0) == -1 and call(act=5) == -1 and call(act=-1) == -1
+    assert call(N=511, act=4) == -1 and call(X=None) == -1 and call(W=None) == -1 and call(Y=None) == -1
+    assert call(dtype=3) == -2 and call(K=1 << 21) == -2 and call(N=1 << 21) == -2 and call(T=1 << 31) == -2
+    assert call(X=odd) == -4 and call(W=odd) == -4 and call(ws=ctypes.c_void_p(128)) == -4
+    assert call(ws=None) == -3 and call(bytes_=need - 1) == -3
+    assert call(None, None, 0, 4000, 512, 1, 0, None, None, 0) == 0
+    need = L.opmx_linear_epilogue_backward_workspace_bytes(64, 4000, 512, 1, 1)
+
+    def back(dY=ONE, X=ONE, q=None, code=None, W=ONE, H=ONE, T=64, K=4000, N=512, dtype=1, act=1, dX=ONE, dW=ONE, dB=ONE,
+             ws=ONE, bytes_=need):
+        return L.opmx_linear_epilogue_backward(dY, X, q, code, W, H, T, K, N, dtype, act, dX, dW, dB, ws, bytes_, None)
+
+    assert back(T=-1) == -1 and back(K=0) == -1 and back(N=0) == -1 and back(act=9) == -1 and back(N=511, act=4) == -1
+    assert back(dtype=9) == -2 and back(K=1 << 21) == -2
+    assert back(dY=None) == -1 and back(H=None) == -1 and back(W=None) == -1 and back(X=None) == -1
+    assert back(q=ONE) == -1 and back(code=ONE) == -1 and back(X=None, q=ONE) == -1
+    assert back(X=odd) == -4 and back(W=odd) == -4 and back(dY=odd, act=0) == -4
+    assert back(ws=None) == -3 and back(bytes_=need - 1) == -3 and back(ws=ctypes.c_void_p(257)) == -4
+    assert back(dX=None, dW=None, dB=None) == 0
+
+
 @pytest.mark.gpu
 def test_package_refusals():
     d = torch.device("cuda:0")
@@ -101,6 +134,16 @@ def test_package_refusals():
         OPMX.moe_balance_loss(x.double(), 15, 2)
     with pytest.raises(RuntimeError, match="no CPU path"):
         OPMX.moe_balance_loss(x, 15, 2, torch.ones(4, dtype=torch.bool))
+    W, lin = torch.randn(6, 15, device=d), OPMX.linear_epilogue
+    for a in ((x, W, None, None, 14, 6), (x, W, None, None, 15, 5), (x[:, :14], W, None, None, 15, 6),
+              (x, W, W[0], None, 15, 6), (x, W, None, x, 15, 6), (x, W, None, None, 15, 6, "relu"),
+              (x, W[:5], None, None, 15, 5, "swiglu"), (x, W, None, torch.zeros(6, device=d), 15, 6)):
+        with pytest.raises(ValueError):
+            lin(*a)
+    for a in ((x.half(), W, None, None, 15, 6), (x, W, W[:, 0].half().contiguous(), None, 15, 6),
+              (x.double(), W.double(), None, None, 15, 6)):
+        with pytest.raises(TypeError):
+            lin(*a)
     leaf = x[:, :14].clone().requires_grad_(True)
     y = OPMX.swiglu_checkpoint8(leaf)
     g, = torch.autograd.grad(y, leaf, torch.ones_like(y).requires_grad_(True), create_graph=True)
