@@ -278,7 +278,8 @@ int opmx_swiglu_checkpoint8_backward(const void *dY, const int8_t *q, const uint
  * Linear.forward torch_function/Linear.py:25-33, and SiLU, GELU, SwiGLU as operators of their own):
  *   H = X W^T + B,  Y = act(H) + R         sums and epilogue in fp32, one rounding
  * X [T,K], W [N,K], B [N] or NULL, R (residual) [T,M] or NULL, Y [T,M]; M = N, or N/2 with OPMX_ACTIVATION_SWIGLU.
- * H: NULL, or [T,N], receives H rounded to dtype for the backward pass.
+ * H: NULL, or opmx_linear_epilogue_kept_bytes() bytes, 16-byte aligned, that receive H for the backward pass: in float32 as
+ * it is, otherwise 24 bits of it (4 or 3 bytes per value; the layout is the library's).
  * backward: from dY [T,M]
  *   dH = dY * act'(H) (rounded to dtype),  dX = dH W [T,K],  dW = dH^T X [N,K],  dB = sum_t dH [N] (summed unrounded)
  * each of dX, dW, dB may be NULL (not wanted).  dX needs W; dW needs X, or its 8-bit form x_q, x_code (see
@@ -287,6 +288,7 @@ int opmx_swiglu_checkpoint8_backward(const void *dY, const int8_t *q, const uint
  * (OPMX_ERR_ALIGNMENT otherwise), the others anywhere their type allows.
  * workspace: opmx_linear_epilogue[_backward]_workspace_bytes(), 256-byte aligned, contents arbitrary, not shared with
  * a call running at the same time.  Results do not vary from call to call.  K < 2^21. */
+size_t opmx_linear_epilogue_kept_bytes(int64_t T, int64_t N, int dtype);
 size_t opmx_linear_epilogue_workspace_bytes(int64_t T, int64_t K, int64_t N, int dtype, int activation);
 int opmx_linear_epilogue(const void *X, const void *W, const void *B, const void *R, int64_t T, int64_t K, int64_t N,
                          int dtype, int activation, void *Y, void *H, void *workspace, size_t workspace_bytes, void *stream);

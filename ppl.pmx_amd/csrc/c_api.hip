@@ -397,6 +397,12 @@ static bool linear_sizes_ok(int64_t T, int64_t K, int64_t N)
     return K < most && N < most && T < rows;
 }
 
+size_t opmx_linear_epilogue_kept_bytes(int64_t T, int64_t N, int dtype)
+{
+    if (T <= 0 || N <= 0 || !dtype_ok(dtype)) return 0;
+    return static_cast<size_t>(T) * static_cast<size_t>(N) * (dtype == OPMX_DTYPE_F32 ? 4 : 3);
+}
+
 size_t opmx_linear_epilogue_workspace_bytes(int64_t T, int64_t K, int64_t N, int dtype, int activation)
 {
     if (T <= 0 || K <= 0 || N <= 0 || !dtype_ok(dtype) || !linear_sizes_ok(T, K, N)) return 256;
@@ -413,6 +419,7 @@ int opmx_linear_epilogue(const void *X, const void *W, const void *B, const void
     if (T == 0 || N == 0) return OPMX_OK;
     if (!X || !W || !Y || K == 0) return OPMX_ERR_BAD_ARGUMENT;
     if (K * static_cast<int64_t>(elt(dtype)) % 16 == 0 && !(aligned16(X) && aligned16(W))) return OPMX_ERR_ALIGNMENT;
+    if (H && !aligned16(H)) return OPMX_ERR_ALIGNMENT;
     const size_t need = linear_epilogue_workspace_bytes(T, K, N, dtype, activation);
     if (need > 256 && (!workspace || workspace_bytes < need)) return OPMX_ERR_WORKSPACE;
     if (workspace && (reinterpret_cast<uintptr_t>(workspace) & 255u)) return OPMX_ERR_ALIGNMENT;
@@ -443,6 +450,7 @@ int opmx_linear_epilogue_backward(const void *dY, const void *X, const int8_t *x
     const int64_t size = static_cast<int64_t>(elt(dtype));
     if (K * size % 16 == 0 && ((dX && !aligned16(W)) || (dW && !x_q && !aligned16(X)))) return OPMX_ERR_ALIGNMENT;
     if (activation == OPMX_ACTIVATION_NONE && N * size % 16 == 0 && !aligned16(dY)) return OPMX_ERR_ALIGNMENT;
+    if (H && !aligned16(H)) return OPMX_ERR_ALIGNMENT;
     const size_t need = linear_epilogue_backward_workspace_bytes(T, K, N, dtype, activation);
     if (need > 256 && (!workspace || workspace_bytes < need)) return OPMX_ERR_WORKSPACE;
     if (workspace && (reinterpret_cast<uintptr_t>(workspace) & 255u)) return OPMX_ERR_ALIGNMENT;

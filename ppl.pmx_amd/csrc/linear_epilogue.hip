@@ -6,8 +6,7 @@
 //   slope       dH from dY and the kept H in one pass, with the column sums for dB
 //   join        products with few tiles are cut along k; the fp32 sums of the ranges meet here, in order, and
 //               go through the epilogue
-// H is kept in the tensors' type: its rounding moves act'(H) by at most |act''| |H| eps / 2, no more than the
-// rounding of dH to that type, which the matrix units need anyway, moves the products.
+// dH is rounded to the tensors' type for the matrix units; H is kept with 16 bits of mantissa (keep8).
 #include "checkpoint8.h"
 #include "linear_epilogue.h"
 
@@ -34,7 +33,7 @@ __global__ __launch_bounds__(256) void pad_kernel(const T *__restrict__ X, int64
 // dH [T][pitch] (zeros behind the N values) from dY [T, ncols] and H [T, N]; sums: per row chunk (blockIdx.y) the
 // column sums [chunks][N] in fp32, before dH is rounded.  Lanes go over columns, 8 each, blockDim.y rows at a time.
 template <typename T, bool GATED>
-__global__ __launch_bounds__(256) void slope_kernel(const T *__restrict__ dY, const T *__restrict__ H, int64_t Ttok,
+__global__ __launch_bounds__(256) void slope_kernel(const T *__restrict__ dY, const void *__restrict__ H, int64_t Ttok,
                                                     int64_t N, int64_t ncols, int64_t pitch, int64_t rows_per_chunk,
                                                     int act, T *__restrict__ dH, float *__restrict__ sums)
 {
@@ -52,8 +51,8 @@ __global__ __launch_bounds__(256) void slope_kernel(const T *__restrict__ dY, co
             load8(dY + r * ncols + c, left, d);
             if (GATED) {
                 float a[8], g[8];
-                load8(H + r * N + c, left, a);
-                load8(H + r * N + ncols + c, left, g);
+                kept8<T>(H, Ttok * N, r * N + c, left, a);
+                kept8<T>(H, Ttok * N, r * N + ncols + c, left, g);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const float s = logistic_for<T>(a[j]);
@@ -68,7 +67,7 @@ __global__ __launch_bounds__(256) void slope_kernel(const T *__restrict__ dY, co
                 }
             } else {
                 if (act != OPMX_ACTIVATION_NONE) {
-                    load8(H + r * N + c, left, h);
+                    kept8<T>(H, Ttok * N, r * N + c, left, h);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) d[j] *= slope<T>(act, h[j]);
                 }
@@ -313,10 +312,10 @@ int backward_impl(const void *dY, const void *X, const void *xq, const void *xco
         Lanes l = lanes_over(plan.chunk, gated ? ncols : plan.pitch_n);
         l.grid.y = static_cast<unsigned>(ceil_div(Ttok, plan.chunk));
         if (gated)
-            slope_kernel<T, true><<<l.grid, l.block, 0, s>>>(static_cast<const T *>(dY), static_cast<const T *>(H), Ttok, N, ncols,
+            slope_kernel<T, true><<<l.grid, l.block, 0, s>>>(static_cast<const T *>(dY), H, Ttok, N, ncols,
                                                              plan.pitch_n, plan.chunk, act, out, sums);
         else
-            slope_kernel<T, false><<<l.grid, l.block, 0, s>>>(static_cast<const T *>(dY), static_cast<const T *>(H), Ttok, N, ncols,
+            slope_kernel<T, false><<<l.grid, l.block, 0, s>>>(static_cast<const T *>(dY), H, Ttok, N, ncols,
                                                               plan.pitch_n, plan.chunk, act, out, sums);
         OPMX_LAUNCH_CHECK();
     }

@@ -47,7 +47,7 @@ class LinearEpilogue(torch.autograd.Function):
             Bc = None if B is None else B.detach().contiguous()
             Rc = None if residual is None else residual.detach().contiguous()
             Y = torch.empty(*lead, M, dtype=W.dtype, device=dev)
-            H = torch.empty(T, N, dtype=W.dtype, device=dev) if keep_h else None
+            H = torch.empty(L.opmx_linear_epilogue_kept_bytes(T, N, dt), dtype=torch.uint8, device=dev) if keep_h else None
             nbytes = L.opmx_linear_epilogue_workspace_bytes(T, K, N, dt, act)
             ws = _lib.workspace(nbytes, dev) if nbytes > 256 else None
             _lib.check(L.opmx_linear_epilogue(_lib.ptr(Xc), _lib.ptr(Wc), _lib.ptr(Bc), _lib.ptr(Rc), T, K, N, dt, act,
@@ -94,7 +94,7 @@ def linear_epilogue(X: torch.Tensor, W: torch.Tensor, B: torch.Tensor, residual:
 
     X [*, in_features], W [out_features, in_features], B [out_features] or None; ``activation`` is none, silu, gelu,
     gelu_tanh or swiglu (as ``swiglu``: first half the gated one, output and residual [*, out_features / 2]).
-    Differentiable in X, W, B and residual.  Where an activation needs it, X W^T + B is kept for the backward pass in
-    the tensors' dtype.  ``checkpoint8`` keeps X for the gradient of W in 8 bits (``checkpoint8_pack``) instead of
+    Differentiable in X, W, B and residual.  Where an activation needs it, X W^T + B is kept for the backward pass, in
+    4 bytes per value for float32 and in 3 for the 16-bit types.  ``checkpoint8`` keeps X for the gradient of W in 8 bits (``checkpoint8_pack``) instead of
     as it is; the other gradients do not change."""
     return LinearEpilogue.apply(X, W, B, residual, in_features, out_features, activation, bool(checkpoint8))

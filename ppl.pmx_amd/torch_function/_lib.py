@@ -54,6 +54,7 @@ _SIGNATURES = {
     "opmx_checkpoint8_unpack": (_int, [_vp, _vp, _i64, _i64, _int, _vp, _vp]),
     "opmx_swiglu_checkpoint8": (_int, [_vp, _i64, _i64, _f, _int, _vp, _vp, _vp, _vp]),
     "opmx_swiglu_checkpoint8_backward": (_int, [_vp, _vp, _vp, _i64, _i64, _f, _int, _vp, _vp]),
+    "opmx_linear_epilogue_kept_bytes": (_sz, [_i64, _i64, _int]),
     "opmx_linear_epilogue_workspace_bytes": (_sz, [_i64, _i64, _i64, _int, _int]),
     "opmx_linear_epilogue": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _int, _vp, _vp, _vp, _sz, _vp]),
     "opmx_linear_epilogue_backward_workspace_bytes": (_sz, [_i64, _i64, _i64, _int, _int]),

@@ -5,8 +5,8 @@ Tolerances, u = eps / 2 of the type, f = 2^-24.
   grow like the root of their number, so the root mean square of the total is f sqrt(n) / 2.4 times the root of the
   sum of squares q of the products; 4 f (8 + sqrt(n)) q is about ten of those.
   Y: that times the largest slope of the activation, its own arithmetic (8 + 2 |exponent|) f, and one rounding u.
-  dH: H is kept with a rounding u, which moves act'(H) by u |H| max |act''| (1/2 silu, 0.8 gelu), and dH is rounded by u
-  (not in float32, whose u is f).  These errors are independent from value to value: their part of dX and dW is four
+  dH: H is kept in 24 bits (float32: 32), a rounding v = 2^-16 (f) that moves act'(H) by v |H| max |act''| (1/2 silu,
+  0.8 gelu), and dH is rounded by u.  These errors are independent from value to value: their part of dX and dW is four
   times the root of their sum of squares with each at its bound (about seven standard deviations)."""
 import pytest
 import torch
@@ -67,18 +67,19 @@ def forward_tolerance(X, W, B, R, H, Y, act, dtype):
 
 def backward_tolerances(Xh, W, H, dY, act, dtype, ref):
     u = torch.finfo(dtype).eps / 2
+    v = F if dtype == torch.float32 else 2.0 ** -16
     d = dY.double().abs()
     K, N, T = W.shape[1], W.shape[0], Xh.shape[0]
     eh = sum_error(Xh, W.t(), K)                 # H itself is a sum
     if act == "swiglu":
         a, g = H.chunk(2, -1)
-        ra, rg = (u * a.abs() + eh.chunk(2, -1)[0]), (u * g.abs() + eh.chunk(2, -1)[1])
+        ra, rg = (v * a.abs() + eh.chunk(2, -1)[0]), (v * g.abs() + eh.chunk(2, -1)[1])
         arith = F * (16 + 4 * a.abs())
         e = torch.cat([d * (1.1 * rg + 0.5 * g.abs() * ra + arith * g.abs() * (1 + a.abs())),
                        d * (1.1 * ra + arith * a.abs())], -1)
     else:
         arith = 0 if act == "none" else F * (16 + 4 * H.abs()) * (1 + H.abs())
-        e = d * (CURVE[act] * (u * H.abs() + eh) + arith)
+        e = d * (CURVE[act] * (v * H.abs() + eh) + arith)
     dH = torch.cat([f * dY.double() for f in O.act(H, act)[1]], -1)
     tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
     ew = e + (0 if act == "none" else u * dH.abs() + tiny)      # rounded, too

@@ -105,6 +105,8 @@ def test_linear_epilogue_c_interface():
     assert back(dY=None) == -1 and back(H=None) == -1 and back(W=None) == -1 and back(X=None) == -1
     assert back(q=ONE) == -1 and back(code=ONE) == -1 and back(X=None, q=ONE) == -1
     assert back(X=odd) == -4 and back(W=odd) == -4 and back(dY=odd, act=0) == -4
+    assert back(H=ctypes.c_void_p(264)) == -4
+    assert L.opmx_linear_epilogue_kept_bytes(5, 7, 1) == 105 and L.opmx_linear_epilogue_kept_bytes(5, 7, 0) == 140
     assert back(ws=None) == -3 and back(bytes_=need - 1) == -3 and back(ws=ctypes.c_void_p(257)) == -4
     assert back(dX=None, dW=None, dB=None) == 0
 
