@@ -287,7 +287,7 @@ int opmx_swiglu_checkpoint8_backward(const void *dY, const int8_t *q, const uint
  * X, W, dY start at multiples of 16 bytes where K (dY: N, without an activation) is a multiple of 16 bytes
  * (OPMX_ERR_ALIGNMENT otherwise), the others anywhere their type allows.
  * workspace: opmx_linear_epilogue[_backward]_workspace_bytes(), 256-byte aligned, contents arbitrary, not shared with
- * a call running at the same time.  Results do not vary from call to call.  K < 2^21. */
+ * a call running at the same time (may be NULL where that says 256: nothing is needed).  Results do not vary from call to call.  K < 2^21. */
 size_t opmx_linear_epilogue_kept_bytes(int64_t T, int64_t N, int dtype);
 size_t opmx_linear_epilogue_workspace_bytes(int64_t T, int64_t K, int64_t N, int dtype, int activation);
 int opmx_linear_epilogue(const void *X, const void *W, const void *B, const void *R, int64_t T, int64_t K, int64_t N,
@@ -303,7 +303,8 @@ int opmx_linear_epilogue_backward(const void *dY, const void *X, const int8_t *x
  *   loss = E sum_e f_e (1/n) sum_t p[t,e]: 1 for a router that spreads evenly; 0 when no token is kept.
  * scores [T,E] (dtype); token_mask [T] bytes, 0 = the token does not count (NULL: all count);
  * loss: one float; expert_count [E] int64; weight [E] float: w_e = E f_e / n, what the backward pass needs;
- * workspace: opmx_moe_balance_loss_workspace_bytes(), 16-byte aligned, not shared with a call running at the same time.
+ * workspace: opmx_moe_balance_loss_workspace_bytes(), 16-byte aligned, not shared with a call running at the same time
+ * (may be NULL where that says 256: nothing is needed).
  * backward, f held constant:  dscores[t,e] = dloss p[t,e] (w_e - sum_j w_j p[t,j]), 0 for tokens that do not
  * count; dloss: one float on the device.  E and k limits are those of opmx_moe_select. */
 size_t opmx_moe_balance_loss_workspace_bytes(int64_t T, int E);

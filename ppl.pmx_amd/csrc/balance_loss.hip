@@ -8,7 +8,7 @@
 // difference of its expert_offset.  A row of -inf alone has p = 0: it has nothing to spread.
 //
 // Scores are read once in each direction and the gradient is written once.  A token belongs to L lanes
-// (a power of two), each of which holds V of its E scores in registers.  A lane meets the same V experts in
+// (a power of two, a constant of the kernel), each of which holds V of its E scores in registers.  A lane meets the same V experts in
 // every token, so sums over tokens stay in registers until the block is done.  The k-th largest score
 // comes from lists, not from k rounds of a wave-wide maximum: every lane keeps the KL largest of its keys sorted
 // (one median-of-three per slot and key) and the lists of the L lanes meet in log2 L bitonic
@@ -21,7 +21,6 @@
 namespace opmx {
 namespace {
 
-constexpr int kThreads = 512, kWaves = kThreads / kWave;
 constexpr int kMaxBlocks = 256;
 
 template <typename T> struct Key {
@@ -48,16 +47,56 @@ template <> struct Key<float> {
     }
 };
 
+// Exchanges inside rows of 16 lanes are register moves (DPP); only those across rows go through LDS.
+template <int CTRL, typename U> __device__ __forceinline__ U dpp(U v)
+{
+    int b;
+    __builtin_memcpy(&b, &v, 4);
+    b = __builtin_amdgcn_update_dpp(0, b, CTRL, 0xF, 0xF, true);
+    U r;
+    __builtin_memcpy(&r, &b, 4);
+    return r;
+}
+// The value of a lane of the other half of a group of 2 D lanes, when all lanes of a half hold the same.
+template <int D, typename U> __device__ __forceinline__ U other_half(U v)
+{
+    if constexpr (D == 1) return dpp<0xB1>(v);          // quad_perm 1,0,3,2
+    else if constexpr (D == 2) return dpp<0x4E>(v);     // quad_perm 2,3,0,1
+    else if constexpr (D == 4) return dpp<0x141>(v);    // row_half_mirror
+    else if constexpr (D == 8) return dpp<0x140>(v);    // row_mirror
+    else return __shfl_xor(v, D, kWave);
+}
+// Sum over the lanes that are equal mod L (a power of two), in every one of them.
+template <int L, typename U> __device__ __forceinline__ U sum_mod(U v)
+{
+    if (L <= 1) v += dpp<0xB1>(v);
+    if (L <= 2) v += dpp<0x4E>(v);
+    if (L <= 4) v += dpp<0x124>(v);                     // row_ror 4: lanes i and i + 4, then
+    if (L <= 8) v += dpp<0x128>(v);                     // row_ror 8: the other two of the four
+    if (L <= 16) v += __shfl_xor(v, 16, kWave);
+    if (L <= 32) v += __shfl_xor(v, 32, kWave);
+    return v;
+}
+// f(D) for D = 1, 2, ... below L (a constant).
+#define OPMX_HALVES(f)               \
+    do {                             \
+        if constexpr (L > 1) f(1);   \
+        if constexpr (L > 2) f(2);   \
+        if constexpr (L > 4) f(4);   \
+        if constexpr (L > 8) f(8);   \
+        if constexpr (L > 16) f(16); \
+    } while (0)
+
 __device__ __forceinline__ uint32_t umax_(uint32_t a, uint32_t b) { return a > b ? a : b; }
 __device__ __forceinline__ uint32_t umin_(uint32_t a, uint32_t b) { return a < b ? a : b; }
 
 // The id of a lane's i-th score: chunks of N consecutive ids go round the L lanes of the token.
-template <int N> __device__ __forceinline__ int expert_of(int i, int lane, int L) { return ((i / N) * L + lane) * N + i % N; }
+template <int N, int L> __device__ __forceinline__ int expert_of(int i, int lane) { return ((i / N) * L + lane) * N + i % N; }
 
 // A lane's V scores of token t as floats; experts past E read as -inf.  keys (KEYS) get 0 there, which no
 // score's key is.
-template <typename T, int N, int V, bool KEYS>
-__device__ __forceinline__ void load_scores(const T *__restrict__ row, int E, int lane, int L, float (&z)[V],
+template <typename T, int N, int V, int L, bool KEYS>
+__device__ __forceinline__ void load_scores(const T *__restrict__ row, int E, int lane, float (&z)[V],
                                             uint32_t (&key)[KEYS ? V : 1])
 {
 #pragma unroll
@@ -81,21 +120,24 @@ __device__ __forceinline__ void load_scores(const T *__restrict__ row, int E, in
     }
 }
 
-// z -> softmax over the token's L lanes.
-template <int V> __device__ __forceinline__ void softmax_(float (&z)[V], int L)
+// z -> softmax over the token's L lanes.  The hardware's exp2: z - m and its product with log2 e are off by |z - m|
+// 2^-24 each, so is the result, plus an ulp.
+template <int V, int L> __device__ __forceinline__ void softmax_(float (&z)[V])
 {
     float m = z[0];
 #pragma unroll
     for (int i = 1; i < V; ++i) m = fmaxf(m, z[i]);
-    for (int d = 1; d < L; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, kWave));
+#define OPMX_MAX(D) m = fmaxf(m, other_half<D>(m))
+    OPMX_HALVES(OPMX_MAX);
     const bool nothing = m == -INFINITY;     // (a NaN among the scores is not: it makes the sum NaN below)
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        z[i] = z[i] == -INFINITY ? 0.0f : expf(z[i] - m);
+        z[i] = z[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((z[i] - m) * 1.44269504088896341f);
         sum += z[i];
     }
-    for (int d = 1; d < L; d <<= 1) sum += __shfl_xor(sum, d, kWave);
+#define OPMX_SUM(D) sum += other_half<D>(sum)
+    OPMX_HALVES(OPMX_SUM);
     const float r = nothing && sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
     for (int i = 0; i < V; ++i) z[i] *= r;
@@ -110,12 +152,12 @@ template <int KL> __device__ __forceinline__ void insert(uint32_t (&a)[KL], uint
     a[0] = umax_(a[0], x);
 }
 
-// a: the KL largest of a's and the xor-partner's lists, sorted again.
-template <int KL> __device__ __forceinline__ void merge(uint32_t (&a)[KL], int d)
+// a: the KL largest of a's and the other half's lists, sorted again.
+template <int KL, int D> __device__ __forceinline__ void merge(uint32_t (&a)[KL])
 {
     uint32_t b[KL];
 #pragma unroll
-    for (int j = 0; j < KL; ++j) b[j] = __shfl_xor(a[KL - 1 - j], d, kWave);
+    for (int j = 0; j < KL; ++j) b[j] = other_half<D>(a[KL - 1 - j]);
 #pragma unroll
     for (int j = 0; j < KL; ++j) a[j] = umax_(a[j], b[j]);                      // bitonic
 #pragma unroll
@@ -129,15 +171,19 @@ template <int KL> __device__ __forceinline__ void merge(uint32_t (&a)[KL], int d
             }
 }
 
+// a[i] of a descending list, as a maximum over a[i], a[i+1], ...: a selection by index would put the list into LDS,
+// at an address that every workgroup works out from the dispatch packet in host memory (57 ns each, one after the other:
+// 15 us of a launch of 256).
 template <int KL> __device__ __forceinline__ uint32_t at(const uint32_t (&a)[KL], int i)
 {
-    uint32_t v = a[0];
+    uint32_t v = 0u;
 #pragma unroll
-    for (int j = 1; j < KL; ++j) v = i == j ? a[j] : v;
+    for (int j = 0; j < KL; ++j) v = umax_(v, j >= i ? a[j] : 0u);
     return v;
 }
 
 // What the sums over tokens become: loss, counts, and w for the backward pass.  One block.
+template <int THREADS>
 __device__ __forceinline__ void finish(double psum, int64_t count, int64_t kept, int e, int E, int k, double *red,
                                        float *loss, int64_t *counts, float *w)
 {
@@ -151,7 +197,7 @@ __device__ __forceinline__ void finish(double psum, int64_t count, int64_t kept,
     }
     red[threadIdx.x] = part;
     __syncthreads();
-    for (int s = kThreads / 2; s >= 1; s >>= 1) {
+    for (int s = THREADS / 2; s >= 1; s >>= 1) {
         if (static_cast<int>(threadIdx.x) < s) red[threadIdx.x] += red[threadIdx.x + s];
         __syncthreads();
     }
@@ -160,19 +206,20 @@ __device__ __forceinline__ void finish(double psum, int64_t count, int64_t kept,
 
 // Sums over the tokens of a block.  A single block finishes by itself; several leave psum [blocks][E], counts
 // [blocks][E] and kept [blocks] in the workspace.
-template <typename T, int N, int V, int KL>
-__global__ __launch_bounds__(kThreads) void balance_kernel(const T *__restrict__ scores,
+template <typename T, int N, int V, int L, int KL, int THREADS>
+__global__ __launch_bounds__(THREADS) void balance_kernel(const T *__restrict__ scores,
                                                            const uint8_t *__restrict__ mask, int64_t Ttok, int E, int k,
-                                                           int L, float *__restrict__ part_p, int32_t *__restrict__ part_c,
+                                                           float *__restrict__ part_p, int32_t *__restrict__ part_c,
                                                            int32_t *__restrict__ part_n, float *__restrict__ loss,
                                                            int64_t *__restrict__ counts, float *__restrict__ w)
 {
-    __shared__ float s_p[kWaves][OPMX_MOE_MAX_EXPERTS];
-    __shared__ int32_t s_c[kWaves][OPMX_MOE_MAX_EXPERTS];
-    __shared__ int32_t s_n[kWaves];
-    __shared__ double s_red[kThreads];
+    constexpr int WAVES = THREADS / kWave;
+    __shared__ float s_p[WAVES][OPMX_MOE_MAX_EXPERTS];
+    __shared__ int32_t s_c[WAVES][OPMX_MOE_MAX_EXPERTS];
+    __shared__ int32_t s_n[WAVES];
+    __shared__ double s_red[THREADS];
     const int lane = lane_id() % L, wave = threadIdx.x / kWave;
-    const int per_block = kThreads / L;
+    const int per_block = THREADS / L;
     float psum[V];
     int32_t cnt[V];
 #pragma unroll
@@ -188,15 +235,16 @@ __global__ __launch_bounds__(kThreads) void balance_kernel(const T *__restrict__
         const T *row = scores + (t < Ttok ? t : Ttok - 1) * E;
         float z[V];
         uint32_t key[V];
-        load_scores<T, N, V, true>(row, E, lane, L, z, key);
+        load_scores<T, N, V, L, true>(row, E, lane, z, key);
         uint32_t list[KL];
 #pragma unroll
         for (int j = 0; j < KL; ++j) list[j] = 0u;
 #pragma unroll
         for (int i = 0; i < V; ++i) insert<KL>(list, key[i]);
-        for (int d = 1; d < L; d <<= 1) merge<KL>(list, d);
+#define OPMX_MERGE(D) merge<KL, D>(list)
+        OPMX_HALVES(OPMX_MERGE);
         const uint32_t kth = at<KL>(list, k - 1);
-        softmax_<V>(z, L);
+        softmax_<V, L>(z);
         if constexpr (Key<T>::unique) {
 #pragma unroll
             for (int i = 0; i < V; ++i) cnt[i] += keep && key[i] >= kth ? 1 : 0;
@@ -207,10 +255,8 @@ __global__ __launch_bounds__(kThreads) void balance_kernel(const T *__restrict__
                 above += key[i] > kth ? 1 : 0;
                 equal += key[i] == kth ? 1 : 0;
             }
-            for (int d = 1; d < L; d <<= 1) {
-                above += __shfl_xor(above, d, kWave);
-                equal += __shfl_xor(equal, d, kWave);
-            }
+#define OPMX_COUNT(D) above += other_half<D>(above), equal += other_half<D>(equal)
+            OPMX_HALVES(OPMX_COUNT);
             const int left = k - above;      // so many of the equal ones are picked, the lowest ids first
             if (!__any(equal > left)) {
 #pragma unroll
@@ -246,17 +292,15 @@ __global__ __launch_bounds__(kThreads) void balance_kernel(const T *__restrict__
     // over the tokens of the wave, then of the block
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        for (int d = L; d < kWave; d <<= 1) {
-            psum[i] += __shfl_xor(psum[i], d, kWave);
-            cnt[i] += __shfl_xor(cnt[i], d, kWave);
-        }
-        const int e = expert_of<N>(i, lane, L);
+        psum[i] = sum_mod<L>(psum[i]);
+        cnt[i] = sum_mod<L>(cnt[i]);
+        const int e = expert_of<N, L>(i, lane);
         if (lane_id() < L && e < E) {
             s_p[wave][e] = psum[i];
             s_c[wave][e] = cnt[i];
         }
     }
-    for (int d = 1; d < kWave; d <<= 1) kept += __shfl_xor(kept, d, kWave);
+    kept = sum_mod<1>(kept);
     if (lane_id() == 0) s_n[wave] = kept;
     __syncthreads();
     const int e = threadIdx.x;
@@ -264,15 +308,15 @@ __global__ __launch_bounds__(kThreads) void balance_kernel(const T *__restrict__
     int32_t c = 0, n = 0;
     if (e < E) {
 #pragma unroll
-        for (int v = 0; v < kWaves; ++v) {
+        for (int v = 0; v < WAVES; ++v) {
             p += s_p[v][e];
             c += s_c[v][e];
         }
     }
 #pragma unroll
-    for (int v = 0; v < kWaves; ++v) n += s_n[v];
+    for (int v = 0; v < WAVES; ++v) n += s_n[v];
     if (gridDim.x == 1) {
-        finish(p, c, n, e, E, k, s_red, loss, counts, w);
+        finish<THREADS>(p, c, n, e, E, k, s_red, loss, counts, w);
         return;
     }
     if (e < E) {
@@ -283,31 +327,48 @@ __global__ __launch_bounds__(kThreads) void balance_kernel(const T *__restrict__
 }
 
 // The blocks' sums: thread (slice, e) adds every slices-th block's, in order, then slice 0 adds the slices.
-__global__ __launch_bounds__(kThreads) void balance_finish_kernel(const float *__restrict__ part_p,
-                                                                  const int32_t *__restrict__ part_c,
-                                                                  const int32_t *__restrict__ part_n, int blocks, int E,
-                                                                  int k, float *__restrict__ loss,
-                                                                  int64_t *__restrict__ counts, float *__restrict__ w)
+constexpr int kFinish = 1024;
+__global__ __launch_bounds__(kFinish) void balance_finish_kernel(const float *__restrict__ part_p,
+                                                                 const int32_t *__restrict__ part_c,
+                                                                 const int32_t *__restrict__ part_n, int blocks, int E,
+                                                                 int k, float *__restrict__ loss,
+                                                                 int64_t *__restrict__ counts, float *__restrict__ w)
 {
-    __shared__ double s_red[kThreads];
-    __shared__ int64_t s_c[kThreads];
+    __shared__ double s_red[kFinish];
+    __shared__ int64_t s_c[kFinish];
     __shared__ int64_t s_n;
-    const int slices = kThreads / E < 32 ? kThreads / E : 32;   // E <= 256: at least two
+    const int slices = kFinish / E < 32 ? kFinish / E : 32;      // E <= 256: at least four
     const int slice = threadIdx.x / E, e = threadIdx.x % E;
     double p = 0.0;
     int64_t c = 0;
-    if (slice < slices)
-#pragma unroll 8
-        for (int b = slice; b < blocks; b += slices) {
+    if (slice < slices) {
+        int b = slice;
+        for (; b + 15 * slices < blocks; b += 16 * slices) {     // sixteen pairs of loads in flight
+            float pv[16];
+            int32_t cv[16];
+#pragma unroll
+            for (int u = 0; u < 16; ++u) {
+                pv[u] = part_p[(b + u * slices) * E + e];
+                cv[u] = part_c[(b + u * slices) * E + e];
+            }
+#pragma unroll
+            for (int u = 0; u < 16; ++u) {
+                p += pv[u];
+                c += cv[u];
+            }
+        }
+        for (; b < blocks; b += slices) {
             p += part_p[b * E + e];
             c += part_c[b * E + e];
         }
+    }
     s_red[threadIdx.x] = p;
     s_c[threadIdx.x] = c;
     if (threadIdx.x < kWave) {
-        int64_t n = 0;
-        for (int b = threadIdx.x; b < blocks; b += kWave) n += part_n[b];
-        for (int d = 1; d < kWave; d <<= 1) n += __shfl_xor(n, d, kWave);
+        int32_t n = 0;
+#pragma unroll
+        for (int b = 0; b < kMaxBlocks; b += kWave) n += b + static_cast<int>(threadIdx.x) < blocks ? part_n[b + threadIdx.x] : 0;
+        n = sum_mod<1>(n);                                       // T < 2^31
         if (threadIdx.x == 0) s_n = n;
     }
     __syncthreads();
@@ -318,21 +379,21 @@ __global__ __launch_bounds__(kThreads) void balance_finish_kernel(const float *_
         }
     const int64_t n = s_n;
     __syncthreads();                         // s_red is used again
-    finish(p, c, n, slice == 0 ? e : E, E, k, s_red, loss, counts, w);
+    finish<kFinish>(p, c, n, slice == 0 ? e : E, E, k, s_red, loss, counts, w);
 }
 
-template <typename T, int N, int V>
+template <typename T, int N, int V, int L>
 __global__ __launch_bounds__(256) void balance_backward_kernel(const T *__restrict__ scores,
                                                                const uint8_t *__restrict__ mask,
                                                                const float *__restrict__ w,
                                                                const float *__restrict__ dloss, int64_t Ttok, int E,
-                                                               int L, T *__restrict__ dscores)
+                                                               T *__restrict__ dscores)
 {
     const int lane = lane_id() % L, per_block = 256 / L;
     float wv[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        const int e = expert_of<N>(i, lane, L);
+        const int e = expert_of<N, L>(i, lane);
         wv[i] = e < E ? w[e] : 0.0f;
     }
     const float scale = *dloss;
@@ -342,12 +403,13 @@ __global__ __launch_bounds__(256) void balance_backward_kernel(const T *__restri
         const bool keep = t < Ttok && (mask == nullptr || mask[t] != 0);
         float z[V];
         uint32_t none[1];
-        load_scores<T, N, V, false>(scores + (t < Ttok ? t : Ttok - 1) * E, E, lane, L, z, none);
-        softmax_<V>(z, L);
+        load_scores<T, N, V, L, false>(scores + (t < Ttok ? t : Ttok - 1) * E, E, lane, z, none);
+        softmax_<V, L>(z);
         float dot = 0.0f;
 #pragma unroll
         for (int i = 0; i < V; ++i) dot += z[i] * wv[i];
-        for (int d = 1; d < L; d <<= 1) dot += __shfl_xor(dot, d, kWave);
+#define OPMX_DOT(D) dot += other_half<D>(dot)
+        OPMX_HALVES(OPMX_DOT);
         if (t >= Ttok) continue;             // (the last trip: nobody needs this lane again)
         T *out = dscores + t * E;
 #pragma unroll
@@ -369,54 +431,54 @@ __global__ __launch_bounds__(256) void balance_backward_kernel(const T *__restri
     }
 }
 
-// Lanes per token: E scores over V per lane.
-inline int lanes_for(int E, int V, int N)
+// Lanes L per token and scores V per lane.  Up to 64 experts a lane holds 8 scores: more lanes per token, and the few
+// tokens of a batch spread over more of them; blocks of 4 waves.  Beyond, 16, and blocks of 16 waves: the sums of
+// one block per CU are all that the second launch has to add.  L is a constant of the kernels, whose code
+// then has no branches.
+constexpr int kFewExperts = 64, kFewThreads = 256, kManyThreads = 1024;
+inline int lanes_few(int E) { return E <= 8 ? 1 : E <= 16 ? 2 : E <= 32 ? 4 : 8; }
+inline int lanes_many(int E) { return E <= 128 ? 8 : 16; }
+
+struct Forward {
+    const void *scores, *mask;
+    int64_t Ttok;
+    int E, k, blocks;
+    float *pp;
+    int32_t *pc, *pn;
+    float *loss;
+    int64_t *counts;
+    float *w;
+};
+template <typename T, int N, int V, int L, int KL, int THREADS> void forward_launch(const Forward &f, hipStream_t s)
 {
-    int L = 1;
-    while (L * V < (E + N - 1) / N * N) L <<= 1;
-    return L;
+    balance_kernel<T, N, V, L, KL, THREADS><<<f.blocks, THREADS, 0, s>>>(
+        static_cast<const T *>(f.scores), static_cast<const uint8_t *>(f.mask), f.Ttok, f.E, f.k, f.pp, f.pc, f.pn, f.loss,
+        f.counts, f.w);
 }
-
-// Up to 64 experts a lane holds 8 scores: more lanes per token, and the few tokens of a batch spread over more
-// of them.  Beyond, 16: fewer merges per token, and registers for two waves per SIMD more than with 32.  Lists of 32 keys leave registers for 8 scores only.
-constexpr int kFewExperts = 64;
-
-template <typename T, int N, int V>
-int balance_forward(const void *scores, const void *mask, int64_t Ttok, int E, int k, int blocks, float *pp, int32_t *pc,
-                    int32_t *pn, float *loss, int64_t *counts, float *w, hipStream_t s)
+template <typename T, int N> void forward_sums(const Forward &f, hipStream_t s)
 {
-    const int L = lanes_for(E, V, N);
-    const T *z = static_cast<const T *>(scores);
-    const uint8_t *m = static_cast<const uint8_t *>(mask);
-    if (k <= 2) balance_kernel<T, N, V, 2><<<blocks, kThreads, 0, s>>>(z, m, Ttok, E, k, L, pp, pc, pn, loss, counts, w);
-    else if (k <= 8) balance_kernel<T, N, V, 8><<<blocks, kThreads, 0, s>>>(z, m, Ttok, E, k, L, pp, pc, pn, loss, counts, w);
-    else balance_kernel<T, N, 8, 32><<<blocks, kThreads, 0, s>>>(z, m, Ttok, E, k, lanes_for(E, 8, N), pp, pc, pn, loss,
-                                                                counts, w);
-    OPMX_LAUNCH_CHECK();
-    if (blocks > 1) {
-        balance_finish_kernel<<<1, kThreads, 0, s>>>(pp, pc, pn, blocks, E, k, loss, counts, w);
-        OPMX_LAUNCH_CHECK();
+    if (f.k > 8) {                  // lists of 32 keys leave registers for 8 scores only
+        if (f.E <= 64) forward_launch<T, N, 8, 8, 32, 256>(f, s);
+        else forward_launch<T, N, 8, 32, 32, 256>(f, s);
+    } else if (f.E <= kFewExperts) {
+        switch (lanes_few(f.E)) {
+            case 1: forward_launch<T, N, 8, 1, 8, kFewThreads>(f, s); break;
+            case 2: forward_launch<T, N, 8, 2, 8, kFewThreads>(f, s); break;
+            case 4: forward_launch<T, N, 8, 4, 8, kFewThreads>(f, s); break;
+            default: forward_launch<T, N, 8, 8, 8, kFewThreads>(f, s); break;
+        }
+    } else if (lanes_many(f.E) == 8) {
+        forward_launch<T, N, 16, 8, 8, kManyThreads>(f, s);
+    } else {
+        forward_launch<T, N, 16, 16, 8, kManyThreads>(f, s);
     }
-    return OPMX_OK;
 }
 
-template <typename T, int N, int V>
-int balance_backward(const void *scores, const void *mask, const float *w, const float *dloss, int64_t Ttok, int E,
-                     void *dscores, hipStream_t s)
-{
-    const int L = lanes_for(E, V, N);
-    const int64_t blocks = ceil_div(Ttok, 256 / L), most = 16 * 256;
-    balance_backward_kernel<T, N, V><<<static_cast<unsigned>(blocks < most ? blocks : most), 256, 0, s>>>(
-        static_cast<const T *>(scores), static_cast<const uint8_t *>(mask), w, dloss, Ttok, E, L, static_cast<T *>(dscores));
-    OPMX_LAUNCH_CHECK();
-    return OPMX_OK;
-}
-
-// One block serves a decoding batch in one launch; beyond that one block per CU and a second launch.
+// One block serves a decoding batch in one launch; beyond that at most one block per CU and a second launch.
 inline int blocks_for(int64_t Ttok, int E)
 {
-    const int L = lanes_for(E, E <= kFewExperts ? 8 : 16, 1);
-    const int64_t b = ceil_div(Ttok, kThreads / L);
+    const bool few = E <= kFewExperts;
+    const int64_t b = ceil_div(Ttok, few ? kFewThreads / lanes_few(E) : kManyThreads / lanes_many(E));
     return static_cast<int>(b <= 1 ? 1 : (b < kMaxBlocks ? b : kMaxBlocks));
 }
 
@@ -425,28 +487,58 @@ int forward_impl(const void *scores, const void *mask, int64_t Ttok, int E, int 
                  float *w, hipStream_t s)
 {
     constexpr int n = Vec16<T>::n;
-    const int blocks = blocks_for(Ttok, E);
-    float *pp = static_cast<float *>(ws);
-    int32_t *pc = reinterpret_cast<int32_t *>(pp + static_cast<int64_t>(blocks) * E), *pn = pc + static_cast<int64_t>(blocks) * E;
-    const bool vec = E % n == 0 && aligned16(scores);
-    if (E <= kFewExperts)
-        return vec ? balance_forward<T, n, 8>(scores, mask, Ttok, E, k, blocks, pp, pc, pn, loss, counts, w, s)
-                   : balance_forward<T, 1, 8>(scores, mask, Ttok, E, k, blocks, pp, pc, pn, loss, counts, w, s);
-    return vec ? balance_forward<T, n, 16>(scores, mask, Ttok, E, k, blocks, pp, pc, pn, loss, counts, w, s)
-               : balance_forward<T, 1, 16>(scores, mask, Ttok, E, k, blocks, pp, pc, pn, loss, counts, w, s);
+    Forward f{scores, mask, Ttok, E, k, blocks_for(Ttok, E), static_cast<float *>(ws), nullptr, nullptr, loss, counts, w};
+    f.pc = reinterpret_cast<int32_t *>(f.pp + static_cast<int64_t>(f.blocks) * E);
+    f.pn = f.pc + static_cast<int64_t>(f.blocks) * E;
+    if (E % n == 0 && aligned16(scores)) forward_sums<T, n>(f, s);
+    else forward_sums<T, 1>(f, s);
+    OPMX_LAUNCH_CHECK();
+    if (f.blocks > 1) {
+        balance_finish_kernel<<<1, kFinish, 0, s>>>(f.pp, f.pc, f.pn, f.blocks, E, k, loss, counts, w);
+        OPMX_LAUNCH_CHECK();
+    }
+    return OPMX_OK;
 }
 
+struct Backward {
+    const void *scores, *mask;
+    const float *w, *dloss;
+    int64_t Ttok;
+    int E;
+    void *dscores;
+};
+template <typename T, int N, int V, int L> void backward_launch(const Backward &b, hipStream_t s)
+{
+    const int64_t blocks = ceil_div(b.Ttok, 256 / L), most = 16 * 256;
+    balance_backward_kernel<T, N, V, L><<<static_cast<unsigned>(blocks < most ? blocks : most), 256, 0, s>>>(
+        static_cast<const T *>(b.scores), static_cast<const uint8_t *>(b.mask), b.w, b.dloss, b.Ttok, b.E,
+        static_cast<T *>(b.dscores));
+}
+template <typename T, int N> void backward_grads(const Backward &b, hipStream_t s)
+{
+    if (b.E <= kFewExperts) {
+        switch (lanes_few(b.E)) {
+            case 1: backward_launch<T, N, 8, 1>(b, s); break;
+            case 2: backward_launch<T, N, 8, 2>(b, s); break;
+            case 4: backward_launch<T, N, 8, 4>(b, s); break;
+            default: backward_launch<T, N, 8, 8>(b, s); break;
+        }
+    } else if (lanes_many(b.E) == 8) {
+        backward_launch<T, N, 16, 8>(b, s);
+    } else {
+        backward_launch<T, N, 16, 16>(b, s);
+    }
+}
 template <typename T>
 int backward_impl(const void *scores, const void *mask, const float *w, const float *dloss, int64_t Ttok, int E,
                   void *dscores, hipStream_t s)
 {
     constexpr int n = Vec16<T>::n;
-    const bool vec = E % n == 0 && aligned16(scores) && aligned16(dscores);
-    if (E <= kFewExperts)
-        return vec ? balance_backward<T, n, 8>(scores, mask, w, dloss, Ttok, E, dscores, s)
-                   : balance_backward<T, 1, 8>(scores, mask, w, dloss, Ttok, E, dscores, s);
-    return vec ? balance_backward<T, n, 16>(scores, mask, w, dloss, Ttok, E, dscores, s)
-               : balance_backward<T, 1, 16>(scores, mask, w, dloss, Ttok, E, dscores, s);
+    const Backward b{scores, mask, w, dloss, Ttok, E, dscores};
+    if (E % n == 0 && aligned16(scores) && aligned16(dscores)) backward_grads<T, n>(b, s);
+    else backward_grads<T, 1>(b, s);
+    OPMX_LAUNCH_CHECK();
+    return OPMX_OK;
 }
 
 }  // namespace
@@ -454,8 +546,10 @@ int backward_impl(const void *scores, const void *mask, const float *w, const fl
 size_t moe_balance_loss_workspace_bytes(int64_t Ttok, int E)
 {
     if (Ttok <= 0 || E <= 0 || E > OPMX_MOE_MAX_EXPERTS) return 256;
-    const size_t b = static_cast<size_t>(blocks_for(Ttok, E)) * (static_cast<size_t>(E) * 8 + 4);
-    return (b + 255) / 256 * 256;
+    const int blocks = blocks_for(Ttok, E);
+    if (blocks == 1) return 256;             // finishes by itself
+    const size_t b = static_cast<size_t>(blocks) * (static_cast<size_t>(E) * 8 + 4);
+    return (b + 255) / 256 * 256 + 256;
 }
 
 int launch_moe_balance_loss(const void *scores, const void *mask, int64_t T, int E, int k, int dtype, float *loss,

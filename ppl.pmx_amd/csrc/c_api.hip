@@ -468,7 +468,8 @@ int opmx_moe_balance_loss(const void *scores, const uint8_t *token_mask, int64_t
     if (!dtype_ok(dtype) || E > OPMX_MOE_MAX_EXPERTS || k > OPMX_MOE_MAX_EXPERTS_PER_TOKEN) return OPMX_ERR_UNSUPPORTED;
     if (T > (int64_t{1} << 31) / k) return OPMX_ERR_UNSUPPORTED;
     if (!loss || !expert_count || !weight || (T > 0 && !scores)) return OPMX_ERR_BAD_ARGUMENT;
-    if (T > 0 && (!workspace || workspace_bytes < moe_balance_loss_workspace_bytes(T, E))) return OPMX_ERR_WORKSPACE;
+    const size_t need = moe_balance_loss_workspace_bytes(T, E);
+    if (need > 256 && (!workspace || workspace_bytes < need)) return OPMX_ERR_WORKSPACE;
     if (workspace && !aligned16(workspace)) return OPMX_ERR_ALIGNMENT;
     return launch_moe_balance_loss(scores, token_mask, T, E, k, dtype, loss, expert_count, weight, workspace, st(stream));
 }

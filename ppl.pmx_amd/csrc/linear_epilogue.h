@@ -17,35 +17,49 @@ template <typename T> __device__ __forceinline__ float logistic_for(float x)
     else return sigmoidf_(x);
 }
 
-constexpr float kSqrtHalf = 0.70710678118654752f, kGeluC = 0.79788456080286536f, kGeluA = 0.044715f;
+constexpr float kGeluC = 0.79788456080286536f, kGeluA = 0.044715f;
 constexpr float kInvSqrt2Pi = 0.39894228040143268f;
 
-// erfc keeps its relative accuracy where 1 + erf would cancel (h < 0).
+// Phi(h) for GELU, and e^(-h^2 / 2), which the slope needs as well.  With z = |h| / sqrt 2, erfc(z) = e^(-z^2) t S(t) where
+// t = 1 / (1 + 0.4 z) and S is smooth: a polynomial of degree 8 fitted to scipy's erfcx for z <= 14 (beyond,
+// e^(-z^2) is 0 in fp32) is within 9e-8 of it, relatively, on both sides: Phi keeps its digits where it is small.
+// In fp32 the whole is within 4e-7 (1 + h^2 / 4).  The library's erfc costs four times the instructions, in an epilogue
+// whose time no matrix instruction hides.
+__device__ __forceinline__ float normal_cdf(float h, float &bell)
+{
+    constexpr float kHalf[9] = {0.5f * 0.22566290199756622f, 0.5f * 0.22593672573566437f, 0.5f * 0.20561064779758453f,
+                                0.5f * 0.17847903072834015f, 0.5f * 0.11547110229730606f, 0.5f * 0.035431284457445145f,
+                                0.5f * 0.13050033152103424f, 0.5f * -0.16306036710739136f, 0.5f * 0.0459684394299984f};
+    const float t = __builtin_amdgcn_rcpf(1.0f + 0.28284271247461901f * fabsf(h));
+    float s = kHalf[8];
+#pragma unroll
+    for (int i = 7; i >= 0; --i) s = s * t + kHalf[i];
+    bell = __builtin_amdgcn_exp2f(h * h * -0.72134752044448170f);
+    const float tail = bell * t * s;
+    return h < 0.0f ? tail : 1.0f - tail;
+}
+
 template <typename T> __device__ __forceinline__ float activate(int act, float h)
 {
-    switch (act) {
-        case OPMX_ACTIVATION_SILU: return h * logistic_for<T>(h);
-        case OPMX_ACTIVATION_GELU: return 0.5f * h * erfcf(-h * kSqrtHalf);
-        case OPMX_ACTIVATION_GELU_TANH: return h * logistic_for<T>(2.0f * kGeluC * (h + kGeluA * h * h * h));
+    if (act == OPMX_ACTIVATION_GELU) {
+        float bell;
+        return h * normal_cdf(h, bell);
     }
-    return h;
+    // silu and the tanh form of gelu are h s(x)
+    const float x = act == OPMX_ACTIVATION_SILU ? h : 2.0f * kGeluC * (h + kGeluA * h * h * h);
+    return h * logistic_for<T>(x);
 }
 template <typename T> __device__ __forceinline__ float slope(int act, float h)
 {
-    switch (act) {
-        case OPMX_ACTIVATION_SILU: {
-            const float s = logistic_for<T>(h);
-            return s + h * s * (1.0f - s);
-        }
-        case OPMX_ACTIVATION_GELU:
-            return 0.5f * erfcf(-h * kSqrtHalf) + h * expf(-0.5f * h * h) * kInvSqrt2Pi;
-        case OPMX_ACTIVATION_GELU_TANH: {
-            const float s = logistic_for<T>(2.0f * kGeluC * (h + kGeluA * h * h * h));
-            const float q = h * h;
-            return s + h * s * (1.0f - s) * (2.0f * kGeluC * (1.0f + 3.0f * kGeluA * q));
-        }
+    if (act == OPMX_ACTIVATION_GELU) {
+        float bell;
+        const float cdf = normal_cdf(h, bell);
+        return cdf + h * bell * kInvSqrt2Pi;
     }
-    return 1.0f;
+    const bool silu = act == OPMX_ACTIVATION_SILU;
+    const float s = logistic_for<T>(silu ? h : 2.0f * kGeluC * (h + kGeluA * h * h * h));
+    const float dx = silu ? 1.0f : 2.0f * kGeluC * (1.0f + 3.0f * kGeluA * h * h);
+    return s + h * s * (1.0f - s) * dx;
 }
 
 // Eight consecutive values of a row at any address; `left` of them exist.
@@ -162,22 +176,16 @@ struct Epilogue {
 
 namespace {
 
-// Columns col .. col+7 of row `row` (h; with SwiGLU h holds the first half's and g the second half's columns).
+// Columns col .. col+7 of row `row` (h; with SwiGLU h holds the first half's and g the second half's columns): bias,
+// what is kept, activation.  The result is in h.
 template <typename T, bool GATED>
-__device__ __forceinline__ void finish8(const Epilogue &e, int64_t row, int64_t col, float (&h)[8], float (&g)[8])
+__device__ __forceinline__ void activate8(const Epilogue &e, int64_t row, int64_t col, int64_t left, const float (&bh)[8],
+                                          const float (&bg)[8], float (&h)[8], float (&g)[8])
 {
-    const int64_t left = e.ncols - col;
-    if (left <= 0) return;
-    if (e.bias) {
-        float b[8];
-        load8(static_cast<const T *>(e.bias) + col, left, b);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) h[j] += b[j];
-        if (GATED) {
-            load8(static_cast<const T *>(e.bias) + e.ncols + col, left, b);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) g[j] += b[j];
-        }
+    for (int j = 0; j < 8; ++j) {
+        h[j] += bh[j];
+        if (GATED) g[j] += bg[j];
     }
     if (e.H) {
         keep8<T>(e.H, e.rows * e.N, row * e.N + col, left, h);
@@ -190,13 +198,15 @@ __device__ __forceinline__ void finish8(const Epilogue &e, int64_t row, int64_t 
 #pragma unroll
         for (int j = 0; j < 8; ++j) h[j] = activate<T>(e.act, h[j]);
     }
-    if (e.residual) {
-        float r[8];
-        load8(static_cast<const T *>(e.residual) + row * e.ncols + col, left, r);
+}
+template <typename T, bool GATED>
+__device__ __forceinline__ void load_bias8(const Epilogue &e, int64_t col, float (&bh)[8], float (&bg)[8])
+{
 #pragma unroll
-        for (int j = 0; j < 8; ++j) h[j] += r[j];
-    }
-    store8(static_cast<T *>(e.Y) + row * e.ncols + col, left, h);
+    for (int j = 0; j < 8; ++j) bh[j] = bg[j] = 0.0f;
+    if (e.bias == nullptr || col >= e.ncols) return;
+    load8(static_cast<const T *>(e.bias) + col, e.ncols - col, bh);
+    if (GATED) load8(static_cast<const T *>(e.bias) + e.ncols + col, e.ncols - col, bg);
 }
 
 }  // namespace
@@ -210,8 +220,12 @@ struct Operand {
     int64_t pitch;
     bool k_major;
 };
+// Tiles of C, by rows: 256 x 256 (eight waves, two k-tiles in LDS), and 128 columns wide with two k-tiles in LDS (two
+// workgroups per CU) or four (one, for products with fewer tiles than CUs: the loads have three k-tiles' time); 64 and
+// 32 rows are for few rows in all.
+enum class Tile { k256, k128, k128Deep, k64, k32 };
 // ranges > 1: k is cut into that many ranges, e.part must hold their sums.
-int launch_linear_gemm(const Operand &P, const Operand &Q, int64_t Kc, int dtype, const Epilogue &e, int tile, int ranges,
+int launch_linear_gemm(const Operand &P, const Operand &Q, int64_t Kc, int dtype, const Epilogue &e, Tile tile, int ranges,
                        hipStream_t s);
 
 }  // namespace opmx

@@ -16,12 +16,17 @@ namespace {
 inline int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
 // X [R, C] dense -> [R][pitch], zeros behind the C values.
+// Two tensors of the same C in one launch (blockIdx.z).
 template <typename T>
-__global__ __launch_bounds__(256) void pad_kernel(const T *__restrict__ X, int64_t R, int64_t C, int64_t pitch,
-                                                  T *__restrict__ out)
+__global__ __launch_bounds__(256) void pad_kernel(const T *__restrict__ X0, int64_t R0, T *__restrict__ out0,
+                                                  const T *__restrict__ X1, int64_t R1, T *__restrict__ out1, int64_t C,
+                                                  int64_t pitch)
 {
     const int64_t c = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) * 8;
     if (c >= pitch) return;
+    const T *X = blockIdx.z ? X1 : X0;
+    T *out = blockIdx.z ? out1 : out0;
+    const int64_t R = blockIdx.z ? R1 : R0;
     const int64_t step = static_cast<int64_t>(gridDim.y) * blockDim.y;
     for (int64_t r = static_cast<int64_t>(blockIdx.y) * blockDim.y + threadIdx.y; r < R; r += step) {
         float v[8];
@@ -30,15 +35,18 @@ __global__ __launch_bounds__(256) void pad_kernel(const T *__restrict__ X, int64
     }
 }
 
-// dH [T][pitch] (zeros behind the N values) from dY [T, ncols] and H [T, N]; sums: per row chunk (blockIdx.y) the
-// column sums [chunks][N] in fp32, before dH is rounded.  Lanes go over columns, 8 each, blockDim.y rows at a time.
+// dH [T][pitch] (zeros behind the N values) from dY [T, ncols] and the kept H; sums: per row chunk (blockIdx.y)
+// the column sums [chunks][N] in fp32, before dH is rounded.  A block takes 512 columns (a wave 8 per lane) and
+// every fourth row per wave.  Memory bound: SwiGLU over [4096, 2 x 14336] bfloat16 moves 704 MB.
+constexpr int kSlopeCols = 512, kSlopeWaves = 4;
 template <typename T, bool GATED>
 __global__ __launch_bounds__(256) void slope_kernel(const T *__restrict__ dY, const void *__restrict__ H, int64_t Ttok,
                                                     int64_t N, int64_t ncols, int64_t pitch, int64_t rows_per_chunk,
                                                     int act, T *__restrict__ dH, float *__restrict__ sums)
 {
-    __shared__ float s_sum[256 * 8 * (GATED ? 2 : 1)];
-    const int64_t c = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) * 8;
+    __shared__ float s_sum[kSlopeWaves][GATED ? 2 : 1][kSlopeCols];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t c = static_cast<int64_t>(blockIdx.x) * kSlopeCols + lane * 8;
     const int64_t left = ncols - c;
     const int64_t r0 = static_cast<int64_t>(blockIdx.y) * rows_per_chunk;
     const int64_t r1 = r0 + rows_per_chunk < Ttok ? r0 + rows_per_chunk : Ttok;
@@ -46,7 +54,8 @@ __global__ __launch_bounds__(256) void slope_kernel(const T *__restrict__ dY, co
 #pragma unroll
     for (int j = 0; j < 8; ++j) sum[0][j] = sum[1][j] = 0.0f;
     if (left > 0) {
-        for (int64_t r = r0 + threadIdx.y; r < r1; r += blockDim.y) {
+#pragma unroll 2
+        for (int64_t r = r0 + wave; r < r1; r += kSlopeWaves) {
             float d[8], h[8];
             load8(dY + r * ncols + c, left, d);
             if (GATED) {
@@ -63,7 +72,9 @@ __global__ __launch_bounds__(256) void slope_kernel(const T *__restrict__ dY, co
                 }
                 if (dH) {
                     store8(dH + r * pitch + c, left, d);
-                    store8(dH + r * pitch + ncols + c, left < 8 ? left : pitch - ncols - c, h);
+                    store8(dH + r * pitch + ncols + c, left, h);
+                    if (left <= 8)                                                     // the lane of the last columns
+                        for (int64_t p = N; p < pitch; ++p) dH[r * pitch + p] = from_f32<T>(0.0f);
                 }
             } else {
                 if (act != OPMX_ACTIVATION_NONE) {
@@ -79,59 +90,80 @@ __global__ __launch_bounds__(256) void slope_kernel(const T *__restrict__ dY, co
                 if (dH) store8(dH + r * pitch + c, pitch - c, d);
             }
         }
-        if (GATED && dH && left <= 8)                    // the row's pad, by the lane of its last columns
-            for (int64_t r = r0 + threadIdx.y; r < r1; r += blockDim.y)
-                for (int64_t p = N; p < pitch; ++p) dH[r * pitch + p] = from_f32<T>(0.0f);
     }
     if (sums == nullptr) return;
-    const int t = threadIdx.y * blockDim.x + threadIdx.x;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        s_sum[j * 256 + t] = sum[0][j];
-        if (GATED) s_sum[(8 + j) * 256 + t] = sum[1][j];
+        s_sum[wave][0][lane * 8 + j] = sum[0][j];
+        if (GATED) s_sum[wave][GATED ? 1 : 0][lane * 8 + j] = sum[1][j];
     }
     __syncthreads();
-    if (threadIdx.y == 0 && left > 0) {
+    for (int i = threadIdx.x; i < kSlopeCols; i += 256) {
+        const int64_t col = static_cast<int64_t>(blockIdx.x) * kSlopeCols + i;
+        if (col >= ncols) break;
+        float a = 0.0f, b = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            float a = 0.0f, b = 0.0f;
-            for (unsigned y = 0; y < blockDim.y; ++y) {
-                a += s_sum[j * 256 + y * blockDim.x + threadIdx.x];
-                if (GATED) b += s_sum[(8 + j) * 256 + y * blockDim.x + threadIdx.x];
-            }
-            if (j < left) {
-                sums[blockIdx.y * N + c + j] = a;
-                if (GATED) sums[blockIdx.y * N + ncols + c + j] = b;
-            }
+        for (int v = 0; v < kSlopeWaves; ++v) {
+            a += s_sum[v][0][i];
+            if (GATED) b += s_sum[v][GATED ? 1 : 0][i];
         }
+        sums[blockIdx.y * N + col] = a;
+        if (GATED) sums[blockIdx.y * N + ncols + col] = b;
     }
 }
 
+// The chunks' column sums: a block takes 64 columns, each of its 16 waves every 16th chunk.
 template <typename T>
-__global__ __launch_bounds__(256) void column_sum_kernel(const float *__restrict__ sums, int64_t chunks, int64_t N,
-                                                         T *__restrict__ dB)
+__global__ __launch_bounds__(1024) void column_sum_kernel(const float *__restrict__ sums, int64_t chunks, int64_t N,
+                                                          T *__restrict__ dB)
 {
-    const int64_t c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    if (c >= N) return;
+    __shared__ double s_sum[16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t c = static_cast<int64_t>(blockIdx.x) * 64 + lane;
     double v = 0.0;
-#pragma unroll 8
-    for (int64_t i = 0; i < chunks; ++i) v += sums[i * N + c];
-    dB[c] = from_f32<T>(static_cast<float>(v));
+    if (c < N)
+#pragma unroll 4
+        for (int64_t i = wave; i < chunks; i += 16) v += sums[i * N + c];
+    s_sum[wave][lane] = v;
+    __syncthreads();
+    if (wave == 0 && c < N) {
+#pragma unroll
+        for (int w = 1; w < 16; ++w) v += s_sum[w][lane];
+        dB[c] = from_f32<T>(static_cast<float>(v));
+    }
 }
 
 // The fp32 sums of the k ranges, added in order, through the epilogue.
+constexpr int kJoin = 64;      // few values, long chains of loads: spread over as many CUs as there are
 template <typename T, bool GATED>
-__global__ __launch_bounds__(256) void join_kernel(Epilogue e, int ranges)
+__global__ __launch_bounds__(kJoin) void join_kernel(Epilogue e, int ranges)
 {
     const int64_t chunks = (e.ncols + 7) / 8;
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * kJoin + threadIdx.x;
     if (at >= chunks * e.rows) return;
     const int64_t m = at / chunks, c = (at - m * chunks) * 8;
     float h[8], g[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) h[j] = g[j] = 0.0f;
-    for (int i = 0; i < ranges; ++i) {
-        const float *p = e.part + (i * e.rows + m) * e.pitch + c;
+    const float *p = e.part + m * e.pitch + c;
+    const int64_t step = e.rows * e.pitch;
+    int i = 0;
+    for (; i + 4 <= ranges; i += 4, p += 4 * step) {          // four ranges' loads in flight
+        float v[4][8], u[4][8];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            load8(p + q * step, 8, v[q]);
+            if (GATED) load8(p + q * step + e.pitch / 2, 8, u[q]);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                h[j] += v[q][j];
+                if (GATED) g[j] += u[q][j];
+            }
+    }
+    for (; i < ranges; ++i, p += step) {
         float v[8];
         load8(p, 8, v);
 #pragma unroll
@@ -142,32 +174,54 @@ __global__ __launch_bounds__(256) void join_kernel(Epilogue e, int ranges)
             for (int j = 0; j < 8; ++j) g[j] += v[j];
         }
     }
-    finish8<T, GATED>(e, m, c, h, g);
+    const int64_t left = e.ncols - c;
+    float bh[8], bg[8], res[8];
+    load_bias8<T, GATED>(e, c, bh, bg);
+    if (e.residual) load8(static_cast<const T *>(e.residual) + m * e.ncols + c, left, res);
+    activate8<T, GATED>(e, m, c, left, bh, bg, h, g);
+    if (e.residual) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) h[j] += res[j];
+    }
+    store8(static_cast<T *>(e.Y) + m * e.ncols + c, left, h);
 }
 
-// Tile and k ranges of a product of `rows` x `ncols` outputs (gated: ncols pairs of them) over Kc.
+// Tile and k ranges of a product of `rows` x `ncols` outputs (gated: ncols pairs of them) over Kc; k_rows: both
+// operands hold k along their rows.
 struct Cut {
-    int tile, ranges;
+    Tile tile;
+    int ranges;
     int64_t pitch;      // of the ranges' sums
     size_t bytes;       // of the ranges' sums
 };
-Cut cut_for(int64_t rows, int64_t ncols, int64_t Kc, bool gated, int dtype)
+Cut cut_for(int64_t rows, int64_t ncols, int64_t Kc, bool gated, bool k_rows, int dtype)
 {
-    Cut c{128, 1, 0, 0};
-    const int64_t width = gated ? 2 * ncols : ncols;
-    const int64_t t256 = ceil_div(rows, 256) * ceil_div(width, 256);
-    if (dtype != OPMX_DTYPE_F32 && t256 >= 192) c.tile = 256;
-    if (c.tile == 128) {
-        const int64_t tiles = ceil_div(rows, 128) * ceil_div(width, 128);
-        const int64_t nk = ceil_div(Kc, dtype == OPMX_DTYPE_F32 ? 32 : 64);
-        int64_t r = tiles > 0 ? 512 / tiles : 1;
+    Cut c{Tile::k128, 1, 0, 0};
+    const bool f32 = dtype == OPMX_DTYPE_F32;
+    const int64_t width = gated ? 2 * ncols : ncols, columns = ceil_div(width, 128);
+    int64_t tiles = ceil_div(rows, 128) * columns;
+    const int64_t nk = ceil_div(Kc, f32 ? 32 : 64);
+    if (!f32 && ceil_div(rows, 256) * ceil_div(width, 256) >= 192) {
+        c.tile = Tile::k256;
+    } else if (!k_rows && rows <= 64) {
+        // the weights are read once whatever happens: as many workgroups as LDS holds, at least 4 k-tiles each
+        c.tile = rows <= 32 ? Tile::k32 : Tile::k64;
+        int64_t r = columns > 0 ? 512 / columns : 1;
         if (r > nk / 4) r = nk / 4;
-        if (r > 32) r = 32;
-        if (r > 1) {
-            const int64_t per = ceil_div(nk, r);
-            c.ranges = static_cast<int>(ceil_div(nk, per));
+        c.ranges = static_cast<int>(r < 1 ? 1 : r > 32 ? 32 : r);
+    } else if (tiles > 0 && tiles <= 256) {
+        // A k-tile takes about 0.35 us (fp32 1.8), joining the ranges 8 us, a CU holds one workgroup.
+        c.tile = Tile::k128Deep;
+        double best = 0;
+        for (int64_t r = 1; r <= 16 && r * 4 <= (nk > 4 ? nk : 4); ++r) {
+            const double us = static_cast<double>(ceil_div(tiles * r, 256) * ceil_div(nk, r)) * (f32 ? 1.8 : 0.35) + (r > 1 ? 8.0 : 0.0);
+            if (r == 1 || us < best) {
+                best = us;
+                c.ranges = static_cast<int>(r);
+            }
         }
     }
+    if (c.ranges > 1) c.ranges = static_cast<int>(ceil_div(nk, ceil_div(nk, c.ranges)));      // none of them empty
     if (c.ranges > 1) {
         c.pitch = gated ? 2 * up(ncols, 8) : up(ncols, 8);
         c.bytes = static_cast<size_t>(c.ranges) * rows * c.pitch * 4;
@@ -177,10 +231,10 @@ Cut cut_for(int64_t rows, int64_t ncols, int64_t Kc, bool gated, int dtype)
 
 template <typename T> int join(const Epilogue &e, int ranges, hipStream_t s)
 {
-    const int64_t blocks = ceil_div(ceil_div(e.ncols, 8) * e.rows, 256);
+    const int64_t blocks = ceil_div(ceil_div(e.ncols, 8) * e.rows, kJoin);
     if (blocks >= (int64_t{1} << 31)) return OPMX_ERR_UNSUPPORTED;
-    if (e.act == OPMX_ACTIVATION_SWIGLU) join_kernel<T, true><<<static_cast<unsigned>(blocks), 256, 0, s>>>(e, ranges);
-    else join_kernel<T, false><<<static_cast<unsigned>(blocks), 256, 0, s>>>(e, ranges);
+    if (e.act == OPMX_ACTIVATION_SWIGLU) join_kernel<T, true><<<static_cast<unsigned>(blocks), kJoin, 0, s>>>(e, ranges);
+    else join_kernel<T, false><<<static_cast<unsigned>(blocks), kJoin, 0, s>>>(e, ranges);
     OPMX_LAUNCH_CHECK();
     return OPMX_OK;
 }
@@ -189,7 +243,7 @@ template <typename T>
 int product(const Operand &P, const Operand &Q, int64_t Kc, Epilogue e, void *ws, hipStream_t s)
 {
     const bool gated = e.act == OPMX_ACTIVATION_SWIGLU;
-    const Cut c = cut_for(e.rows, e.ncols, Kc, gated, DType<T>::id);
+    const Cut c = cut_for(e.rows, e.ncols, Kc, gated, Q.k_major, DType<T>::id);
     if (c.ranges > 1) {
         e.part = static_cast<float *>(ws);
         e.pitch = c.pitch;
@@ -211,11 +265,14 @@ inline Lanes lanes_over(int64_t rows, int64_t cols)
             dim3(bx, 256 / bx)};
 }
 
-template <typename T> int pad(const void *X, int64_t R, int64_t C, int64_t pitch, void *out, hipStream_t s)
+template <typename T>
+int pad(const void *X0, int64_t R0, void *out0, const void *X1, int64_t R1, void *out1, int64_t C, hipStream_t s)
 {
-    if (R == 0) return OPMX_OK;
-    const Lanes l = lanes_over(R, pitch);
-    pad_kernel<T><<<l.grid, l.block, 0, s>>>(static_cast<const T *>(X), R, C, pitch, static_cast<T *>(out));
+    const int64_t pitch = up(C, 16 / sizeof(T));
+    Lanes l = lanes_over(R0 > R1 ? R0 : R1, pitch);
+    l.grid.z = X1 ? 2 : 1;
+    pad_kernel<T><<<l.grid, l.block, 0, s>>>(static_cast<const T *>(X0), R0, static_cast<T *>(out0), static_cast<const T *>(X1),
+                                             R1, static_cast<T *>(out1), C, pitch);
     OPMX_LAUNCH_CHECK();
     return OPMX_OK;
 }
@@ -232,16 +289,16 @@ ForwardPlan forward_plan(int64_t Ttok, int64_t K, int64_t N, int dtype, int act)
     p.x = 0;
     p.w = p.x + (padded ? up(Ttok * pitch * esize, 256) : 0);
     p.part = p.w + (padded ? up(N * pitch * esize, 256) : 0);
-    p.total = p.part + up(cut_for(Ttok, gated ? N / 2 : N, K, gated, dtype).bytes, 256);
+    p.total = p.part + up(cut_for(Ttok, gated ? N / 2 : N, K, gated, false, dtype).bytes, 256);
     return p;
 }
 
-// Rows per chunk of the column sums: a few thousand blocks at most, 16 rows a chunk at least.
+// Rows per chunk of the slope pass: 8 (two per wave) while that leaves at most 4096 blocks, then more; 512 chunks at most.
 inline int64_t chunk_rows(int64_t Ttok, int64_t ncols)
 {
-    const int64_t strips = ceil_div(ncols, 2048);
-    int64_t rows = 16;
-    while (ceil_div(Ttok, rows) * strips > 4096 || ceil_div(Ttok, rows) > 512) rows <<= 1;
+    const int64_t strips = ceil_div(ncols, kSlopeCols);
+    int64_t rows = 8;
+    while ((ceil_div(Ttok, rows) * strips > 4096 && rows < 64) || ceil_div(Ttok, rows) > 512) rows <<= 1;
     return rows;
 }
 
@@ -264,7 +321,7 @@ BackwardPlan backward_plan(int64_t Ttok, int64_t K, int64_t N, int dtype, int ac
     p.w = p.x + up(Ttok * p.pitch_k * esize, 256);          // padded, or unpacked from 8 bits
     p.sums = p.w + (p.padded ? up(N * p.pitch_k * esize, 256) : 0);
     p.part = p.sums + up(ceil_div(Ttok, p.chunk) * N * 4, 256);
-    const size_t a = cut_for(Ttok, K, N, false, dtype).bytes, b = cut_for(N, K, Ttok, false, dtype).bytes;
+    const size_t a = cut_for(Ttok, K, N, false, false, dtype).bytes, b = cut_for(N, K, Ttok, false, true, dtype).bytes;
     p.total = p.part + up(a > b ? a : b, 256);
     return p;
 }
@@ -278,8 +335,7 @@ int forward_impl(const void *X, const void *W, const void *B, const void *R, int
     int64_t pitch = K;
     if (K % n != 0) {
         pitch = up(K, n);
-        int rc = pad<T>(X, Ttok, K, pitch, ws + plan.x, s);
-        if (rc == OPMX_OK) rc = pad<T>(W, N, K, pitch, ws + plan.w, s);
+        const int rc = pad<T>(X, Ttok, ws + plan.x, W, N, ws + plan.w, K, s);
         if (rc != OPMX_OK) return rc;
         X = ws + plan.x;
         W = ws + plan.w;
@@ -309,53 +365,50 @@ int backward_impl(const void *dY, const void *X, const void *xq, const void *xco
     if (Ttok > 0 && (want_dh || dB)) {
         T *out = want_dh ? reinterpret_cast<T *>(ws + plan.dh) : nullptr;
         float *sums = dB ? reinterpret_cast<float *>(ws + plan.sums) : nullptr;
-        Lanes l = lanes_over(plan.chunk, gated ? ncols : plan.pitch_n);
-        l.grid.y = static_cast<unsigned>(ceil_div(Ttok, plan.chunk));
+        const dim3 grid(static_cast<unsigned>(ceil_div(ncols, kSlopeCols)), static_cast<unsigned>(ceil_div(Ttok, plan.chunk)));
         if (gated)
-            slope_kernel<T, true><<<l.grid, l.block, 0, s>>>(static_cast<const T *>(dY), H, Ttok, N, ncols,
+            slope_kernel<T, true><<<grid, 256, 0, s>>>(static_cast<const T *>(dY), H, Ttok, N, ncols,
                                                              plan.pitch_n, plan.chunk, act, out, sums);
         else
-            slope_kernel<T, false><<<l.grid, l.block, 0, s>>>(static_cast<const T *>(dY), H, Ttok, N, ncols,
+            slope_kernel<T, false><<<grid, 256, 0, s>>>(static_cast<const T *>(dY), H, Ttok, N, ncols,
                                                               plan.pitch_n, plan.chunk, act, out, sums);
         OPMX_LAUNCH_CHECK();
     }
     if (plan.own_dh) dH = ws + plan.dh;
     if (dB) {
-        column_sum_kernel<T><<<static_cast<unsigned>(ceil_div(N, 256)), 256, 0, s>>>(
+        column_sum_kernel<T><<<static_cast<unsigned>(ceil_div(N, 64)), 1024, 0, s>>>(
             reinterpret_cast<const float *>(ws + plan.sums), ceil_div(Ttok, plan.chunk), N, static_cast<T *>(dB));
         OPMX_LAUNCH_CHECK();
     }
+    // W and X as the products take them
+    int64_t pitch_w = K, pitch_x = K;
+    const bool pad_w = plan.padded && dX, pad_x = plan.padded && dW && !xq && Ttok > 0;
+    if (pad_w && pad_x) rc = pad<T>(W, N, ws + plan.w, X, Ttok, ws + plan.x, K, s);
+    else if (pad_w) rc = pad<T>(W, N, ws + plan.w, nullptr, 0, nullptr, K, s);
+    else if (pad_x) rc = pad<T>(X, Ttok, ws + plan.x, nullptr, 0, nullptr, K, s);
+    if (rc == OPMX_OK && dW && xq) rc = launch_checkpoint8_unpack(xq, xcode, Ttok, K, DType<T>::id, ws + plan.x, s, plan.pitch_k);
+    if (rc != OPMX_OK) return rc;
+    if (pad_w) {
+        W = ws + plan.w;
+        pitch_w = plan.pitch_k;
+    }
+    if (pad_x || (dW && xq)) {
+        X = ws + plan.x;
+        pitch_x = plan.pitch_k;
+    }
     Epilogue e;
     if (dX) {
-        int64_t pitch = K;
-        if (plan.padded) {
-            pitch = plan.pitch_k;
-            rc = pad<T>(W, N, K, pitch, ws + plan.w, s);
-            if (rc != OPMX_OK) return rc;
-            W = ws + plan.w;
-        }
         e.Y = dX;
         e.rows = Ttok;
         e.N = e.ncols = K;
-        rc = product<T>({W, pitch, true}, {dH, plan.pitch_n, false}, N, e, ws + plan.part, s);
+        rc = product<T>({W, pitch_w, true}, {dH, plan.pitch_n, false}, N, e, ws + plan.part, s);
         if (rc != OPMX_OK) return rc;
     }
     if (dW) {
-        int64_t pitch = K;
-        if (xq) {
-            pitch = plan.pitch_k;
-            rc = launch_checkpoint8_unpack(xq, xcode, Ttok, K, DType<T>::id, ws + plan.x, s, pitch);
-            X = ws + plan.x;
-        } else if (plan.padded) {
-            pitch = plan.pitch_k;
-            rc = pad<T>(X, Ttok, K, pitch, ws + plan.x, s);
-            X = ws + plan.x;
-        }
-        if (rc != OPMX_OK) return rc;
         e.Y = dW;
         e.rows = N;
         e.N = e.ncols = K;
-        rc = product<T>({X, pitch, true}, {dH, plan.pitch_n, true}, Ttok, e, ws + plan.part, s);
+        rc = product<T>({X, pitch_x, true}, {dH, plan.pitch_n, true}, Ttok, e, ws + plan.part, s);
     }
     return rc;
 }

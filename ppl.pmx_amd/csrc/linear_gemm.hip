@@ -5,8 +5,8 @@
 //     gradient X   Q = dH [T,N],  P = W [N,K] read as (c = K, k = N): k runs over rows
 //     gradient W   Q = dH [T,N],  P = X [T,K], k = T: k runs over rows in both
 //
-// A workgroup owns a BM x BN tile of C and walks k in tiles of 128 bytes (64 values, 32 in fp32), two LDS buffers,
-// loaded straight into LDS.  P is the A operand of the MFMAs and Q the B operand, so a lane ends up with four
+// A workgroup owns a BM x BN tile of C and walks k in tiles of 128 bytes (64 values, 32 in fp32), loaded straight into
+// LDS and up to three tiles ahead.  P is the A operand of the MFMAs and Q the B operand, so a lane ends up with four
 // neighbouring columns of a row.
 //   rows along k:     LDS [row][8 chunks of 16 bytes], chunk c in slot c ^ (row / 2 % 8): a fragment is one
 //                     16-byte read, conflict free;
@@ -60,6 +60,13 @@ template <typename T> __device__ __forceinline__ int unit_swizzle(int k)
 {
     if constexpr (sizeof(T) == 2) return (k & 3) | ((k >> 3 & 1) << 2);
     else return (k >> 2) & 3;
+}
+
+// Waits until at most N of the wave's loads are outstanding (they land in order) and all its LDS reads are done.
+template <int N> __device__ __forceinline__ void wait_loads()
+{
+    static_assert(N < 64, "the counter has six bits");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
 }
 
 // One operand's share of a thread: LOADS 16-byte pieces of a k-tile of ROWS rows.
@@ -120,14 +127,14 @@ template <typename T, int ROWS, int THREADS, bool KM, bool GATED> struct Loader 
     }
 };
 
-// Eight transposing reads, waited for: four fragments of a k-major tile.  Written as one block because the compiler
-// puts a wait for every outstanding global -> LDS load in front of the builtin (it takes it for a store), and the
-// next k-tile's loads are in flight by design.  a: LDS addresses of the fragments' lanes at k step 0.
+// Transposing reads, waited for: the fragments of four (two) groups of 16 rows of a k-major tile.  One block of assembly
+// because the compiler puts a wait for every outstanding global -> LDS load in front of the builtin (it takes it for a
+// store), and the next k-tiles' loads are in flight by design.  a: LDS addresses of the fragments' lanes at k step 0.
+typedef uint32_t u32pair __attribute__((ext_vector_type(2)));
 template <int KSTEP_BYTES, int HALF_BYTES, typename F>
 __device__ __forceinline__ void transposed4(F *f, const uint32_t *a)
 {
-    typedef uint32_t pair __attribute__((ext_vector_type(2)));
-    pair v[8];
+    u32pair v[8];
     asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%12\n\t"
                  "ds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
                  "ds_read_b64_tr_b16 %2, %9 offset:%12\n\t"
@@ -143,6 +150,21 @@ __device__ __forceinline__ void transposed4(F *f, const uint32_t *a)
 #pragma unroll
     for (int j = 0; j < 4; ++j) __builtin_memcpy(&f[j], &v[2 * j], 16);
 }
+template <int KSTEP_BYTES, int HALF_BYTES, typename F>
+__device__ __forceinline__ void transposed2(F *f, const uint32_t *a)
+{
+    u32pair v[4];
+    asm volatile("ds_read_b64_tr_b16 %0, %4 offset:%6\n\t"
+                 "ds_read_b64_tr_b16 %1, %4 offset:%7\n\t"
+                 "ds_read_b64_tr_b16 %2, %5 offset:%6\n\t"
+                 "ds_read_b64_tr_b16 %3, %5 offset:%7\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3])
+                 : "v"(a[0]), "v"(a[1]), "n"(KSTEP_BYTES), "n"(KSTEP_BYTES + HALF_BYTES)
+                 : "memory");
+#pragma unroll
+    for (int j = 0; j < 2; ++j) __builtin_memcpy(&f[j], &v[2 * j], 16);
+}
 
 // The fragments of N groups of 16 rows from row 16 * row16 on, k step KS (0, 1), of an LDS tile of ROWS rows.
 template <typename T, int ROWS, bool KM, int KS, int N>
@@ -157,16 +179,18 @@ __device__ __forceinline__ void fragments(const char *lds, int row16, int lane, 
             f[i] = *reinterpret_cast<const frag *>(lds + ((row16 + i) * 16 + r) * kTileBytes + slot * 16);
     } else if constexpr (sizeof(T) == 2) {
         // lane r of a group of 16 reads four columns of k row r / 4 and receives four k rows of column r
-        static_assert(N % 4 == 0, "four fragments per block of reads");
+        static_assert(N % 4 == 0 || N == 2, "four or two fragments per block of reads");
+        constexpr int B = N < 4 ? 2 : 4;
         const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(OPMX_LDS(lds)));
         const int k = g * 8 + (r >> 2);             // neither the second half (k + 4) nor KS (k + 32) changes the swizzle
 #pragma unroll
-        for (int i = 0; i < N; i += 4) {
-            uint32_t a[4];
+        for (int i = 0; i < N; i += B) {
+            uint32_t a[B];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < B; ++j)
                 a[j] = base + k * (ROWS * 2) + (((row16 + i + j) ^ unit_swizzle<T>(k)) << 5) + (r & 3) * 8;
-            transposed4<KS * 32 * ROWS * 2, 4 * ROWS * 2>(f + i, a);
+            if constexpr (B == 4) transposed4<KS * 32 * ROWS * 2, 4 * ROWS * 2>(f + i, a);
+            else transposed2<KS * 32 * ROWS * 2, 4 * ROWS * 2>(f + i, a);
         }
     } else {
 #pragma unroll
@@ -193,14 +217,15 @@ __device__ __forceinline__ void place(int64_t id, int64_t mt, int64_t nt, int64_
     c = in / high;
 }
 
-template <typename T, int BM, int BN, int WM, int WN, bool PK, bool QK, bool GATED>
-__global__ __launch_bounds__(WM *WN *kWave) void linear_gemm_kernel(Operand P, Operand Q, int64_t Kc, Epilogue e, int64_t mt,
+template <typename T, int BM, int BN, int WM, int WN, int STAGES, bool PK, bool QK, bool GATED>
+__global__ __launch_bounds__(WM *WN *kWave, 2) void linear_gemm_kernel(Operand P, Operand Q, int64_t Kc, Epilogue e, int64_t mt,
                                                                     int64_t nt, int64_t ktiles_per_range)
 {
     constexpr int THREADS = WM * WN * kWave, WTM = BM / WM, WTN = BN / WN, TM = WTM / 16, TN = WTN / 16;
     constexpr int STAGE = (BM + BN) * kTileBytes, BK = kTileBytes / sizeof(T);
     constexpr int BNO = GATED ? BN / 2 : BN;
-    static_assert(WTN == 64 && (TM == 4 || TM == 8), "the epilogue stages 64 x 64 pieces");
+    constexpr int PIECE = WTM < 64 ? WTM : 64;
+    static_assert(WTN == 64 && (TM == 2 || TM == 4 || TM == 8), "the epilogue stages pieces of 64 columns");
     using frag = typename Step<T>::frag;
     extern __shared__ __attribute__((aligned(16))) char smem[];
 
@@ -235,10 +260,11 @@ __global__ __launch_bounds__(WM *WN *kWave) void linear_gemm_kernel(Operand P, O
     };
     auto half = [&](const char *cur, auto ks_tag, auto h_tag, const frag (&p)[TN]) {
         constexpr int KS = decltype(ks_tag)::value, H = decltype(h_tag)::value;
-        frag q[4];
-        fragments<T, BM, QK, KS, 4>(cur, wm * TM + H * 4, lane, q);
+        constexpr int C = TM < 4 ? TM : 4;
+        frag q[C];
+        fragments<T, BM, QK, KS, C>(cur, wm * TM + H * 4, lane, q);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < C; ++i)
 #pragma unroll
             for (int j = 0; j < TN; ++j) acc[j][H * 4 + i] = Step<T>::mma(p[j], q[i], acc[j][H * 4 + i]);
     };
@@ -248,60 +274,116 @@ __global__ __launch_bounds__(WM *WN *kWave) void linear_gemm_kernel(Operand P, O
         half(cur, ks_tag, std::integral_constant<int, 0>{}, p);
         if constexpr (TM == 8) half(cur, ks_tag, std::integral_constant<int, 1>{}, p);
     };
-    load(smem, klen);
-    __syncthreads();                                       // waits for the loads as well
+    // STAGES - 1 k-tiles are on their way at any time.  Past the last one the loads go on, from nowhere, so that the
+    // number of outstanding ones that means "tile kt has landed" stays the same.
+    constexpr int AHEAD = (STAGES - 2) * (decltype(lp)::LOADS + decltype(lq)::LOADS);
+    int64_t k_left = klen;
+    int fill = 0;                                          // the stage that the next tile goes to
+    auto load_next = [&]() {
+        load(smem + fill * STAGE, k_left);
+        k_left -= BK;
+        fill = fill + 1 == STAGES ? 0 : fill + 1;
+    };
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) load_next();
+    int stage = 0;
     for (int kt = 0; kt < nk; ++kt) {
-        const char *cur = smem + (kt & 1) * STAGE;
-        if (kt + 1 < nk) load(smem + ((kt + 1) & 1) * STAGE, klen - static_cast<int64_t>(kt + 1) * BK);
+        wait_loads<AHEAD>();                               // this wave's loads of tile kt, and its reads of tile kt - 1
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        load_next();                                       // into the stage that tile kt - 1 was in
+        const char *cur = smem + stage * STAGE;
         multiply(cur, std::integral_constant<int, 0>{});
         multiply(cur, std::integral_constant<int, 1>{});
-        __syncthreads();
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
     }
+    wait_loads<0>();                                       // the epilogue uses the same memory
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
 
-    // The wave's columns go through LDS in pieces of 64 x 64 fp32 values of its own (16-byte chunks xored with the
+    // The wave's columns go through LDS in pieces of (up to) 64 x 64 fp32 values of its own (16-byte chunks xored with the
     // row), so that a lane then has eight neighbouring columns of a row.
-    char *mine = smem + wave * (64 * 256);
+    char *mine = smem + wave * (PIECE * 256);
     const int r = lane & 15, g = lane >> 4;
+    constexpr int PER_ROW = GATED ? 4 : 8, ROWS = kWave / PER_ROW;       // lanes per row, rows per trip
+    const int c8 = lane % PER_ROW;
+    const int64_t c = c0 + wn * (GATED ? 32 : 64) + c8 * 8, left = e.ncols - c;
+    auto staged = [&](int row, int chunk) { return reinterpret_cast<float4_t *>(mine + row * 256 + ((chunk ^ (row & 15)) << 4)); };
+    float bias_h[8], bias_g[8];
+    load_bias8<T, GATED>(e, c, bias_h, bias_g);
 #pragma unroll
-    for (int piece = 0; piece < WTM / 64; ++piece) {
+    for (int piece = 0; piece < WTM / PIECE; ++piece) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < PIECE / 16; ++i)
 #pragma unroll
             for (int j = 0; j < TN; ++j)
-                *reinterpret_cast<float4_t *>(mine + (i * 16 + r) * 256 + (((j * 4 + g) ^ r) << 4)) = acc[j][piece * 4 + i];
+                *staged(i * 16 + r, j * 4 + g) = acc[j][piece * (PIECE / 16) + i];
         asm volatile("" ::: "memory");
         __builtin_amdgcn_wave_barrier();
-        constexpr int PER_ROW = GATED ? 4 : 8, ROWS = kWave / PER_ROW;       // lanes per row, rows per trip
-#pragma unroll 1
-        for (int t = 0; t < 64 / ROWS; ++t) {
-            const int row = t * ROWS + lane / PER_ROW, c8 = lane % PER_ROW;
-            float h[8], gate[8];
+        if (e.part) {
+#pragma unroll 2
+            for (int t = 0; t < PIECE / ROWS; ++t) {
+                const int row = t * ROWS + lane / PER_ROW;
+                const int64_t m = m0 + wm * WTM + piece * PIECE + row;
+                if (m >= e.rows || left <= 0) continue;
+                float *at = e.part + (blockIdx.y * e.rows + m) * e.pitch + c;      // whole chunks: the pitch holds them
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const float4_t v = *reinterpret_cast<const float4_t *>(mine + row * 256 + (((c8 * 2 + x) ^ (row & 15)) << 4));
-#pragma unroll
-                for (int y = 0; y < 4; ++y) h[x * 4 + y] = v[y];
-                if (GATED) {
-                    const float4_t u = *reinterpret_cast<const float4_t *>(mine + row * 256 + (((8 + c8 * 2 + x) ^ (row & 15)) << 4));
-#pragma unroll
-                    for (int y = 0; y < 4; ++y) gate[x * 4 + y] = u[y];
+                for (int x = 0; x < 2; ++x) {
+                    *reinterpret_cast<float4_any *>(at + x * 4) = *staged(row, c8 * 2 + x);
+                    if (GATED) *reinterpret_cast<float4_any *>(at + e.pitch / 2 + x * 4) = *staged(row, 8 + c8 * 2 + x);
                 }
             }
-            const int64_t m = m0 + wm * WTM + piece * 64 + row;
-            const int64_t c = c0 + wn * (GATED ? 32 : 64) + c8 * 8;
-            if (m < e.rows && c < e.ncols) {
-                if (e.part) {
-                    // whole chunks: the pitch holds them
-                    float *at = e.part + (blockIdx.y * e.rows + m) * e.pitch + c;
+        } else {
+            const bool shaped = GATED || e.act != OPMX_ACTIVATION_NONE || e.H;
+            if (shaped) {
+                // in place, in a rolled loop: the code of eight activations once
+#pragma unroll 1
+                for (int t = 0; t < PIECE / ROWS; ++t) {
+                    const int row = t * ROWS + lane / PER_ROW;
+                    const int64_t m = m0 + wm * WTM + piece * PIECE + row;
+                    if (m >= e.rows || left <= 0) continue;
+                    float h[8], gate[8];
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        *reinterpret_cast<float4_any *>(at + x * 4) = float4_any{h[x * 4], h[x * 4 + 1], h[x * 4 + 2], h[x * 4 + 3]};
-                        if (GATED)
-                            *reinterpret_cast<float4_any *>(at + e.pitch / 2 + x * 4) =
-                                float4_any{gate[x * 4], gate[x * 4 + 1], gate[x * 4 + 2], gate[x * 4 + 3]};
+                        const float4_t v = *staged(row, c8 * 2 + x);
+                        const float4_t u = GATED ? *staged(row, 8 + c8 * 2 + x) : v;
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) {
+                            h[x * 4 + y] = v[y];
+                            gate[x * 4 + y] = u[y];
+                        }
                     }
-                } else {
-                    finish8<T, GATED>(e, m, c, h, gate);
+                    activate8<T, GATED>(e, m, c, left, bias_h, bias_g, h, gate);
+#pragma unroll
+                    for (int x = 0; x < 2; ++x)
+                        *staged(row, c8 * 2 + x) = float4_t{h[x * 4], h[x * 4 + 1], h[x * 4 + 2], h[x * 4 + 3]};
+                }
+            }
+            constexpr int GROUP = PIECE / ROWS < 4 ? PIECE / ROWS : 4;              // residual rows in flight
+#pragma unroll 1
+            for (int t0 = 0; t0 < PIECE / ROWS; t0 += GROUP) {
+                float res[GROUP][8];
+#pragma unroll
+                for (int t = 0; t < GROUP; ++t) {
+                    const int64_t m = m0 + wm * WTM + piece * PIECE + (t0 + t) * ROWS + lane / PER_ROW;
+                    if (e.residual && m < e.rows && left > 0)
+                        load8(static_cast<const T *>(e.residual) + m * e.ncols + c, left, res[t]);
+                }
+#pragma unroll
+                for (int t = 0; t < GROUP; ++t) {
+                    const int row = (t0 + t) * ROWS + lane / PER_ROW;
+                    const int64_t m = m0 + wm * WTM + piece * PIECE + row;
+                    if (m >= e.rows || left <= 0) continue;
+                    float h[8];
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const float4_t v = *staged(row, c8 * 2 + x);
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) h[x * 4 + y] = v[y];
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) h[j] += (shaped ? 0.0f : bias_h[j]) + (e.residual ? res[t][j] : 0.0f);
+                    store8(static_cast<T *>(e.Y) + m * e.ncols + c, left, h);
                 }
             }
         }
@@ -310,46 +392,57 @@ __global__ __launch_bounds__(WM *WN *kWave) void linear_gemm_kernel(Operand P, O
     }
 }
 
-template <typename T, int BM, int BN, int WM, int WN, bool PK, bool QK, bool GATED>
+template <typename T, int BM, int BN, int WM, int WN, int STAGES, bool PK, bool QK, bool GATED>
 int launch(const Operand &P, const Operand &Q, int64_t Kc, const Epilogue &e, int ranges, hipStream_t s)
 {
-    constexpr int BNO = GATED ? BN / 2 : BN, BK = kTileBytes / sizeof(T), SMEM = 2 * (BM + BN) * kTileBytes;
+    constexpr int BNO = GATED ? BN / 2 : BN, BK = kTileBytes / sizeof(T), SMEM = STAGES * (BM + BN) * kTileBytes;
     const int64_t mt = ceil_div(e.rows, BM), nt = ceil_div(e.ncols, BNO), nk = ceil_div(Kc, BK);
     const int64_t per = nk > 0 ? ceil_div(nk, ranges) : 1;
     const int64_t used = nk > 0 ? ceil_div(nk, per) : 1;    // every range holds at least one k-tile
     if (mt * nt == 0) return OPMX_OK;
     if (mt * nt >= (int64_t{1} << 31) || used > 65535 || (ranges > 1 && used != ranges)) return OPMX_ERR_UNSUPPORTED;
     static std::atomic<uint64_t> done{0};
-    const void *k = reinterpret_cast<const void *>(&linear_gemm_kernel<T, BM, BN, WM, WN, PK, QK, GATED>);
+    const void *k = reinterpret_cast<const void *>(&linear_gemm_kernel<T, BM, BN, WM, WN, STAGES, PK, QK, GATED>);
     if (!ensure_dynamic_smem(k, SMEM, done)) return OPMX_ERR_LAUNCH;
-    linear_gemm_kernel<T, BM, BN, WM, WN, PK, QK, GATED>
+    linear_gemm_kernel<T, BM, BN, WM, WN, STAGES, PK, QK, GATED>
         <<<dim3(static_cast<unsigned>(mt * nt), static_cast<unsigned>(used)), WM * WN * kWave, SMEM, s>>>(P, Q, Kc, e, mt, nt, per);
     OPMX_LAUNCH_CHECK();
     return OPMX_OK;
 }
 
-template <typename T, int BM, int BN, int WM, int WN>
+template <typename T, int BM, int BN, int WM, int WN, int STAGES>
 int by_layout(const Operand &P, const Operand &Q, int64_t Kc, const Epilogue &e, int ranges, hipStream_t s)
 {
-    if (e.act == OPMX_ACTIVATION_SWIGLU) return launch<T, BM, BN, WM, WN, false, false, true>(P, Q, Kc, e, ranges, s);
-    if (!P.k_major) return launch<T, BM, BN, WM, WN, false, false, false>(P, Q, Kc, e, ranges, s);
-    if (!Q.k_major) return launch<T, BM, BN, WM, WN, true, false, false>(P, Q, Kc, e, ranges, s);
-    return launch<T, BM, BN, WM, WN, true, true, false>(P, Q, Kc, e, ranges, s);
+    if (e.act == OPMX_ACTIVATION_SWIGLU) return launch<T, BM, BN, WM, WN, STAGES, false, false, true>(P, Q, Kc, e, ranges, s);
+    if (!P.k_major) return launch<T, BM, BN, WM, WN, STAGES, false, false, false>(P, Q, Kc, e, ranges, s);
+    if (!Q.k_major) return launch<T, BM, BN, WM, WN, STAGES, true, false, false>(P, Q, Kc, e, ranges, s);
+    if constexpr (BM >= 128) return launch<T, BM, BN, WM, WN, STAGES, true, true, false>(P, Q, Kc, e, ranges, s);
+    return OPMX_ERR_UNSUPPORTED;
+}
+
+template <typename T> int by_tile(const Operand &P, const Operand &Q, int64_t Kc, const Epilogue &e, Tile tile, int ranges, hipStream_t s)
+{
+    switch (tile) {
+        case Tile::k256:
+            if constexpr (sizeof(T) == 2) return by_layout<T, 256, 256, 2, 4, 2>(P, Q, Kc, e, ranges, s);
+            break;
+        case Tile::k128: return by_layout<T, 128, 128, 2, 2, 2>(P, Q, Kc, e, ranges, s);
+        case Tile::k128Deep: return by_layout<T, 128, 128, 4, 2, 4>(P, Q, Kc, e, ranges, s);
+        case Tile::k64: return by_layout<T, 64, 128, 2, 2, 3>(P, Q, Kc, e, ranges, s);
+        case Tile::k32: return by_layout<T, 32, 128, 1, 2, 4>(P, Q, Kc, e, ranges, s);
+    }
+    return OPMX_ERR_UNSUPPORTED;
 }
 
 }  // namespace
 
-int launch_linear_gemm(const Operand &P, const Operand &Q, int64_t Kc, int dtype, const Epilogue &e, int tile, int ranges,
+int launch_linear_gemm(const Operand &P, const Operand &Q, int64_t Kc, int dtype, const Epilogue &e, Tile tile, int ranges,
                        hipStream_t s)
 {
     switch (dtype) {
-        case OPMX_DTYPE_F32: return by_layout<float, 128, 128, 2, 2>(P, Q, Kc, e, ranges, s);
-        case OPMX_DTYPE_F16:
-            return tile == 256 ? by_layout<f16, 256, 256, 2, 4>(P, Q, Kc, e, ranges, s)
-                               : by_layout<f16, 128, 128, 2, 2>(P, Q, Kc, e, ranges, s);
-        case OPMX_DTYPE_BF16:
-            return tile == 256 ? by_layout<bf16, 256, 256, 2, 4>(P, Q, Kc, e, ranges, s)
-                               : by_layout<bf16, 128, 128, 2, 2>(P, Q, Kc, e, ranges, s);
+        case OPMX_DTYPE_F32: return by_tile<float>(P, Q, Kc, e, tile, ranges, s);
+        case OPMX_DTYPE_F16: return by_tile<f16>(P, Q, Kc, e, tile, ranges, s);
+        case OPMX_DTYPE_BF16: return by_tile<bf16>(P, Q, Kc, e, tile, ranges, s);
     }
     return OPMX_ERR_UNSUPPORTED;
 }

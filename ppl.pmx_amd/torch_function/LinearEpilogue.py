@@ -43,9 +43,9 @@ class LinearEpilogue(torch.autograd.Function):
         keep_h = activation != "none" and any(need[:3])
         L = _lib.lib()
         with _lib.on_device(dev):
-            Xc, Wc = _dense(X.detach()), _dense(W.detach())
-            Bc = None if B is None else B.detach().contiguous()
-            Rc = None if residual is None else residual.detach().contiguous()
+            Xc, Wc = _dense(X), _dense(W)           # (autograd records nothing in here)
+            Bc = None if B is None else B.contiguous()
+            Rc = None if residual is None else residual.contiguous()
             Y = torch.empty(*lead, M, dtype=W.dtype, device=dev)
             H = torch.empty(L.opmx_linear_epilogue_kept_bytes(T, N, dt), dtype=torch.uint8, device=dev) if keep_h else None
             nbytes = L.opmx_linear_epilogue_workspace_bytes(T, K, N, dt, act)

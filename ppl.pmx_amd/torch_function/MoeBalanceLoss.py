@@ -28,9 +28,10 @@ class MoeBalanceLoss(torch.autograd.Function):
             loss = torch.empty((), dtype=torch.float32, device=dev)
             count = torch.empty(E, dtype=torch.int64, device=dev)
             weight = torch.empty(E, dtype=torch.float32, device=dev)
-            ws = _lib.workspace(L.opmx_moe_balance_loss_workspace_bytes(T, E), dev)
+            nbytes = L.opmx_moe_balance_loss_workspace_bytes(T, E)
+            ws = _lib.workspace(nbytes, dev) if nbytes > 256 else None
             _lib.check(L.opmx_moe_balance_loss(_lib.ptr(sc), _lib.ptr(mc), T, E, k, dt, _lib.ptr(loss), _lib.ptr(count),
-                                               _lib.ptr(weight), _lib.ptr(ws), ws.numel(), _lib.stream_ptr(dev)),
+                                               _lib.ptr(weight), _lib.ptr(ws), nbytes, _lib.stream_ptr(dev)),
                        "moe_balance_loss")
         if ctx.needs_input_grad[0]:
             # a contiguous input is saved as itself, so autograd notices a change in place before the backward pass
