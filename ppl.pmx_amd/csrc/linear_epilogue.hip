@@ -138,10 +138,11 @@ constexpr int kJoin = 64;      // few values, long chains of loads: spread over 
 template <typename T, bool GATED>
 __global__ __launch_bounds__(kJoin) void join_kernel(Epilogue e, int ranges)
 {
-    const int64_t chunks = (e.ncols + 7) / 8;
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * kJoin + threadIdx.x;
-    if (at >= chunks * e.rows) return;
-    const int64_t m = at / chunks, c = (at - m * chunks) * 8;
+    // (fewer than 2^31 values in ranges' sums of one range: see cut_for; a 64-bit division would cost a microsecond)
+    const uint32_t chunks = static_cast<uint32_t>((e.ncols + 7) / 8), at = blockIdx.x * kJoin + threadIdx.x;
+    const uint32_t row = at / chunks;
+    if (row >= static_cast<uint64_t>(e.rows)) return;
+    const int64_t m = row, c = static_cast<int64_t>(at - row * chunks) * 8;
     float h[8], g[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) h[j] = g[j] = 0.0f;
@@ -232,7 +233,7 @@ Cut cut_for(int64_t rows, int64_t ncols, int64_t Kc, bool gated, bool k_rows, in
 template <typename T> int join(const Epilogue &e, int ranges, hipStream_t s)
 {
     const int64_t blocks = ceil_div(ceil_div(e.ncols, 8) * e.rows, kJoin);
-    if (blocks >= (int64_t{1} << 31)) return OPMX_ERR_UNSUPPORTED;
+    if (blocks >= (int64_t{1} << 25)) return OPMX_ERR_UNSUPPORTED;      // 32-bit counts in the kernel
     if (e.act == OPMX_ACTIVATION_SWIGLU) join_kernel<T, true><<<static_cast<unsigned>(blocks), kJoin, 0, s>>>(e, ranges);
     else join_kernel<T, false><<<static_cast<unsigned>(blocks), kJoin, 0, s>>>(e, ranges);
     OPMX_LAUNCH_CHECK();

@@ -112,7 +112,7 @@ template <typename T, int ROWS, int THREADS, bool KM, bool GATED> struct Loader 
         }
     }
     // Loads piece i of the current k-tile, of which k_left values exist, to lds + its place.
-    __device__ __forceinline__ void issue(int i, char *lds, int64_t k_left) const
+    __device__ __forceinline__ void issue(int i, char *lds, int k_left) const
     {
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
         const int piece0 = i * THREADS + wave * kWave;                       // of the wave: uniform
@@ -205,21 +205,122 @@ __device__ __forceinline__ void fragments(const char *lds, int row16, int lane, 
 
 // Tile ids to tiles.  Ids go round the 8 XCDs; each XCD takes a contiguous eighth of the tiles, in bands of 8
 // row tiles walked column by column, so that the 32 workgroups an XCD runs share 8 + 4 operand tiles in its L2.
-__device__ __forceinline__ void place(int64_t id, int64_t mt, int64_t nt, int64_t &m, int64_t &c)
+// (32-bit throughout: a launch has fewer than 2^31 tiles, and a 64-bit division takes microseconds of a lone wave.)
+__device__ __forceinline__ void place(uint32_t id, uint32_t mt, uint32_t nt, int64_t &m, int64_t &c)
 {
-    const int64_t total = mt * nt, per = total / 8, rest = total % 8;
-    const int64_t x = id % 8;
-    const int64_t t = x * per + (x < rest ? x : rest) + id / 8;
-    const int64_t band = t / (8 * nt), first = band * 8;
-    const int64_t high = mt - first < 8 ? mt - first : 8;
-    const int64_t in = t - band * 8 * nt;
-    m = first + in % high;
-    c = in / high;
+    const uint32_t total = mt * nt, per = total / 8, rest = total % 8, x = id % 8;
+    const uint32_t t = x * per + (x < rest ? x : rest) + id / 8;
+    const uint32_t band = t / (8 * nt), first = band * 8;
+    const uint32_t high = mt - first < 8 ? mt - first : 8;
+    const uint32_t in = t - band * 8 * nt, col = in / high;
+    m = first + (in - col * high);
+    c = col;
+}
+
+// What becomes of a wave's tile: acc[j][i] holds row 16 i + lane % 16 and columns 16 j + 4 (lane / 16) + v.  It goes through
+// LDS in pieces of (up to) 64 x 64 fp32 values of the wave's own (16-byte chunks xored with the row), so that a lane
+// then has eight neighbouring columns of a row.  m0, c0: the first row and (output) column.
+template <typename T, int TM, int TN, bool GATED>
+__device__ __forceinline__ void write_columns(const float4_t (&acc)[TN][TM], const Epilogue &e, int64_t m0, int64_t c0, int lane,
+                                              char *mine)
+{
+    constexpr int PIECE = TM < 4 ? TM * 16 : 64, DOWN = TM * 16 / PIECE, PIECES = DOWN * (TN / 4);
+    const int r = lane & 15, g = lane >> 4;
+    constexpr int PER_ROW = GATED ? 4 : 8, ROWS = kWave / PER_ROW;       // lanes per row, rows per trip
+    const int c8 = lane % PER_ROW;
+    auto staged = [&](int row, int chunk) { return reinterpret_cast<float4_t *>(mine + row * 256 + ((chunk ^ (row & 15)) << 4)); };
+#pragma unroll 1
+    for (int p = 0; p < PIECES; ++p) {                   // (the code behind the staging stands once)
+        const int piece = p % DOWN;
+        const int64_t c = c0 + p / DOWN * (GATED ? 32 : 64) + c8 * 8, left = e.ncols - c;
+        float bias_h[8], bias_g[8];
+        load_bias8<T, GATED>(e, c, bias_h, bias_g);
+#pragma unroll
+        for (int u = 0; u < PIECES; ++u)
+            if (p == u) {
+#pragma unroll
+                for (int i = 0; i < PIECE / 16; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        *staged(i * 16 + r, j * 4 + g) = acc[u / DOWN * 4 + j][u % DOWN * (PIECE / 16) + i];
+            }
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_wave_barrier();
+        if (e.part) {
+#pragma unroll 2
+            for (int t = 0; t < PIECE / ROWS; ++t) {
+                const int row = t * ROWS + lane / PER_ROW;
+                const int64_t m = m0 + piece * PIECE + row;
+                if (m >= e.rows || left <= 0) continue;
+                float *at = e.part + (blockIdx.y * e.rows + m) * e.pitch + c;      // whole chunks: the pitch holds them
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    *reinterpret_cast<float4_any *>(at + x * 4) = *staged(row, c8 * 2 + x);
+                    if (GATED) *reinterpret_cast<float4_any *>(at + e.pitch / 2 + x * 4) = *staged(row, 8 + c8 * 2 + x);
+                }
+            }
+        } else {
+            const bool shaped = GATED || e.act != OPMX_ACTIVATION_NONE || e.H;
+            if (shaped) {
+                // in place, in a rolled loop: the code of eight activations once
+#pragma unroll 1
+                for (int t = 0; t < PIECE / ROWS; ++t) {
+                    const int row = t * ROWS + lane / PER_ROW;
+                    const int64_t m = m0 + piece * PIECE + row;
+                    if (m >= e.rows || left <= 0) continue;
+                    float h[8], gate[8];
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const float4_t v = *staged(row, c8 * 2 + x);
+                        const float4_t u = GATED ? *staged(row, 8 + c8 * 2 + x) : v;
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) {
+                            h[x * 4 + y] = v[y];
+                            gate[x * 4 + y] = u[y];
+                        }
+                    }
+                    activate8<T, GATED>(e, m, c, left, bias_h, bias_g, h, gate);
+#pragma unroll
+                    for (int x = 0; x < 2; ++x)
+                        *staged(row, c8 * 2 + x) = float4_t{h[x * 4], h[x * 4 + 1], h[x * 4 + 2], h[x * 4 + 3]};
+                }
+            }
+            constexpr int GROUP = PIECE / ROWS < 4 ? PIECE / ROWS : 4;              // residual rows in flight
+#pragma unroll 1
+            for (int t0 = 0; t0 < PIECE / ROWS; t0 += GROUP) {
+                float res[GROUP][8];
+#pragma unroll
+                for (int t = 0; t < GROUP; ++t) {
+                    const int64_t m = m0 + piece * PIECE + (t0 + t) * ROWS + lane / PER_ROW;
+                    if (e.residual && m < e.rows && left > 0)
+                        load8(static_cast<const T *>(e.residual) + m * e.ncols + c, left, res[t]);
+                }
+#pragma unroll
+                for (int t = 0; t < GROUP; ++t) {
+                    const int row = (t0 + t) * ROWS + lane / PER_ROW;
+                    const int64_t m = m0 + piece * PIECE + row;
+                    if (m >= e.rows || left <= 0) continue;
+                    float h[8];
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const float4_t v = *staged(row, c8 * 2 + x);
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) h[x * 4 + y] = v[y];
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) h[j] += (shaped ? 0.0f : bias_h[j]) + (e.residual ? res[t][j] : 0.0f);
+                    store8(static_cast<T *>(e.Y) + m * e.ncols + c, left, h);
+                }
+            }
+        }
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_wave_barrier();
+    }
 }
 
 template <typename T, int BM, int BN, int WM, int WN, int STAGES, bool PK, bool QK, bool GATED>
-__global__ __launch_bounds__(WM *WN *kWave, 2) void linear_gemm_kernel(Operand P, Operand Q, int64_t Kc, Epilogue e, int64_t mt,
-                                                                    int64_t nt, int64_t ktiles_per_range)
+__global__ __launch_bounds__(WM *WN *kWave, 2) void linear_gemm_kernel(Operand P, Operand Q, int64_t Kc, Epilogue e, uint32_t mt,
+                                                                    uint32_t nt, int64_t ktiles_per_range)
 {
     constexpr int THREADS = WM * WN * kWave, WTM = BM / WM, WTN = BN / WN, TM = WTM / 16, TN = WTN / 16;
     constexpr int STAGE = (BM + BN) * kTileBytes, BK = kTileBytes / sizeof(T);
@@ -250,7 +351,8 @@ __global__ __launch_bounds__(WM *WN *kWave, 2) void linear_gemm_kernel(Operand P
 #pragma unroll
         for (int i = 0; i < TM; ++i) acc[j][i] = float4_t{0.f, 0.f, 0.f, 0.f};
 
-    auto load = [&](char *stage, int64_t left) {
+    auto load = [&](char *stage, int64_t k_left) {
+        const int left = k_left < BK ? static_cast<int>(k_left) : BK;
 #pragma unroll
         for (int i = 0; i < lq.LOADS; ++i) lq.issue(i, stage, left);
 #pragma unroll
@@ -301,95 +403,318 @@ __global__ __launch_bounds__(WM *WN *kWave, 2) void linear_gemm_kernel(Operand P
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 
-    // The wave's columns go through LDS in pieces of (up to) 64 x 64 fp32 values of its own (16-byte chunks xored with the
-    // row), so that a lane then has eight neighbouring columns of a row.
-    char *mine = smem + wave * (PIECE * 256);
-    const int r = lane & 15, g = lane >> 4;
-    constexpr int PER_ROW = GATED ? 4 : 8, ROWS = kWave / PER_ROW;       // lanes per row, rows per trip
-    const int c8 = lane % PER_ROW;
-    const int64_t c = c0 + wn * (GATED ? 32 : 64) + c8 * 8, left = e.ncols - c;
-    auto staged = [&](int row, int chunk) { return reinterpret_cast<float4_t *>(mine + row * 256 + ((chunk ^ (row & 15)) << 4)); };
-    float bias_h[8], bias_g[8];
-    load_bias8<T, GATED>(e, c, bias_h, bias_g);
-#pragma unroll
-    for (int piece = 0; piece < WTM / PIECE; ++piece) {
-#pragma unroll
-        for (int i = 0; i < PIECE / 16; ++i)
-#pragma unroll
-            for (int j = 0; j < TN; ++j)
-                *staged(i * 16 + r, j * 4 + g) = acc[j][piece * (PIECE / 16) + i];
-        asm volatile("" ::: "memory");
-        __builtin_amdgcn_wave_barrier();
-        if (e.part) {
-#pragma unroll 2
-            for (int t = 0; t < PIECE / ROWS; ++t) {
-                const int row = t * ROWS + lane / PER_ROW;
-                const int64_t m = m0 + wm * WTM + piece * PIECE + row;
-                if (m >= e.rows || left <= 0) continue;
-                float *at = e.part + (blockIdx.y * e.rows + m) * e.pitch + c;      // whole chunks: the pitch holds them
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    *reinterpret_cast<float4_any *>(at + x * 4) = *staged(row, c8 * 2 + x);
-                    if (GATED) *reinterpret_cast<float4_any *>(at + e.pitch / 2 + x * 4) = *staged(row, 8 + c8 * 2 + x);
-                }
-            }
-        } else {
-            const bool shaped = GATED || e.act != OPMX_ACTIVATION_NONE || e.H;
-            if (shaped) {
-                // in place, in a rolled loop: the code of eight activations once
-#pragma unroll 1
-                for (int t = 0; t < PIECE / ROWS; ++t) {
-                    const int row = t * ROWS + lane / PER_ROW;
-                    const int64_t m = m0 + wm * WTM + piece * PIECE + row;
-                    if (m >= e.rows || left <= 0) continue;
-                    float h[8], gate[8];
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const float4_t v = *staged(row, c8 * 2 + x);
-                        const float4_t u = GATED ? *staged(row, 8 + c8 * 2 + x) : v;
-#pragma unroll
-                        for (int y = 0; y < 4; ++y) {
-                            h[x * 4 + y] = v[y];
-                            gate[x * 4 + y] = u[y];
-                        }
-                    }
-                    activate8<T, GATED>(e, m, c, left, bias_h, bias_g, h, gate);
-#pragma unroll
-                    for (int x = 0; x < 2; ++x)
-                        *staged(row, c8 * 2 + x) = float4_t{h[x * 4], h[x * 4 + 1], h[x * 4 + 2], h[x * 4 + 3]};
-                }
-            }
-            constexpr int GROUP = PIECE / ROWS < 4 ? PIECE / ROWS : 4;              // residual rows in flight
-#pragma unroll 1
-            for (int t0 = 0; t0 < PIECE / ROWS; t0 += GROUP) {
-                float res[GROUP][8];
-#pragma unroll
-                for (int t = 0; t < GROUP; ++t) {
-                    const int64_t m = m0 + wm * WTM + piece * PIECE + (t0 + t) * ROWS + lane / PER_ROW;
-                    if (e.residual && m < e.rows && left > 0)
-                        load8(static_cast<const T *>(e.residual) + m * e.ncols + c, left, res[t]);
-                }
-#pragma unroll
-                for (int t = 0; t < GROUP; ++t) {
-                    const int row = (t0 + t) * ROWS + lane / PER_ROW;
-                    const int64_t m = m0 + wm * WTM + piece * PIECE + row;
-                    if (m >= e.rows || left <= 0) continue;
-                    float h[8];
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const float4_t v = *staged(row, c8 * 2 + x);
-#pragma unroll
-                        for (int y = 0; y < 4; ++y) h[x * 4 + y] = v[y];
-                    }
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) h[j] += (shaped ? 0.0f : bias_h[j]) + (e.residual ? res[t][j] : 0.0f);
-                    store8(static_cast<T *>(e.Y) + m * e.ncols + c, left, h);
-                }
-            }
-        }
-        asm volatile("" ::: "memory");
-        __builtin_amdgcn_wave_barrier();
+    write_columns<T, TM, TN, GATED>(acc, e, m0 + wm * WTM, c0 + wn * (GATED ? 32 : 64), lane, smem + wave * (PIECE * 256));
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// The product of many rows (16-bit types): 256 x 256 tiles, four waves of 128 x 128.
+//
+// Against eight waves of 128 x 64 the wave tiles read a third less from LDS per operation: with eight, reads and
+// arriving loads together keep LDS busy for all of the 2048 clocks that the matrix units take per k-tile.  One wave
+// per SIMD has to overlap by itself: the 64 MFMAs of a k step (32 values) go in four blocks of 16, and each block
+// reads four of the sixteen fragments of the next step behind its first MFMAs and waits for them at its end.  The
+// accumulators fill the 256 accumulation registers.  A block is one piece of assembly: its order is the issue order,
+// the wait stands where the reads are, and the compiler's own wait in front of transposing reads does not come in.
+//
+// Step 0 of k-tile t reads the fragments of step 1 from the same stage; after it all waves have read all of the stage.
+// Between the steps a wave waits for its loads of k-tile t + 1 (issued a k-tile ago) and for the other waves; step 1
+// then reads the first fragments of k-tile t + 1 from the other stage and loads k-tile t + 2 into this one.
+#define OPMX_WIDE_ROWS(OP)                                                                                            \
+    asm volatile("s_nop 1\n\t"                                                                                        \
+                 "v_mfma_f32_16x16x32_" OP " %0, %20, %24, %0\n\t"                                                    \
+                 "ds_read_b128 %16, %28 offset:%29\n\t"                                                               \
+                 "v_mfma_f32_16x16x32_" OP " %1, %21, %24, %1\n\t"                                                    \
+                 "v_mfma_f32_16x16x32_" OP " %2, %22, %24, %2\n\t"                                                    \
+                 "ds_read_b128 %17, %28 offset:%30\n\t"                                                               \
+                 "v_mfma_f32_16x16x32_" OP " %3, %23, %24, %3\n\t"                                                    \
+                 "v_mfma_f32_16x16x32_" OP " %4, %20, %25, %4\n\t"                                                    \
+                 "ds_read_b128 %18, %28 offset:%31\n\t"                                                               \
+                 "v_mfma_f32_16x16x32_" OP " %5, %21, %25, %5\n\t"                                                    \
+                 "v_mfma_f32_16x16x32_" OP " %6, %22, %25, %6\n\t"                                                    \
+                 "ds_read_b128 %19, %28 offset:%32\n\t"                                                               \
+                 "v_mfma_f32_16x16x32_" OP " %7, %23, %25, %7\n\t"                                                    \
+                 "v_mfma_f32_16x16x32_" OP " %8, %20, %26, %8\n\t"                                                    \
+                 "v_mfma_f32_16x16x32_" OP " %9, %21, %26, %9\n\t"                                                    \
+                 "v_mfma_f32_16x16x32_" OP " %10, %22, %26, %10\n\t"                                                  \
+                 "v_mfma_f32_16x16x32_" OP " %11, %23, %26, %11\n\t"                                                  \
+                 "v_mfma_f32_16x16x32_" OP " %12, %20, %27, %12\n\t"                                                  \
+                 "v_mfma_f32_16x16x32_" OP " %13, %21, %27, %13\n\t"                                                  \
+                 "v_mfma_f32_16x16x32_" OP " %14, %22, %27, %14\n\t"                                                  \
+                 "v_mfma_f32_16x16x32_" OP " %15, %23, %27, %15\n\t"                                                  \
+                 "s_waitcnt lgkmcnt(0)"                                                                               \
+                 : "+a"(acc[PH * 4 + 0][QH * 4 + 0]), "+a"(acc[PH * 4 + 1][QH * 4 + 0]), "+a"(acc[PH * 4 + 2][QH * 4  \
+                 + 0]), "+a"(acc[PH * 4 + 3][QH * 4 + 0]), "+a"(acc[PH * 4 + 0][QH * 4 + 1]), "+a"(acc[PH * 4 + 1][QH \
+                 * 4 + 1]), "+a"(acc[PH * 4 + 2][QH * 4 + 1]), "+a"(acc[PH * 4 + 3][QH * 4 + 1]), "+a"(acc[PH * 4 +   \
+                 0][QH * 4 + 2]), "+a"(acc[PH * 4 + 1][QH * 4 + 2]), "+a"(acc[PH * 4 + 2][QH * 4 + 2]), "+a"(acc[PH * \
+                 4 + 3][QH * 4 + 2]), "+a"(acc[PH * 4 + 0][QH * 4 + 3]), "+a"(acc[PH * 4 + 1][QH * 4 + 3]),           \
+                 "+a"(acc[PH * 4 + 2][QH * 4 + 3]), "+a"(acc[PH * 4 + 3][QH * 4 + 3]), "=&v"(f[F0 + 0]), "=&v"(f[F0 + \
+                 1]), "=&v"(f[F0 + 2]), "=&v"(f[F0 + 3])                                                              \
+                 : "v"(p[PH * 4 + 0]), "v"(p[PH * 4 + 1]), "v"(p[PH * 4 + 2]), "v"(p[PH * 4 + 3]), "v"(q[QH * 4 +     \
+                 0]), "v"(q[QH * 4 + 1]), "v"(q[QH * 4 + 2]), "v"(q[QH * 4 + 3]), "v"(at[0]), "n"((F0 + 0) * 2048),   \
+                 "n"((F0 + 1) * 2048), "n"((F0 + 2) * 2048), "n"((F0 + 3) * 2048)                                     \
+                 : "memory")
+#define OPMX_WIDE_COLUMNS(OP)                                                                                         \
+    asm volatile("s_nop 1\n\t"                                                                                        \
+                 "v_mfma_f32_16x16x32_" OP " %0, %24, %28, %0\n\t"                                                    \
+                 "ds_read_b64_tr_b16 %16, %32 offset:%36\n\t"                                                         \
+                 "v_mfma_f32_16x16x32_" OP " %1, %25, %28, %1\n\t"                                                    \
+                 "ds_read_b64_tr_b16 %17, %32 offset:%37\n\t"                                                         \
+                 "v_mfma_f32_16x16x32_" OP " %2, %26, %28, %2\n\t"                                                    \
+                 "ds_read_b64_tr_b16 %18, %33 offset:%36\n\t"                                                         \
+                 "v_mfma_f32_16x16x32_" OP " %3, %27, %28, %3\n\t"                                                    \
+                 "ds_read_b64_tr_b16 %19, %33 offset:%37\n\t"                                                         \
+                 "v_mfma_f32_16x16x32_" OP " %4, %24, %29, %4\n\t"                                                    \
+                 "ds_read_b64_tr_b16 %20, %34 offset:%36\n\t"                                                         \
+                 "v_mfma_f32_16x16x32_" OP " %5, %25, %29, %5\n\t"                                                    \
+                 "ds_read_b64_tr_b16 %21, %34 offset:%37\n\t"                                                         \
+                 "v_mfma_f32_16x16x32_" OP " %6, %26, %29, %6\n\t"                                                    \
+                 "ds_read_b64_tr_b16 %22, %35 offset:%36\n\t"                                                         \
+                 "v_mfma_f32_16x16x32_" OP " %7, %27, %29, %7\n\t"                                                    \
+                 "ds_read_b64_tr_b16 %23, %35 offset:%37\n\t"                                                         \
+                 "v_mfma_f32_16x16x32_" OP " %8, %24, %30, %8\n\t"                                                    \
+                 "v_mfma_f32_16x16x32_" OP " %9, %25, %30, %9\n\t"                                                    \
+                 "v_mfma_f32_16x16x32_" OP " %10, %26, %30, %10\n\t"                                                  \
+                 "v_mfma_f32_16x16x32_" OP " %11, %27, %30, %11\n\t"                                                  \
+                 "v_mfma_f32_16x16x32_" OP " %12, %24, %31, %12\n\t"                                                  \
+                 "v_mfma_f32_16x16x32_" OP " %13, %25, %31, %13\n\t"                                                  \
+                 "v_mfma_f32_16x16x32_" OP " %14, %26, %31, %14\n\t"                                                  \
+                 "v_mfma_f32_16x16x32_" OP " %15, %27, %31, %15\n\t"                                                  \
+                 "s_waitcnt lgkmcnt(0)"                                                                               \
+                 : "+a"(acc[PH * 4 + 0][QH * 4 + 0]), "+a"(acc[PH * 4 + 1][QH * 4 + 0]), "+a"(acc[PH * 4 + 2][QH * 4  \
+                 + 0]), "+a"(acc[PH * 4 + 3][QH * 4 + 0]), "+a"(acc[PH * 4 + 0][QH * 4 + 1]), "+a"(acc[PH * 4 + 1][QH \
+                 * 4 + 1]), "+a"(acc[PH * 4 + 2][QH * 4 + 1]), "+a"(acc[PH * 4 + 3][QH * 4 + 1]), "+a"(acc[PH * 4 +   \
+                 0][QH * 4 + 2]), "+a"(acc[PH * 4 + 1][QH * 4 + 2]), "+a"(acc[PH * 4 + 2][QH * 4 + 2]), "+a"(acc[PH * \
+                 4 + 3][QH * 4 + 2]), "+a"(acc[PH * 4 + 0][QH * 4 + 3]), "+a"(acc[PH * 4 + 1][QH * 4 + 3]),           \
+                 "+a"(acc[PH * 4 + 2][QH * 4 + 3]), "+a"(acc[PH * 4 + 3][QH * 4 + 3]), "=&v"(v[0]), "=&v"(v[1]),      \
+                 "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7])                         \
+                 : "v"(p[PH * 4 + 0]), "v"(p[PH * 4 + 1]), "v"(p[PH * 4 + 2]), "v"(p[PH * 4 + 3]), "v"(q[QH * 4 +     \
+                 0]), "v"(q[QH * 4 + 1]), "v"(q[QH * 4 + 2]), "v"(q[QH * 4 + 3]), "v"(at[0]), "v"(at[1]), "v"(at[2]), \
+                 "v"(at[3]), "n"(KS * 16384), "n"(KS * 16384 + 2048)                                                  \
+                 : "memory")
+
+// acc[PH * 4 + j][QH * 4 + i] += p[PH * 4 + j] q[QH * 4 + i], and the fragments F0 ... F0 + 3 of the next step into f.  KM:
+// from a k-major tile, at[0 ... 3] their LDS addresses at k step 0; else at[0] the address of fragment 0 at the step.
+// The two wait states in front: the compiler may have moved a fragment just before, and does not see MFMAs in assembly.
+#define OPMX_WIDE_BLOCK(T, OP)                                                                                        \
+    template <int PH, int QH, int F0, bool KM, int KS>                                                                \
+    __device__ __forceinline__ void wide_block(float4_t (&acc)[8][8], const Step<T>::frag (&p)[8],                    \
+                                               const Step<T>::frag (&q)[8], Step<T>::frag (&f)[8], const uint32_t *at) \
+    {                                                                                                                 \
+        if constexpr (KM) {                                                                                           \
+            u32pair v[8];                                                                                             \
+            OPMX_WIDE_COLUMNS(OP);                                                                                    \
+            _Pragma("unroll") for (int j = 0; j < 4; ++j) __builtin_memcpy(&f[F0 + j], &v[2 * j], 16);                \
+        } else {                                                                                                      \
+            OPMX_WIDE_ROWS(OP);                                                                                       \
+        }                                                                                                             \
     }
+OPMX_WIDE_BLOCK(f16, "f16")
+OPMX_WIDE_BLOCK(bf16, "bf16")
+
+// LDS addresses of a lane's fragments of one operand: first = the wave's first row / 16 (a multiple of 8), base = the
+// tile's address.
+template <bool KM> struct WideReader {
+    uint32_t a[KM ? 8 : 2];
+    __device__ __forceinline__ void init(uint32_t base, int first, int lane)
+    {
+        const int r = lane & 15, g = lane >> 4;
+        if constexpr (KM) {
+            const int k = g * 8 + (r >> 2);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                a[i] = base + k * 512 + (((first + i) ^ unit_swizzle<f16>(k)) << 5) + (r & 3) * 8;
+        } else {
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) a[ks] = base + (first * 16 + r) * kTileBytes + (((ks * 4 + g) ^ ((r >> 1) & 7)) << 4);
+        }
+    }
+    // for the fragments F0 ... F0 + 3 of k step KS in the stage at `stage` bytes
+    template <int F0, int KS> __device__ __forceinline__ void at(uint32_t stage, uint32_t (&out)[4]) const
+    {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) out[i] = (KM ? a[KM ? F0 + i : 0] : a[KM ? 0 : KS]) + stage;
+    }
+};
+
+template <typename T, bool PK, bool QK, bool GATED>
+__global__ __launch_bounds__(256, 1) void linear_gemm_wide_kernel(Operand P, Operand Q, int64_t Kc, Epilogue e, uint32_t mt,
+                                                                  uint32_t nt)
+{
+    constexpr int BM = 256, BN = 256, STAGE = (BM + BN) * kTileBytes, BK = kTileBytes / sizeof(T);
+    using frag = typename Step<T>::frag;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+
+    int64_t tm, tc;
+    place(blockIdx.x, mt, nt, tm, tc);
+    const int64_t m0 = tm * BM, c0 = tc * (GATED ? BN / 2 : BN);
+    const int nk = static_cast<int>((Kc + BK - 1) / BK);
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int wm = wave >> 1, wn = wave & 1;
+
+    Loader<T, BN, 256, PK, GATED> lp;
+    Loader<T, BM, 256, QK, false> lq;
+    lp.init(P, c0, e.ncols, 0);
+    lq.init(Q, m0, e.rows, 0);
+    WideReader<PK> rp;
+    WideReader<QK> rq;
+    const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(OPMX_LDS(smem)));
+    rp.init(lds + BM * kTileBytes, wn * 8, lane);
+    rq.init(lds, wm * 8, lane);
+
+    float4_t acc[8][8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[j][i] = float4_t{0.f, 0.f, 0.f, 0.f};
+
+    int64_t k_left = Kc;
+    // pieces [4 Q4, 4 Q4 + 4) of the sixteen of the next k-tile to be loaded
+    auto load4 = [&](char *stage, auto q4) {
+        constexpr int Q4 = decltype(q4)::value;
+        const int left = k_left < BK ? static_cast<int>(k_left) : BK;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (Q4 < 2) lq.issue(Q4 * 4 + i, stage, left);
+            else lp.issue((Q4 - 2) * 4 + i, stage + BM * kTileBytes, left);
+        }
+        if constexpr (Q4 == 3) {
+            lq.next();
+            lp.next();
+            k_left -= BK;
+        }
+    };
+    using I0 = std::integral_constant<int, 0>;
+    using I1 = std::integral_constant<int, 1>;
+    using I2 = std::integral_constant<int, 2>;
+    using I3 = std::integral_constant<int, 3>;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        char *stage = smem + t * STAGE;
+        load4(stage, I0{});
+        load4(stage, I1{});
+        load4(stage, I2{});
+        load4(stage, I3{});
+    }
+    wait_loads<16>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    frag pa[8], qa[8], pb[8], qb[8];                     // of step 0 and of step 1
+    fragments<T, BN, PK, 0, 8>(smem + BM * kTileBytes, wn * 8, lane, pa);
+    fragments<T, BM, QK, 0, 8>(smem, wm * 8, lane, qa);
+
+    uint32_t cur = 0, at[4];
+    if constexpr (!PK && !QK) {
+        // Rows along k on both sides: fragments are ordinary reads, so every MFMA can be its own piece of assembly and the
+        // compiler's waits are exact.  Step 0 reads the other step's fragments behind its first 32 MFMAs, then the
+        // stage is free and the loads of k-tile t + 2 go out, one behind every third MFMA, until a sixth of the way
+        // into step 1; in its middle k-tile t + 1 must have landed, almost one and a half k-tiles after its loads.
+        const char *p0 = smem + BM * kTileBytes, *q0 = smem;
+        const int r = lane & 15, g = lane >> 4;
+        const int slot[2] = {(g ^ ((r >> 1) & 7)) << 4, ((4 + g) ^ ((r >> 1) & 7)) << 4};
+        const int rowp = (wn * 128 + r) * kTileBytes, rowq = (wm * 128 + r) * kTileBytes;
+        auto read = [&](uint32_t stage, int ks, int i, frag (&p)[8], frag (&q)[8]) {
+            if (i < 8) p[i < 8 ? i : 0] = *reinterpret_cast<const frag *>(p0 + stage + rowp + slot[ks] + (i & 7) * 16 * kTileBytes);
+            else q[i < 8 ? 0 : i - 8] = *reinterpret_cast<const frag *>(q0 + stage + rowq + slot[ks] + (i & 7) * 16 * kTileBytes);
+        };
+        for (int kt = 0; kt < nk; ++kt) {
+            const int left = k_left < BK ? static_cast<int>(k_left) : BK;
+            char *free_stage = smem + cur;
+            auto load1 = [&](int i) {
+                if (i < 8) lq.issue(i < 8 ? i : 0, free_stage, left);
+                else lp.issue(i < 8 ? 0 : i - 8, free_stage + BM * kTileBytes, left);
+            };
+#pragma unroll
+            for (int m = 0; m < 64; ++m) {
+                Mfma<T>::m16_acc(pa[m % 8], qa[m / 8], acc[m % 8][m / 8]);
+                if (m < 32 && m % 2 == 0) read(cur, 1, m / 2, pb, qb);
+                if (m == 40) {
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                    __builtin_amdgcn_s_barrier();
+                    asm volatile("" ::: "memory");
+                }
+                if (m > 40 && (m - 41) % 5 == 0) load1((m - 41) / 5);
+            }
+#pragma unroll
+            for (int m = 0; m < 64; ++m) {
+                Mfma<T>::m16_acc(pb[m % 8], qb[m / 8], acc[m % 8][m / 8]);
+                                if (m == 32) {
+                    asm volatile("s_waitcnt vmcnt(11)" ::: "memory");
+                    __builtin_amdgcn_s_barrier();
+                    asm volatile("" ::: "memory");
+                }
+                if (m < 53 && (m - 2) % 5 == 0) load1(5 + (m - 2) / 5);
+                if (m > 32 && m % 2 == 1) read(cur ^ STAGE, 0, (m - 33) / 2, pa, qa);
+            }
+            lq.next();
+            lp.next();
+            k_left -= BK;
+            cur ^= STAGE;
+        }
+    } else
+    for (int kt = 0; kt < nk; ++kt) {
+        rp.template at<0, 1>(cur, at);
+        wide_block<0, 0, 0, PK, 1>(acc, pa, qa, pb, at);
+        rp.template at<4, 1>(cur, at);
+        wide_block<1, 0, 4, PK, 1>(acc, pa, qa, pb, at);
+        rq.template at<0, 1>(cur, at);
+        wide_block<0, 1, 0, QK, 1>(acc, pa, qa, qb, at);
+        rq.template at<4, 1>(cur, at);
+        wide_block<1, 1, 4, QK, 1>(acc, pa, qa, qb, at);
+
+        wait_loads<0>();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+
+        char *free_stage = smem + cur;
+        cur ^= STAGE;
+        load4(free_stage, I0{});
+        rp.template at<0, 0>(cur, at);
+        wide_block<0, 0, 0, PK, 0>(acc, pb, qb, pa, at);
+        load4(free_stage, I1{});
+        rp.template at<4, 0>(cur, at);
+        wide_block<1, 0, 4, PK, 0>(acc, pb, qb, pa, at);
+        load4(free_stage, I2{});
+        rq.template at<0, 0>(cur, at);
+        wide_block<0, 1, 0, QK, 0>(acc, pb, qb, qa, at);
+        load4(free_stage, I3{});
+        rq.template at<4, 0>(cur, at);
+        wide_block<1, 1, 4, QK, 0>(acc, pb, qb, qa, at);
+    }
+    // The last MFMAs retire before anything touches an accumulator: the compiler does not know of them.  The empty
+    // statements make every use of one come after the wait.
+    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) asm volatile("" : "+a"(acc[j][i]));
+    wait_loads<0>();                                     // the epilogue uses the same memory
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    write_columns<T, 8, 8, GATED>(acc, e, m0 + wm * 128, c0 + wn * (GATED ? 64 : 128), lane, smem + wave * (64 * 256));
+}
+
+template <typename T, bool PK, bool QK, bool GATED>
+int launch_wide(const Operand &P, const Operand &Q, int64_t Kc, const Epilogue &e, hipStream_t s)
+{
+    constexpr int SMEM = 2 * 512 * kTileBytes;
+    const int64_t mt = ceil_div(e.rows, 256), nt = ceil_div(e.ncols, GATED ? 128 : 256);
+    if (mt * nt == 0) return OPMX_OK;
+    if (mt * nt >= (int64_t{1} << 31)) return OPMX_ERR_UNSUPPORTED;
+    static std::atomic<uint64_t> done{0};
+    const void *k = reinterpret_cast<const void *>(&linear_gemm_wide_kernel<T, PK, QK, GATED>);
+    if (!ensure_dynamic_smem(k, SMEM, done)) return OPMX_ERR_LAUNCH;
+    linear_gemm_wide_kernel<T, PK, QK, GATED><<<static_cast<unsigned>(mt * nt), 256, SMEM, s>>>(
+        P, Q, Kc, e, static_cast<uint32_t>(mt), static_cast<uint32_t>(nt));
+    OPMX_LAUNCH_CHECK();
+    return OPMX_OK;
+}
+
+template <typename T> int by_layout_wide(const Operand &P, const Operand &Q, int64_t Kc, const Epilogue &e, hipStream_t s)
+{
+    if (e.act == OPMX_ACTIVATION_SWIGLU) return launch_wide<T, false, false, true>(P, Q, Kc, e, s);
+    if (!P.k_major) return launch_wide<T, false, false, false>(P, Q, Kc, e, s);
+    if (!Q.k_major) return launch_wide<T, true, false, false>(P, Q, Kc, e, s);
+    return launch_wide<T, true, true, false>(P, Q, Kc, e, s);
 }
 
 template <typename T, int BM, int BN, int WM, int WN, int STAGES, bool PK, bool QK, bool GATED>
@@ -405,7 +730,8 @@ int launch(const Operand &P, const Operand &Q, int64_t Kc, const Epilogue &e, in
     const void *k = reinterpret_cast<const void *>(&linear_gemm_kernel<T, BM, BN, WM, WN, STAGES, PK, QK, GATED>);
     if (!ensure_dynamic_smem(k, SMEM, done)) return OPMX_ERR_LAUNCH;
     linear_gemm_kernel<T, BM, BN, WM, WN, STAGES, PK, QK, GATED>
-        <<<dim3(static_cast<unsigned>(mt * nt), static_cast<unsigned>(used)), WM * WN * kWave, SMEM, s>>>(P, Q, Kc, e, mt, nt, per);
+        <<<dim3(static_cast<unsigned>(mt * nt), static_cast<unsigned>(used)), WM * WN * kWave, SMEM, s>>>(
+            P, Q, Kc, e, static_cast<uint32_t>(mt), static_cast<uint32_t>(nt), per);
     OPMX_LAUNCH_CHECK();
     return OPMX_OK;
 }
@@ -424,7 +750,8 @@ template <typename T> int by_tile(const Operand &P, const Operand &Q, int64_t Kc
 {
     switch (tile) {
         case Tile::k256:
-            if constexpr (sizeof(T) == 2) return by_layout<T, 256, 256, 2, 4, 2>(P, Q, Kc, e, ranges, s);
+            if constexpr (sizeof(T) == 2)
+                if (ranges == 1) return by_layout_wide<T>(P, Q, Kc, e, s);
             break;
         case Tile::k128: return by_layout<T, 128, 128, 2, 2, 2>(P, Q, Kc, e, ranges, s);
         case Tile::k128Deep: return by_layout<T, 128, 128, 4, 2, 4>(P, Q, Kc, e, ranges, s);
