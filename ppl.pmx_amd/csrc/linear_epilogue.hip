@@ -207,7 +207,7 @@ Cut cut_for(int64_t rows, int64_t ncols, int64_t Kc, bool gated, bool k_rows, in
     } else if (!k_rows && rows <= 64) {
         // the weights are read once whatever happens: as many workgroups as LDS holds, at least 4 k-tiles each
         c.tile = rows <= 32 ? Tile::k32 : Tile::k64;
-        int64_t r = columns > 0 ? 512 / columns : 1;
+        int64_t r = columns > 0 && columns < 192 ? 512 / columns : 1;
         if (r > nk / 4) r = nk / 4;
         c.ranges = static_cast<int>(r < 1 ? 1 : r > 32 ? 32 : r);
     } else if (tiles > 0 && tiles <= 256) {
@@ -287,6 +287,7 @@ ForwardPlan forward_plan(int64_t Ttok, int64_t K, int64_t N, int dtype, int act)
     const int64_t esize = dtype == OPMX_DTYPE_F32 ? 4 : 2, n = 16 / esize, pitch = up(K, n);
     const bool gated = act == OPMX_ACTIVATION_SWIGLU, padded = K % n != 0;
     ForwardPlan p{};
+    if (linear_few_rows_serve(Ttok, K, N, dtype)) return p;
     p.x = 0;
     p.w = p.x + (padded ? up(Ttok * pitch * esize, 256) : 0);
     p.part = p.w + (padded ? up(N * pitch * esize, 256) : 0);
@@ -332,15 +333,6 @@ int forward_impl(const void *X, const void *W, const void *B, const void *R, int
                  void *Y, void *H, char *ws, hipStream_t s)
 {
     constexpr int64_t n = 16 / sizeof(T);
-    const ForwardPlan plan = forward_plan(Ttok, K, N, DType<T>::id, act);
-    int64_t pitch = K;
-    if (K % n != 0) {
-        pitch = up(K, n);
-        const int rc = pad<T>(X, Ttok, ws + plan.x, W, N, ws + plan.w, K, s);
-        if (rc != OPMX_OK) return rc;
-        X = ws + plan.x;
-        W = ws + plan.w;
-    }
     Epilogue e;
     e.bias = B;
     e.residual = R;
@@ -350,6 +342,16 @@ int forward_impl(const void *X, const void *W, const void *B, const void *R, int
     e.N = N;
     e.ncols = act == OPMX_ACTIVATION_SWIGLU ? N / 2 : N;
     e.act = act;
+    if (linear_few_rows_serve(Ttok, K, N, DType<T>::id)) return launch_linear_few_rows(X, W, K, DType<T>::id, e, s);
+    const ForwardPlan plan = forward_plan(Ttok, K, N, DType<T>::id, act);
+    int64_t pitch = K;
+    if (K % n != 0) {
+        pitch = up(K, n);
+        const int rc = pad<T>(X, Ttok, ws + plan.x, W, N, ws + plan.w, K, s);
+        if (rc != OPMX_OK) return rc;
+        X = ws + plan.x;
+        W = ws + plan.w;
+    }
     return product<T>({W, pitch, false}, {X, pitch, false}, K, e, ws + plan.part, s);
 }
 

@@ -128,6 +128,15 @@ def test_few_rows_and_long_sums(dtype, act, T, K, N):
     check(T, K, N, dtype, act, train=T not in (1, 16))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act,T,K,N", [("none", 1, 4096, 1100), ("gelu", 16, 4104, 1040), ("swiglu", 3, 4120, 1090),
+                                       ("swiglu", 16, 264, 16500), ("silu", 7, 264, 16402), ("none", 1, 8 << 10, 513),
+                                       ("none", 20, 4096, 1100), ("swiglu", 32, 4099, 1030)])
+def test_weights_streamed_by_few_rows(dtype, act, T, K, N):
+    check(T, K, N, dtype, act, train=False)
+    check(T, K, N, dtype, act, bias=False, residual=False, train=False)
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("act,T,K,N", [("none", 3600, 136, 3400), ("swiglu", 3333, 200, 3600), ("gelu", 3500, 77, 3335)])
 def test_large_tiles(dtype, act, T, K, N):

@@ -82,10 +82,10 @@ def test_balance_loss_c_interface():
 def test_linear_epilogue_c_interface():
     L = _lib.lib()
     odd = ctypes.c_void_p(258)
-    need = L.opmx_linear_epilogue_workspace_bytes(64, 4000, 512, 1, 0)
+    need = L.opmx_linear_epilogue_workspace_bytes(100, 4000, 512, 1, 0)
     assert need % 256 == 0 and need > 256            # cut along k
 
-    def call(X=ONE, W=ONE, T=64, K=4000, N=512, dtype=1, act=0, Y=ONE, ws=ONE, bytes_=need):
+    def call(X=ONE, W=ONE, T=100, K=4000, N=512, dtype=1, act=0, Y=ONE, ws=ONE, bytes_=need):
         return L.opmx_linear_epilogue(X, W, None, None, T, K, N, dtype, act, Y, None, ws, bytes_, None)
 
     assert call(T=-1) == -1 and call(K=-1) == -1 and call(K=0) == -1 and call(act=5) == -1 and call(act=-1) == -1
