@@ -22,28 +22,29 @@ namespace opmx {
 namespace {
 
 constexpr int kMaxBlocks = 256;
+__host__ __device__ inline int pitch_of(int E) { return (E + 3) / 4 * 4; }      // of a block's sums
 
+// A key orders scores as MoeSelect does: NaN first, -0 equal to +0.  No key is 0 or 2^32 - 1.
 template <typename T> struct Key {
     static constexpr bool unique = true;     // 16 bits of score, 16 bits of id
     static __device__ __forceinline__ uint32_t of(T v, int id)
     {
-        uint16_t u;
-        __builtin_memcpy(&u, &v, 2);
-        const float f = to_f32(v);
-        if (f != f) u = 0xFFFFu;
-        else if (f == 0.0f) u = 0x8000u;
-        else u = (u & 0x8000u) ? static_cast<uint16_t>(~u) : static_cast<uint16_t>(u | 0x8000u);
-        return (static_cast<uint32_t>(u) << 16) | (0xFFFFu - static_cast<uint32_t>(id));
+        uint16_t b;
+        __builtin_memcpy(&b, &v, 2);
+        uint32_t u = b;
+        u = u == 0x8000u ? 0u : u;
+        u ^= (u & 0x8000u) ? 0xFFFFu : 0x8000u;
+        u = v != v ? 0xFFFEu : u;
+        return (u << 16) | (0xFFFFu - static_cast<uint32_t>(id));
     }
 };
 template <> struct Key<float> {
     static constexpr bool unique = false;
     static __device__ __forceinline__ uint32_t of(float f, int)
     {
-        if (f != f) return 0xFFFFFFFFu;
-        const uint32_t u = __float_as_uint(f);
-        if (f == 0.0f) return 0x80000000u;
-        return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+        const uint32_t u = __float_as_uint(f + 0.0f);
+        const uint32_t key = u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
+        return f != f ? 0xFFFFFFFEu : key;
     }
 };
 
@@ -65,6 +66,14 @@ template <int D, typename U> __device__ __forceinline__ U other_half(U v)
     else if constexpr (D == 4) return dpp<0x141>(v);    // row_half_mirror
     else if constexpr (D == 8) return dpp<0x140>(v);    // row_mirror
     else return __shfl_xor(v, D, kWave);
+}
+// The value D lanes before in a group, 0 for the group's first D lanes.
+template <int D, int L> __device__ __forceinline__ int lanes_before(int v, int lane)
+{
+    int o;
+    if constexpr (L <= 16) o = dpp<0x110 + D>(v);       // row_shr D: a group lies within a row of 16 lanes
+    else o = __shfl_up(v, D, kWave);
+    return lane >= D ? o : 0;
 }
 // Sum over the lanes that are equal mod L (a power of two), in every one of them.
 template <int L, typename U> __device__ __forceinline__ U sum_mod(U v)
@@ -93,54 +102,58 @@ __device__ __forceinline__ uint32_t umin_(uint32_t a, uint32_t b) { return a < b
 // The id of a lane's i-th score: chunks of N consecutive ids go round the L lanes of the token.
 template <int N, int L> __device__ __forceinline__ int expert_of(int i, int lane) { return ((i / N) * L + lane) * N + i % N; }
 
-// A lane's V scores of token t as floats; experts past E read as -inf.  keys (KEYS) get 0 there, which no
-// score's key is.
+// A lane's V scores of a token as floats; experts past E, and all of a token that does not count, read as -inf.  keys
+// (KEYS) get 0 there.
 template <typename T, int N, int V, int L, bool KEYS>
-__device__ __forceinline__ void load_scores(const T *__restrict__ row, int E, int lane, float (&z)[V],
+__device__ __forceinline__ void load_scores(const T *__restrict__ row, int E, int lane, bool keep, float (&z)[V],
                                             uint32_t (&key)[KEYS ? V : 1])
 {
+    T v[V];
+#pragma unroll
+    for (int c = 0; c < V / N; ++c) {        // E % N == 0: a chunk is whole or absent, and then the last one is read
+        const int e0 = (c * L + lane) * N, at = e0 < E ? e0 : E - N;
+        if constexpr (N == 1) v[c] = row[at];
+        else {
+            const Vec16<T> q = load16_once(row + at);
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[c * N + j] = q.v[j];
+        }
+    }
 #pragma unroll
     for (int c = 0; c < V / N; ++c) {
         const int e0 = (c * L + lane) * N;
-        T v[N];
-        const bool in = e0 < E;              // E % N == 0: a chunk is whole or absent
-        if (in) {
-            if constexpr (N == 1) v[0] = row[e0];
-            else {
-                const Vec16<T> q = load16_once(row + e0);
-#pragma unroll
-                for (int j = 0; j < N; ++j) v[j] = q.v[j];
-            }
-        }
+        const bool in = keep && e0 < E;
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            z[c * N + j] = in ? to_f32(v[j]) : -INFINITY;
-            if constexpr (KEYS) key[c * N + j] = in ? Key<T>::of(v[j], e0 + j) : 0u;
+            const int i = c * N + j;
+            z[i] = in ? to_f32(v[i]) : -INFINITY;
+            if constexpr (KEYS) key[i] = in ? Key<T>::of(v[i], e0 + j) : 0u;
         }
     }
 }
 
-// z -> softmax over the token's L lanes.  The hardware's exp2: z - m and its product with log2 e are off by |z - m|
-// 2^-24 each, so is the result, plus an ulp.
-template <int V, int L> __device__ __forceinline__ void softmax_(float (&z)[V])
+// z -> e^(z - max) over the token's L lanes; the value returned takes them to the softmax.  The hardware's exp2: z - max and its
+// product with log2 e are off by |z - max| 2^-24 each, so is the result, plus an ulp.  (One fma of z would do, but not
+// for masks of the type's lowest value.)  A row of -inf alone gives 0; a NaN or an infinity makes all of the row NaN.
+template <int V, int L> __device__ __forceinline__ float exp_(float (&z)[V])
 {
+    constexpr float kLog2e = 1.44269504088896341f;
     float m = z[0];
 #pragma unroll
     for (int i = 1; i < V; ++i) m = fmaxf(m, z[i]);
 #define OPMX_MAX(D) m = fmaxf(m, other_half<D>(m))
     OPMX_HALVES(OPMX_MAX);
-    const bool nothing = m == -INFINITY;     // (a NaN among the scores is not: it makes the sum NaN below)
+    const bool nothing = m == -INFINITY;
+    m = nothing ? 0.0f : m;
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        z[i] = z[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((z[i] - m) * 1.44269504088896341f);
+        z[i] = __builtin_amdgcn_exp2f((z[i] - m) * kLog2e);
         sum += z[i];
     }
 #define OPMX_SUM(D) sum += other_half<D>(sum)
     OPMX_HALVES(OPMX_SUM);
-    const float r = nothing && sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-    for (int i = 0; i < V; ++i) z[i] *= r;
+    return nothing ? 0.0f : __builtin_amdgcn_rcpf(sum);
 }
 
 // Inserts x into the list a[0] >= a[1] >= ..., dropping the smallest.
@@ -190,22 +203,24 @@ __device__ __forceinline__ void finish(double psum, int64_t count, int64_t kept,
     const double n = kept > 0 ? static_cast<double>(kept) : 1.0;
     double part = 0.0;
     if (e < E) {
-        const double f = static_cast<double>(count) / (static_cast<double>(k) * n);
-        part = static_cast<double>(E) * f * (psum / n);
+        const double weight = static_cast<double>(E) * static_cast<double>(count) / (static_cast<double>(k) * n * n);   // E f / n
+        part = weight * psum;
         counts[e] = count;
-        w[e] = static_cast<float>(static_cast<double>(E) * f / n);
+        w[e] = static_cast<float>(weight);
     }
-    red[threadIdx.x] = part;
+    // E <= 256 values lie in the first four waves
+    for (int d = 1; d < kWave; d <<= 1) part += __shfl_xor(part, d, kWave);
+    if (lane_id() == 0 && threadIdx.x < OPMX_MOE_MAX_EXPERTS) red[threadIdx.x / kWave] = part;
     __syncthreads();
-    for (int s = THREADS / 2; s >= 1; s >>= 1) {
-        if (static_cast<int>(threadIdx.x) < s) red[threadIdx.x] += red[threadIdx.x + s];
-        __syncthreads();
+    if (threadIdx.x == 0) {
+        double v = red[0];
+        for (int i = 1; i < THREADS / kWave && i < OPMX_MOE_MAX_EXPERTS / kWave; ++i) v += red[i];
+        *loss = static_cast<float>(v);
     }
-    if (threadIdx.x == 0) *loss = static_cast<float>(red[0]);
 }
 
-// Sums over the tokens of a block.  A single block finishes by itself; several leave psum [blocks][E], counts
-// [blocks][E] and kept [blocks] in the workspace.
+// Sums over the tokens of a block.  A single block finishes by itself; several leave psum and counts
+// [blocks][pitch_of(E)] and kept [blocks] in the workspace.
 template <typename T, int N, int V, int L, int KL, int THREADS>
 __global__ __launch_bounds__(THREADS) void balance_kernel(const T *__restrict__ scores,
                                                            const uint8_t *__restrict__ mask, int64_t Ttok, int E, int k,
@@ -217,7 +232,7 @@ __global__ __launch_bounds__(THREADS) void balance_kernel(const T *__restrict__ 
     __shared__ float s_p[WAVES][OPMX_MOE_MAX_EXPERTS];
     __shared__ int32_t s_c[WAVES][OPMX_MOE_MAX_EXPERTS];
     __shared__ int32_t s_n[WAVES];
-    __shared__ double s_red[THREADS];
+    __shared__ double s_red[OPMX_MOE_MAX_EXPERTS / kWave];
     const int lane = lane_id() % L, wave = threadIdx.x / kWave;
     const int per_block = THREADS / L;
     float psum[V];
@@ -235,7 +250,7 @@ __global__ __launch_bounds__(THREADS) void balance_kernel(const T *__restrict__ 
         const T *row = scores + (t < Ttok ? t : Ttok - 1) * E;
         float z[V];
         uint32_t key[V];
-        load_scores<T, N, V, L, true>(row, E, lane, z, key);
+        load_scores<T, N, V, L, true>(row, E, lane, keep, z, key);
         uint32_t list[KL];
 #pragma unroll
         for (int j = 0; j < KL; ++j) list[j] = 0u;
@@ -243,50 +258,49 @@ __global__ __launch_bounds__(THREADS) void balance_kernel(const T *__restrict__ 
         for (int i = 0; i < V; ++i) insert<KL>(list, key[i]);
 #define OPMX_MERGE(D) merge<KL, D>(list)
         OPMX_HALVES(OPMX_MERGE);
-        const uint32_t kth = at<KL>(list, k - 1);
-        softmax_<V, L>(z);
-        if constexpr (Key<T>::unique) {
+        const uint32_t kth = keep ? at<KL>(list, k - 1) : 0xFFFFFFFFu;       // no key of a token that does not count reaches it
+        bool tied = false;
+        if constexpr (!Key<T>::unique) {
+            int picked = 0;
 #pragma unroll
-            for (int i = 0; i < V; ++i) cnt[i] += keep && key[i] >= kth ? 1 : 0;
+            for (int i = 0; i < V; ++i) picked += key[i] >= kth ? 1 : 0;
+#define OPMX_PICKED(D) picked += other_half<D>(picked)
+            OPMX_HALVES(OPMX_PICKED);
+            tied = picked > k;               // more equal ones at the k-th place than are to be picked
+        }
+        if (!__any(tied)) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) cnt[i] += key[i] >= kth ? 1 : 0;
         } else {
-            int above = 0, equal = 0;
+            int above = 0;
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                above += key[i] > kth ? 1 : 0;
-                equal += key[i] == kth ? 1 : 0;
-            }
-#define OPMX_COUNT(D) above += other_half<D>(above), equal += other_half<D>(equal)
-            OPMX_HALVES(OPMX_COUNT);
+            for (int i = 0; i < V; ++i) above += key[i] > kth ? 1 : 0;
+#define OPMX_ABOVE(D) above += other_half<D>(above)
+            OPMX_HALVES(OPMX_ABOVE);
             const int left = k - above;      // so many of the equal ones are picked, the lowest ids first
-            if (!__any(equal > left)) {
+            // ids go up chunk by chunk, and within a chunk lane by lane
+            int before = 0;                  // equal ones in the chunks behind us
 #pragma unroll
-                for (int i = 0; i < V; ++i) cnt[i] += keep && key[i] >= kth ? 1 : 0;
-            } else {
-                // ids go up chunk by chunk, and within a chunk lane by lane
-                int before = 0;              // equal ones in the chunks behind us
+            for (int c = 0; c < V / N; ++c) {
+                int mine = 0;
 #pragma unroll
-                for (int c = 0; c < V / N; ++c) {
-                    int mine = 0;
+                for (int j = 0; j < N; ++j) mine += key[c * N + j] == kth ? 1 : 0;
+                int upto = mine, all = mine;
+#define OPMX_PREFIX(D) upto += lanes_before<D, L>(upto, lane), all += other_half<D>(all)
+                OPMX_HALVES(OPMX_PREFIX);
+                int rank = before + upto - mine;
 #pragma unroll
-                    for (int j = 0; j < N; ++j) mine += key[c * N + j] == kth ? 1 : 0;
-                    int upto = mine;
-                    for (int d = 1; d < L; d <<= 1) {
-                        const int o = __shfl_up(upto, d, kWave);
-                        if (lane >= d) upto += o;
-                    }
-                    int rank = before + upto - mine;
-#pragma unroll
-                    for (int j = 0; j < N; ++j) {
-                        const uint32_t q = key[c * N + j];
-                        cnt[c * N + j] += keep && (q > kth || (q == kth && rank < left)) ? 1 : 0;
-                        rank += q == kth ? 1 : 0;
-                    }
-                    before += __shfl(upto, (lane_id() / L) * L + L - 1, kWave);
+                for (int j = 0; j < N; ++j) {
+                    const uint32_t q = key[c * N + j];
+                    cnt[c * N + j] += q > kth || (q == kth && rank < left) ? 1 : 0;
+                    rank += q == kth ? 1 : 0;
                 }
+                before += all;
             }
         }
+        const float scale = exp_<V, L>(z);
 #pragma unroll
-        for (int i = 0; i < V; ++i) psum[i] += keep ? z[i] : 0.0f;
+        for (int i = 0; i < V; ++i) psum[i] = fmaf(z[i], scale, psum[i]);
         kept += keep && lane == 0 ? 1 : 0;
     }
     // over the tokens of the wave, then of the block
@@ -319,67 +333,71 @@ __global__ __launch_bounds__(THREADS) void balance_kernel(const T *__restrict__ 
         finish<THREADS>(p, c, n, e, E, k, s_red, loss, counts, w);
         return;
     }
-    if (e < E) {
-        part_p[static_cast<int64_t>(blockIdx.x) * E + e] = p;
-        part_c[static_cast<int64_t>(blockIdx.x) * E + e] = c;
+    if (e < pitch_of(E)) {                   // (p and c are 0 past E)
+        part_p[blockIdx.x * pitch_of(E) + e] = p;
+        part_c[blockIdx.x * pitch_of(E) + e] = c;
     }
     if (e == 0) part_n[blockIdx.x] = n;
 }
 
-// The blocks' sums: thread (slice, e) adds every slices-th block's, in order, then slice 0 adds the slices.
-constexpr int kFinish = 1024;
-__global__ __launch_bounds__(kFinish) void balance_finish_kernel(const float *__restrict__ part_p,
-                                                                 const int32_t *__restrict__ part_c,
+// The blocks' sums: a thread adds four experts' of every 16th block, eight blocks' loads in flight, then the slices are
+// added in order.  Rows of the sums are pitch_of(E) long: whole 16-byte chunks.
+constexpr int kFinish = 1024, kSlices = 16;
+__global__ __launch_bounds__(kFinish) void balance_finish_kernel(const float4 *__restrict__ part_p,
+                                                                 const int4 *__restrict__ part_c,
                                                                  const int32_t *__restrict__ part_n, int blocks, int E,
                                                                  int k, float *__restrict__ loss,
                                                                  int64_t *__restrict__ counts, float *__restrict__ w)
 {
-    __shared__ double s_red[kFinish];
-    __shared__ int64_t s_c[kFinish];
-    __shared__ int64_t s_n;
-    const int slices = kFinish / E < 32 ? kFinish / E : 32;      // E <= 256: at least four
-    const int slice = threadIdx.x / E, e = threadIdx.x % E;
-    double p = 0.0;
-    int64_t c = 0;
-    if (slice < slices) {
-        int b = slice;
-        for (; b + 15 * slices < blocks; b += 16 * slices) {     // sixteen pairs of loads in flight
-            float pv[16];
-            int32_t cv[16];
+    __shared__ double s_p[kSlices][OPMX_MOE_MAX_EXPERTS];
+    __shared__ int32_t s_c[kSlices][OPMX_MOE_MAX_EXPERTS];       // T < 2^31
+    __shared__ double s_red[OPMX_MOE_MAX_EXPERTS / kWave];
+    __shared__ int32_t s_n;
+    const int quads = pitch_of(E) / 4, slice = threadIdx.x / quads, quad = threadIdx.x % quads;
+    if (slice < kSlices) {
+        double p[4] = {0.0, 0.0, 0.0, 0.0};
+        int32_t c[4] = {0, 0, 0, 0};
+        for (int b0 = slice; b0 < blocks; b0 += 8 * kSlices) {
+            float4 pv[8];
+            int4 cv[8];
 #pragma unroll
-            for (int u = 0; u < 16; ++u) {
-                pv[u] = part_p[(b + u * slices) * E + e];
-                cv[u] = part_c[(b + u * slices) * E + e];
+            for (int u = 0; u < 8; ++u) {                        // (past the last block the last one again, for nothing)
+                const int b = b0 + u * kSlices, at = (b < blocks ? b : blocks - 1) * quads + quad;
+                pv[u] = part_p[at];
+                cv[u] = part_c[at];
             }
+            __builtin_amdgcn_sched_barrier(0);                   // all of them before the first sum
 #pragma unroll
-            for (int u = 0; u < 16; ++u) {
-                p += pv[u];
-                c += cv[u];
-            }
+            for (int u = 0; u < 8; ++u)
+                if (b0 + u * kSlices < blocks) {
+                    p[0] += pv[u].x, p[1] += pv[u].y, p[2] += pv[u].z, p[3] += pv[u].w;
+                    c[0] += cv[u].x, c[1] += cv[u].y, c[2] += cv[u].z, c[3] += cv[u].w;
+                }
         }
-        for (; b < blocks; b += slices) {
-            p += part_p[b * E + e];
-            c += part_c[b * E + e];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            s_p[slice][quad * 4 + j] = p[j];
+            s_c[slice][quad * 4 + j] = c[j];
         }
     }
-    s_red[threadIdx.x] = p;
-    s_c[threadIdx.x] = c;
-    if (threadIdx.x < kWave) {
+    if (threadIdx.x >= kFinish - kWave) {
         int32_t n = 0;
 #pragma unroll
-        for (int b = 0; b < kMaxBlocks; b += kWave) n += b + static_cast<int>(threadIdx.x) < blocks ? part_n[b + threadIdx.x] : 0;
-        n = sum_mod<1>(n);                                       // T < 2^31
-        if (threadIdx.x == 0) s_n = n;
+        for (int b = 0; b < kMaxBlocks; b += kWave) n += b + lane_id() < blocks ? part_n[b + lane_id()] : 0;
+        n = sum_mod<1>(n);
+        if (lane_id() == 0) s_n = n;
     }
     __syncthreads();
-    if (slice == 0)
-        for (int s = 1; s < slices; ++s) {
-            p += s_red[s * E + e];
-            c += s_c[s * E + e];
+    double p = 0.0;
+    int64_t c = 0;
+    const int e = threadIdx.x;
+    if (e < E)
+#pragma unroll
+        for (int v = 0; v < kSlices; ++v) {
+            p += s_p[v][e];
+            c += s_c[v][e];
         }
-    const int64_t n = s_n;
-    __syncthreads();                         // s_red is used again
-    finish<kFinish>(p, c, n, slice == 0 ? e : E, E, k, s_red, loss, counts, w);
+    finish<kFinish>(p, c, s_n, e, E, k, s_red, loss, counts, w);
 }
 
 template <typename T, int N, int V, int L>
@@ -403,11 +421,14 @@ __global__ __launch_bounds__(256) void balance_backward_kernel(const T *__restri
         const bool keep = t < Ttok && (mask == nullptr || mask[t] != 0);
         float z[V];
         uint32_t none[1];
-        load_scores<T, N, V, L, false>(scores + (t < Ttok ? t : Ttok - 1) * E, E, lane, z, none);
-        softmax_<V, L>(z);
+        load_scores<T, N, V, L, false>(scores + (t < Ttok ? t : Ttok - 1) * E, E, lane, keep, z, none);
+        const float inverse = exp_<V, L>(z);
         float dot = 0.0f;
 #pragma unroll
-        for (int i = 0; i < V; ++i) dot += z[i] * wv[i];
+        for (int i = 0; i < V; ++i) {
+            z[i] *= inverse;
+            dot += z[i] * wv[i];
+        }
 #define OPMX_DOT(D) dot += other_half<D>(dot)
         OPMX_HALVES(OPMX_DOT);
         if (t >= Ttok) continue;             // (the last trip: nobody needs this lane again)
@@ -488,13 +509,13 @@ int forward_impl(const void *scores, const void *mask, int64_t Ttok, int E, int 
 {
     constexpr int n = Vec16<T>::n;
     Forward f{scores, mask, Ttok, E, k, blocks_for(Ttok, E), static_cast<float *>(ws), nullptr, nullptr, loss, counts, w};
-    f.pc = reinterpret_cast<int32_t *>(f.pp + static_cast<int64_t>(f.blocks) * E);
-    f.pn = f.pc + static_cast<int64_t>(f.blocks) * E;
+    f.pc = reinterpret_cast<int32_t *>(f.pp + f.blocks * pitch_of(E));
+    f.pn = f.pc + f.blocks * pitch_of(E);
     if (E % n == 0 && aligned16(scores)) forward_sums<T, n>(f, s);
     else forward_sums<T, 1>(f, s);
     OPMX_LAUNCH_CHECK();
     if (f.blocks > 1) {
-        balance_finish_kernel<<<1, kFinish, 0, s>>>(f.pp, f.pc, f.pn, f.blocks, E, k, loss, counts, w);
+        balance_finish_kernel<<<1, kFinish, 0, s>>>(reinterpret_cast<const float4 *>(f.pp), reinterpret_cast<const int4 *>(f.pc), f.pn, f.blocks, E, k, loss, counts, w);
         OPMX_LAUNCH_CHECK();
     }
     return OPMX_OK;
@@ -548,7 +569,7 @@ size_t moe_balance_loss_workspace_bytes(int64_t Ttok, int E)
     if (Ttok <= 0 || E <= 0 || E > OPMX_MOE_MAX_EXPERTS) return 256;
     const int blocks = blocks_for(Ttok, E);
     if (blocks == 1) return 256;             // finishes by itself
-    const size_t b = static_cast<size_t>(blocks) * (static_cast<size_t>(E) * 8 + 4);
+    const size_t b = static_cast<size_t>(blocks) * (static_cast<size_t>(pitch_of(E)) * 8 + 4);
     return (b + 255) / 256 * 256 + 256;
 }
 
