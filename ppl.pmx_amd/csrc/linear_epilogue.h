@@ -8,6 +8,7 @@ namespace opmx {
 namespace {
 
 typedef uint32_t quad_any __attribute__((ext_vector_type(4), aligned(2)));     // 16 bytes at any address
+typedef uint32_t pair_any __attribute__((ext_vector_type(2), aligned(1)));
 typedef float float4_any __attribute__((ext_vector_type(4), aligned(4)));
 
 // The logistic function as in the SwiGLU kernels: accurate where the output keeps its digits.
@@ -144,9 +145,10 @@ template <typename T> __device__ __forceinline__ void kept8(const void *kept, in
         uint16_t a[8];
         uint8_t b[8];
         if (left >= 8) {
-            const quad_any q = *reinterpret_cast<const quad_any *>(hi);
+            const quad_any q = __builtin_nontemporal_load(reinterpret_cast<const quad_any *>(hi));
+            const pair_any u = __builtin_nontemporal_load(reinterpret_cast<const pair_any *>(lo));
             __builtin_memcpy(a, &q, 16);
-            __builtin_memcpy(b, lo, 8);
+            __builtin_memcpy(b, &u, 8);
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
