@@ -222,10 +222,9 @@ struct Operand {
     int64_t pitch;
     bool k_major;
 };
-// Tiles of C, by rows: 256 x 256 (eight waves, two k-tiles in LDS), and 128 columns wide with two k-tiles in LDS (two
-// workgroups per CU) or four (one, for products with fewer tiles than CUs: the loads have three k-tiles' time); 64 and
-// 32 rows are for few rows in all.
-enum class Tile { k256, k128, k128Deep, k64, k32 };
+// Tiles of C: 256 x 256 by four waves of 128 x 128 (16-bit types, k in one range); 128 x 128 with two k-tiles in LDS and
+// 64 x 128 with three, each by four waves and two workgroups to a CU.
+enum class Tile { k256, k128, k64 };
 // ranges > 1: k is cut into that many ranges, e.part must hold their sums.
 int launch_linear_gemm(const Operand &P, const Operand &Q, int64_t Kc, int dtype, const Epilogue &e, Tile tile, int ranges,
                        hipStream_t s);

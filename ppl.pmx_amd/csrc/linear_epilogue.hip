@@ -195,39 +195,45 @@ __global__ __launch_bounds__(kJoin) void join_kernel(Epilogue e, int ranges)
     store8(static_cast<T *>(e.Y) + m * e.ncols + c, left, h);
 }
 
-// Tile and k ranges of a product of `rows` x `ncols` outputs (gated: ncols pairs of them) over Kc; k_rows: both
-// operands hold k along their rows.
+// Tile and k ranges of a product of `rows` x `ncols` outputs (gated: ncols pairs of them) over Kc; p_rows, q_rows:
+// k runs over the rows of P, of Q (Operand::k_major).
 struct Cut {
     Tile tile;
     int ranges;
     int64_t pitch;      // of the ranges' sums
     size_t bytes;       // of the ranges' sums
 };
-Cut cut_for(int64_t rows, int64_t ncols, int64_t Kc, bool gated, bool k_rows, int dtype)
+Cut cut_for(int64_t rows, int64_t ncols, int64_t Kc, bool gated, bool p_rows, bool q_rows, int dtype)
 {
     Cut c{Tile::k128, 1, 0, 0};
     const bool f32 = dtype == OPMX_DTYPE_F32;
     const int64_t width = gated ? 2 * ncols : ncols, columns = ceil_div(width, 128);
-    int64_t tiles = ceil_div(rows, 128) * columns;
     const int64_t nk = ceil_div(Kc, f32 ? 32 : 64);
-    if (!f32 && ceil_div(rows, 256) * ceil_div(width, 256) >= 192) {
+    // The large tile needs most of the 256 CUs busy and k-tiles to spread its start and its end over: against 128 x 128,
+    // 4096 x 8192 outputs over 16 k-tiles 76 us and 78, 4096 x 14336 over 4 77 and 57; with k over the rows of both
+    // operands over 16 152 and 141, 4096 x 4096 over 32 66 and 75.
+    if (!f32 && ceil_div(rows, 256) * ceil_div(width, 256) >= 192 && nk >= (q_rows ? 24 : 16)) {
         c.tile = Tile::k256;
-    } else if (!k_rows && rows <= 64) {
-        // the weights are read once whatever happens: as many workgroups as LDS holds, at least 4 k-tiles each
-        c.tile = rows <= 32 ? Tile::k32 : Tile::k64;
-        int64_t r = columns > 0 && columns < 192 ? 512 / columns : 1;
-        if (r > nk / 4) r = nk / 4;
-        c.ranges = static_cast<int>(r < 1 ? 1 : r > 32 ? 32 : r);
-    } else if (tiles > 0 && tiles <= 256) {
-        // A k-tile takes about 0.35 us (fp32 1.8), joining the ranges 8 us, a CU holds one workgroup.
-        c.tile = Tile::k128Deep;
-        double best = 0;
-        for (int64_t r = 1; r <= 16 && r * 4 <= (nk > 4 ? nk : 4); ++r) {
-            const double us = static_cast<double>(ceil_div(tiles * r, 256) * ceil_div(nk, r)) * (f32 ? 1.8 : 0.35) + (r > 1 ? 8.0 : 0.0);
-            if (r == 1 || us < best) {
-                best = us;
-                c.ranges = static_cast<int>(r);
-            }
+        return c;
+    }
+    // More tiles than CUs: 128 x 128 (float16, 3000 x 2816 outputs over 2048: 54 us, 64 x 128 55, the gradients 47 and 55).
+    // Fewer: 64 x 128 (512 x 1024 over 1024 9 us, 128 x 128 13; 100 x 2048 over 1408 11 and 17), with k in ranges where it is long.
+    if (rows > 64 && ceil_div(rows, 128) * columns > 256) return c;
+    c.tile = Tile::k64;
+    const int64_t tiles = ceil_div(rows, 64) * columns;
+    // Microseconds of a k-tile, of one workgroup on a CU and of two (fp32: bound by the matrix units at either), and of
+    // joining r ranges, fitted to the times of 1 to 16 ranges of 17 products with 20 to 2048 rows: the chosen ones are
+    // within 8 % of the best.
+    const double one = f32 ? 1.1 : p_rows ? 0.45 : 0.34, two = f32 ? 2.2 : p_rows ? 0.65 : 0.62;
+    double best = 0;
+    for (int64_t r = 1; r <= 16 && (r == 1 || r * 4 <= nk); ++r) {
+        const int64_t load = ceil_div(tiles * r, 256);
+        const double mb = static_cast<double>(r * rows * width) * 4e-6;
+        const double us = static_cast<double>(ceil_div(nk, r)) * (static_cast<double>(load / 2) * two + static_cast<double>(load % 2) * one) +
+                          (r > 1 ? 3.0 + 0.4 * static_cast<double>(r) + 0.3 * mb : 0.0);
+        if (r == 1 || us < best) {
+            best = us;
+            c.ranges = static_cast<int>(r);
         }
     }
     if (c.ranges > 1) c.ranges = static_cast<int>(ceil_div(nk, ceil_div(nk, c.ranges)));      // none of them empty
@@ -252,7 +258,7 @@ template <typename T>
 int product(const Operand &P, const Operand &Q, int64_t Kc, Epilogue e, void *ws, hipStream_t s)
 {
     const bool gated = e.act == OPMX_ACTIVATION_SWIGLU;
-    const Cut c = cut_for(e.rows, e.ncols, Kc, gated, Q.k_major, DType<T>::id);
+    const Cut c = cut_for(e.rows, e.ncols, Kc, gated, P.k_major, Q.k_major, DType<T>::id);
     if (c.ranges > 1) {
         e.part = static_cast<float *>(ws);
         e.pitch = c.pitch;
@@ -299,7 +305,7 @@ ForwardPlan forward_plan(int64_t Ttok, int64_t K, int64_t N, int dtype, int act)
     p.x = 0;
     p.w = p.x + (padded ? up(Ttok * pitch * esize, 256) : 0);
     p.part = p.w + (padded ? up(N * pitch * esize, 256) : 0);
-    p.total = p.part + up(cut_for(Ttok, gated ? N / 2 : N, K, gated, false, dtype).bytes, 256);
+    p.total = p.part + up(cut_for(Ttok, gated ? N / 2 : N, K, gated, false, false, dtype).bytes, 256);
     return p;
 }
 
@@ -331,7 +337,7 @@ BackwardPlan backward_plan(int64_t Ttok, int64_t K, int64_t N, int dtype, int ac
     p.w = p.x + up(Ttok * p.pitch_k * esize, 256);          // padded, or unpacked from 8 bits
     p.sums = p.w + (p.padded ? up(N * p.pitch_k * esize, 256) : 0);
     p.part = p.sums + up(ceil_div(Ttok, p.chunk) * N * 4, 256);
-    const size_t a = cut_for(Ttok, K, N, false, false, dtype).bytes, b = cut_for(N, K, Ttok, false, true, dtype).bytes;
+    const size_t a = cut_for(Ttok, K, N, false, true, false, dtype).bytes, b = cut_for(N, K, Ttok, false, true, true, dtype).bytes;
     p.total = p.part + up(a > b ? a : b, 256);
     return p;
 }

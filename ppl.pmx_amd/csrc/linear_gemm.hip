@@ -6,7 +6,7 @@
 //     gradient W   Q = dH [T,N],  P = X [T,K], k = T: k runs over rows in both
 //
 // A workgroup owns a BM x BN tile of C and walks k in tiles of 128 bytes (64 values, 32 in fp32), loaded straight into
-// LDS and up to three tiles ahead.  P is the A operand of the MFMAs and Q the B operand, so a lane ends up with four
+// LDS and one or two tiles ahead.  P is the A operand of the MFMAs and Q the B operand, so a lane ends up with four
 // neighbouring columns of a row.
 //   rows along k:     LDS [row][8 chunks of 16 bytes], chunk c in slot c ^ (row / 2 % 8): a fragment is one
 //                     16-byte read, conflict free;
@@ -55,11 +55,15 @@ template <> struct Step<float> {
     }
 };
 
-// How k-major rows are permuted inside a k row of LDS: the index of a unit (32 bytes; fp32: 64) is xored with this.
-template <typename T> __device__ __forceinline__ int unit_swizzle(int k)
+// How k-major rows are permuted inside a k row of LDS (ROWS values): the index of a unit (32 bytes; fp32: 64) is xored with
+// this.  A transposing read takes, for every half of the wave, one unit of k rows 0 to 3 and 8 to 11 (from a multiple of
+// 16): with 256 bytes per k row and more these differ in all three bits, with 128 bytes the parity of k already tells the
+// halves of the banks apart.
+template <typename T, int ROWS> __device__ __forceinline__ int unit_swizzle(int k)
 {
-    if constexpr (sizeof(T) == 2) return (k & 3) | ((k >> 3 & 1) << 2);
-    else return (k >> 2) & 3;
+    if constexpr (sizeof(T) == 4) return (k >> 2) & 3;
+    else if constexpr (ROWS * sizeof(T) >= 256) return (k & 3) | ((k >> 3 & 1) << 2);
+    else return (k >> 1 & 1) | ((k >> 3 & 1) << 1);
 }
 
 // Waits until at most N of the wave's loads are outstanding (they land in order) and all its LDS reads are done.
@@ -100,7 +104,7 @@ template <typename T, int ROWS, int THREADS, bool KM, bool GATED> struct Loader 
                 constexpr int per_k = ROWS / n;                  // pieces of a k row
                 constexpr int per_unit = sizeof(T) == 2 ? 2 : 4;
                 const int k = piece / per_k, c = piece % per_k;
-                const int r = (((c / per_unit) ^ unit_swizzle<T>(k)) * per_unit + c % per_unit) * n;
+                const int r = (((c / per_unit) ^ unit_swizzle<T, ROWS>(k)) * per_unit + c % per_unit) * n;
                 first_k[i] = k;
                 off[i] = row0 + r < count ? static_cast<uint32_t>((k * o.pitch + r) * esize) : kNowhere;
             } else {
@@ -188,7 +192,7 @@ __device__ __forceinline__ void fragments(const char *lds, int row16, int lane, 
             uint32_t a[B];
 #pragma unroll
             for (int j = 0; j < B; ++j)
-                a[j] = base + k * (ROWS * 2) + (((row16 + i + j) ^ unit_swizzle<T>(k)) << 5) + (r & 3) * 8;
+                a[j] = base + k * (ROWS * 2) + (((row16 + i + j) ^ unit_swizzle<T, ROWS>(k)) << 5) + (r & 3) * 8;
             if constexpr (B == 4) transposed4<KS * 32 * ROWS * 2, 4 * ROWS * 2>(f + i, a);
             else transposed2<KS * 32 * ROWS * 2, 4 * ROWS * 2>(f + i, a);
         }
@@ -198,7 +202,7 @@ __device__ __forceinline__ void fragments(const char *lds, int row16, int lane, 
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int k = KS * 16 + g * 4 + j;
-                f[i][j] = *reinterpret_cast<const float *>(lds + k * (ROWS * 4) + (((row16 + i) ^ unit_swizzle<T>(k)) << 6) + r * 4);
+                f[i][j] = *reinterpret_cast<const float *>(lds + k * (ROWS * 4) + (((row16 + i) ^ unit_swizzle<T, ROWS>(k)) << 6) + r * 4);
             }
     }
 }
@@ -326,7 +330,7 @@ __global__ __launch_bounds__(WM *WN *kWave, 2) void linear_gemm_kernel(Operand P
     constexpr int STAGE = (BM + BN) * kTileBytes, BK = kTileBytes / sizeof(T);
     constexpr int BNO = GATED ? BN / 2 : BN;
     constexpr int PIECE = WTM < 64 ? WTM : 64;
-    static_assert(WTN == 64 && (TM == 2 || TM == 4 || TM == 8), "the epilogue stages pieces of 64 columns");
+    static_assert(WTN == 64 && (TM == 2 || TM == 4), "the epilogue stages pieces of 64 columns");
     using frag = typename Step<T>::frag;
     extern __shared__ __attribute__((aligned(16))) char smem[];
 
@@ -360,21 +364,15 @@ __global__ __launch_bounds__(WM *WN *kWave, 2) void linear_gemm_kernel(Operand P
         lq.next();
         lp.next();
     };
-    auto half = [&](const char *cur, auto ks_tag, auto h_tag, const frag (&p)[TN]) {
-        constexpr int KS = decltype(ks_tag)::value, H = decltype(h_tag)::value;
-        constexpr int C = TM < 4 ? TM : 4;
-        frag q[C];
-        fragments<T, BM, QK, KS, C>(cur, wm * TM + H * 4, lane, q);
-#pragma unroll
-        for (int i = 0; i < C; ++i)
-#pragma unroll
-            for (int j = 0; j < TN; ++j) acc[j][H * 4 + i] = Step<T>::mma(p[j], q[i], acc[j][H * 4 + i]);
-    };
     auto multiply = [&](const char *cur, auto ks_tag) {
-        frag p[TN];
-        fragments<T, BN, PK, decltype(ks_tag)::value, TN>(cur + BM * kTileBytes, wn * TN, lane, p);
-        half(cur, ks_tag, std::integral_constant<int, 0>{}, p);
-        if constexpr (TM == 8) half(cur, ks_tag, std::integral_constant<int, 1>{}, p);
+        constexpr int KS = decltype(ks_tag)::value;
+        frag p[TN], q[TM];
+        fragments<T, BN, PK, KS, TN>(cur + BM * kTileBytes, wn * TN, lane, p);
+        fragments<T, BM, QK, KS, TM>(cur, wm * TM, lane, q);
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[j][i] = Step<T>::mma(p[j], q[i], acc[j][i]);
     };
     // STAGES - 1 k-tiles are on their way at any time.  Past the last one the loads go on, from nowhere, so that the
     // number of outstanding ones that means "tile kt has landed" stays the same.
@@ -522,7 +520,7 @@ template <bool KM> struct WideReader {
             const int k = g * 8 + (r >> 2);
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                a[i] = base + k * 512 + (((first + i) ^ unit_swizzle<f16>(k)) << 5) + (r & 3) * 8;
+                a[i] = base + k * 512 + (((first + i) ^ unit_swizzle<f16, 256>(k)) << 5) + (r & 3) * 8;
         } else {
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) a[ks] = base + (first * 16 + r) * kTileBytes + (((ks * 4 + g) ^ ((r >> 1) & 7)) << 4);
@@ -742,8 +740,7 @@ int by_layout(const Operand &P, const Operand &Q, int64_t Kc, const Epilogue &e,
     if (e.act == OPMX_ACTIVATION_SWIGLU) return launch<T, BM, BN, WM, WN, STAGES, false, false, true>(P, Q, Kc, e, ranges, s);
     if (!P.k_major) return launch<T, BM, BN, WM, WN, STAGES, false, false, false>(P, Q, Kc, e, ranges, s);
     if (!Q.k_major) return launch<T, BM, BN, WM, WN, STAGES, true, false, false>(P, Q, Kc, e, ranges, s);
-    if constexpr (BM >= 128) return launch<T, BM, BN, WM, WN, STAGES, true, true, false>(P, Q, Kc, e, ranges, s);
-    return OPMX_ERR_UNSUPPORTED;
+    return launch<T, BM, BN, WM, WN, STAGES, true, true, false>(P, Q, Kc, e, ranges, s);
 }
 
 template <typename T> int by_tile(const Operand &P, const Operand &Q, int64_t Kc, const Epilogue &e, Tile tile, int ranges, hipStream_t s)
@@ -754,9 +751,7 @@ template <typename T> int by_tile(const Operand &P, const Operand &Q, int64_t Kc
                 if (ranges == 1) return by_layout_wide<T>(P, Q, Kc, e, s);
             break;
         case Tile::k128: return by_layout<T, 128, 128, 2, 2, 2>(P, Q, Kc, e, ranges, s);
-        case Tile::k128Deep: return by_layout<T, 128, 128, 4, 2, 4>(P, Q, Kc, e, ranges, s);
         case Tile::k64: return by_layout<T, 64, 128, 2, 2, 3>(P, Q, Kc, e, ranges, s);
-        case Tile::k32: return by_layout<T, 32, 128, 1, 2, 4>(P, Q, Kc, e, ranges, s);
     }
     return OPMX_ERR_UNSUPPORTED;
 }
