@@ -77,8 +77,17 @@ template <typename T> __device__ __forceinline__ void load8(const T *p, int64_t 
             for (int j = 0; j < n; ++j) v[c * n + j] = to_f32(t[j]);
         }
     } else {
+        // (a load under a condition of its own would be waited for before the next: the first value stands in for those
+        // that do not exist)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = j < left ? to_f32(p[j]) : 0.0f;
+        for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+        if (left > 0) {
+            T t[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) t[j] = p[j < left ? j : 0];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = j < left ? to_f32(t[j]) : 0.0f;
+        }
     }
 }
 template <typename T> __device__ __forceinline__ void store8(T *p, int64_t left, const float (&v)[8])
@@ -152,8 +161,8 @@ template <typename T> __device__ __forceinline__ void kept8(const void *kept, in
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                a[j] = j < left ? hi[j] : 0;
-                b[j] = j < left ? lo[j] : 0;
+                a[j] = hi[j < left ? j : 0];            // left > 0; what does not exist is not used
+                b[j] = lo[j < left ? j : 0];
             }
         }
 #pragma unroll

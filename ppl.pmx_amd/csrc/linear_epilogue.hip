@@ -51,8 +51,11 @@ __global__ __launch_bounds__(256) void slope_kernel(const T *__restrict__ dY, co
 {
     __shared__ float s_sum[kSlopeWaves][GATED ? 2 : 1][kSlopeCols];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t c = static_cast<int64_t>(blockIdx.x) * kSlopeCols + lane * 8;
-    const int64_t left = ncols - c;
+    const int64_t left = ncols - (static_cast<int64_t>(blockIdx.x) * kSlopeCols + lane * 8);
+    // the last columns of a row that is no multiple of 8: eight columns that end there, of which `again` are the
+    // lane before's (the same values twice; they count once in the sums)
+    const int again = left > 0 && left < 8 && ncols >= 8 ? 8 - static_cast<int>(left) : 0;
+    const int64_t c = static_cast<int64_t>(blockIdx.x) * kSlopeCols + lane * 8 - again;
     const int64_t r0 = static_cast<int64_t>(blockIdx.y) * rows_per_chunk;
     const int64_t r1 = r0 + rows_per_chunk < Ttok ? r0 + rows_per_chunk : Ttok;
     float sum[2][8];
@@ -76,12 +79,7 @@ __global__ __launch_bounds__(256) void slope_kernel(const T *__restrict__ dY, co
                     sum[0][j] += d[j];
                     sum[1][j] += h[j];
                 }
-                if (dH) {
-                    store8(dH + r * pitch + c, here, d);
-                    store8(dH + r * pitch + ncols + c, here, h);
-                    if (left <= 8)                                                     // the lane of the last columns
-                        for (int64_t p = N; p < pitch; ++p) dH[r * pitch + p] = from_f32<T>(0.0f);
-                }
+                if (dH) store8(dH + r * pitch + ncols + c, here, h);
             } else {
                 if (act != OPMX_ACTIVATION_NONE) {
                     kept8<T>(H, Ttok * N, r * N + c, here, h);
@@ -89,22 +87,24 @@ __global__ __launch_bounds__(256) void slope_kernel(const T *__restrict__ dY, co
                     for (int j = 0; j < 8; ++j) d[j] *= slope<T>(act, h[j]);
                 }
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    if (j >= here) d[j] = 0.0f;
-                    sum[0][j] += d[j];
-                }
-                if (dH) store8(dH + r * pitch + c, left >= 8 ? 8 : pitch - c, d);
+                for (int j = 0; j < 8; ++j) sum[0][j] += d[j];
+            }
+            if (dH) {
+                store8(dH + r * pitch + c, here, d);
+                if (left <= 8)                                                         // the lane of the last columns
+                    for (int64_t p = N; p < pitch; ++p) dH[r * pitch + p] = from_f32<T>(0.0f);
             }
         }
     };
-    if (left >= 8) rows(std::integral_constant<int, 8>{});
+    if (left >= 8 || again > 0) rows(std::integral_constant<int, 8>{});
     else if (left > 0) rows(left);
     if (sums == nullptr) return;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        s_sum[wave][0][lane * 8 + j] = sum[0][j];
-        if (GATED) s_sum[wave][GATED ? 1 : 0][lane * 8 + j] = sum[1][j];
-    }
+    for (int j = 0; j < 8; ++j)
+        if (j >= again) {
+            s_sum[wave][0][lane * 8 + j - again] = sum[0][j];
+            if (GATED) s_sum[wave][GATED ? 1 : 0][lane * 8 + j - again] = sum[1][j];
+        }
     __syncthreads();
     for (int i = threadIdx.x; i < kSlopeCols; i += 256) {
         const int64_t col = static_cast<int64_t>(blockIdx.x) * kSlopeCols + i;

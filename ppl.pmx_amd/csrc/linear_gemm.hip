@@ -265,30 +265,6 @@ __device__ __forceinline__ void write_columns(const float4_t (&acc)[TN][TM], con
             }
         } else {
             const bool shaped = GATED || e.act != OPMX_ACTIVATION_NONE || e.H;
-            if (shaped) {
-                // in place, in a rolled loop: the code of eight activations once
-#pragma unroll 1
-                for (int t = 0; t < PIECE / ROWS; ++t) {
-                    const int row = t * ROWS + lane / PER_ROW;
-                    const int64_t m = m0 + piece * PIECE + row;
-                    if (m >= e.rows || left <= 0) continue;
-                    float h[8], gate[8];
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const float4_t v = *staged(row, c8 * 2 + x);
-                        const float4_t u = GATED ? *staged(row, 8 + c8 * 2 + x) : v;
-#pragma unroll
-                        for (int y = 0; y < 4; ++y) {
-                            h[x * 4 + y] = v[y];
-                            gate[x * 4 + y] = u[y];
-                        }
-                    }
-                    activate8<T, GATED>(e, m, c, left, bias_h, bias_g, h, gate);
-#pragma unroll
-                    for (int x = 0; x < 2; ++x)
-                        *staged(row, c8 * 2 + x) = float4_t{h[x * 4], h[x * 4 + 1], h[x * 4 + 2], h[x * 4 + 3]};
-                }
-            }
             constexpr int GROUP = PIECE / ROWS < 4 ? PIECE / ROWS : 4;              // residual rows in flight
 #pragma unroll 1
             for (int t0 = 0; t0 < PIECE / ROWS; t0 += GROUP) {
@@ -298,6 +274,30 @@ __device__ __forceinline__ void write_columns(const float4_t (&acc)[TN][TM], con
                     const int64_t m = m0 + piece * PIECE + (t0 + t) * ROWS + lane / PER_ROW;
                     if (e.residual && m < e.rows && left > 0)
                         load8(static_cast<const T *>(e.residual) + m * e.ncols + c, left, res[t]);
+                }
+                if (shaped) {
+                    // in place, in a rolled loop: the code of eight activations once
+#pragma unroll 1
+                    for (int t = t0; t < t0 + GROUP; ++t) {
+                        const int row = t * ROWS + lane / PER_ROW;
+                        const int64_t m = m0 + piece * PIECE + row;
+                        if (m >= e.rows || left <= 0) continue;
+                        float h[8], gate[8];
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const float4_t v = *staged(row, c8 * 2 + x);
+                            const float4_t u = GATED ? *staged(row, 8 + c8 * 2 + x) : v;
+#pragma unroll
+                            for (int y = 0; y < 4; ++y) {
+                                h[x * 4 + y] = v[y];
+                                gate[x * 4 + y] = u[y];
+                            }
+                        }
+                        activate8<T, GATED>(e, m, c, left, bias_h, bias_g, h, gate);
+#pragma unroll
+                        for (int x = 0; x < 2; ++x)
+                            *staged(row, c8 * 2 + x) = float4_t{h[x * 4], h[x * 4 + 1], h[x * 4 + 2], h[x * 4 + 3]};
+                    }
                 }
 #pragma unroll
                 for (int t = 0; t < GROUP; ++t) {
