@@ -9,7 +9,7 @@
 // of W share one reading of it, and a row of X past the last one is the last one again, never stored.
 // Rows of W and X may start anywhere their type allows; the last k values that fill no piece go one by one.
 #include "linear_epilogue.h"
-#include "moe_gemm.h"
+#include "linear_step.h"
 
 namespace opmx {
 namespace {
@@ -17,25 +17,7 @@ namespace {
 constexpr int kFewWaves = 8;
 constexpr int64_t kFewWideColumns = 16384;       // from here on 32 columns per workgroup: 512 workgroups at least
 constexpr int64_t kFewStreamBytes = 8 << 20;     // weights from which on they go through LDS
-
-template <typename T> struct FewStep;
-template <> struct FewStep<f16> {
-    using frag = half8_t;
-    static __device__ __forceinline__ float4_t mma(frag p, frag q, float4_t c) { return Mfma<f16>::m16(p, q, c); }
-};
-template <> struct FewStep<bf16> {
-    using frag = bf16x8_t;
-    static __device__ __forceinline__ float4_t mma(frag p, frag q, float4_t c) { return Mfma<bf16>::m16(p, q, c); }
-};
-template <> struct FewStep<float> {
-    using frag = float4_t;
-    static __device__ __forceinline__ float4_t mma(frag p, frag q, float4_t c)
-    {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(p[j], q[j], c, 0, 0, 0);
-        return c;
-    }
-};
+constexpr int64_t kFewDirectBytes = 24 << 20;    // weights up to which 17 to 32 rows are few
 
 // 16 bytes at any address; `once`: what the caches need not keep.
 template <typename F, bool ONCE> __device__ __forceinline__ F load_frag(const void *p)
@@ -88,7 +70,7 @@ template <typename T, int NT, int RT, bool GATED>
 __global__ __launch_bounds__(kFewWaves *kWave, 2) void few_rows_kernel(const T *__restrict__ X, const T *__restrict__ W, int64_t K,
                                                                         Epilogue e)
 {
-    using frag = typename FewStep<T>::frag;
+    using frag = typename Step<T>::frag;
     constexpr int n = 16 / sizeof(T), STEP = 4 * n;          // k values of a lane's load, of one MFMA step
     constexpr int U = NT * RT >= 4 ? 4 : 8;                  // steps in flight
     constexpr int CB = GATED ? 16 : 16 * RT;                 // columns of Y per workgroup
@@ -130,7 +112,7 @@ __global__ __launch_bounds__(kFewWaves *kWave, 2) void few_rows_kernel(const T *
 #pragma unroll
             for (int i = 0; i < RT; ++i)
 #pragma unroll
-                for (int t = 0; t < NT; ++t) acc[i][t] = FewStep<T>::mma(w[u][i], x[u][t], acc[i][t]);
+                for (int t = 0; t < NT; ++t) acc[i][t] = Step<T>::mma(w[u][i], x[u][t], acc[i][t]);
     }
     for (; s < steps; s += 2 * kFewWaves)
         for (int u = 0; u < 2 && s + u < steps; ++u) {
@@ -143,7 +125,7 @@ __global__ __launch_bounds__(kFewWaves *kWave, 2) void few_rows_kernel(const T *
 #pragma unroll
             for (int i = 0; i < RT; ++i)
 #pragma unroll
-                for (int t = 0; t < NT; ++t) acc[i][t] = FewStep<T>::mma(w[i], x[t], acc[i][t]);
+                for (int t = 0; t < NT; ++t) acc[i][t] = Step<T>::mma(w[i], x[t], acc[i][t]);
         }
     if (K % STEP != 0 && wave == kFewWaves - 1) {            // the values behind the last whole step
         const int64_t k = static_cast<int64_t>(steps) * STEP, left = K - k - g * n;
@@ -151,7 +133,9 @@ __global__ __launch_bounds__(kFewWaves *kWave, 2) void few_rows_kernel(const T *
         auto tail = [&](const T *p) {
             T v[n];
 #pragma unroll
-            for (int j = 0; j < n; ++j) v[j] = j < left ? p[k + j] : from_f32<T>(0.0f);
+            for (int j = 0; j < n; ++j) v[j] = p[k + (j < left ? j : left - 1)];       // (p + k + left - 1: the row's last)
+#pragma unroll
+            for (int j = 0; j < n; ++j) v[j] = j < left ? v[j] : from_f32<T>(0.0f);
             frag f;
             __builtin_memcpy(&f, v, 16);
             return f;
@@ -163,7 +147,7 @@ __global__ __launch_bounds__(kFewWaves *kWave, 2) void few_rows_kernel(const T *
 #pragma unroll
         for (int i = 0; i < RT; ++i)
 #pragma unroll
-            for (int t = 0; t < NT; ++t) acc[i][t] = FewStep<T>::mma(w[i], x[t], acc[i][t]);
+            for (int t = 0; t < NT; ++t) acc[i][t] = Step<T>::mma(w[i], x[t], acc[i][t]);
     }
 #pragma unroll
     for (int i = 0; i < RT; ++i)
@@ -179,7 +163,6 @@ __global__ __launch_bounds__(kFewWaves *kWave, 2) void few_rows_kernel(const T *
 // sees that much of a row at a time, SLOTS - 1 pieces ahead.  The waves share a piece's k, two MFMA steps each.
 // One token, weights not in any cache: 28672 x 4096 SwiGLU fp16 39 us = 6.0 TB/s (the kernel above 47, the tile product 50),
 // 4096 x 4096 8.2 us (9.2, 13.8), 4096 x 14336 22.5 us (29, 27).
-#define OPMX_LDS(p) ((void __attribute__((address_space(3))) *)(p))
 constexpr uint32_t kNowhere = 0x80000000u;      // past every descriptor
 constexpr int kNonTemporal = 2;
 
@@ -203,7 +186,7 @@ template <typename T, int NT, int RT, int WAVES, int SLOTS, bool GATED>
 __global__ __launch_bounds__(WAVES *kWave) void few_rows_stream_kernel(const T *__restrict__ X, const T *__restrict__ W, int64_t K,
                                                               Epilogue e)
 {
-    using frag = typename FewStep<T>::frag;
+    using frag = typename Step<T>::frag;
     constexpr int PIECE = WAVES * 128, n = 16 / sizeof(T), BK = PIECE / sizeof(T);      // two MFMA steps per wave
     constexpr int CB = GATED ? 16 : 16 * RT, LOADS = 2 * (RT + NT), SLOT = 16 * (RT + NT) * PIECE;
     constexpr int PER_LOAD = 1024 / PIECE, LANES = kWave / PER_LOAD;                   // rows of a wave's load, lanes of a row
@@ -277,7 +260,7 @@ __global__ __launch_bounds__(WAVES *kWave) void few_rows_stream_kernel(const T *
 #pragma unroll
             for (int i = 0; i < RT; ++i)
 #pragma unroll
-                for (int t = 0; t < NT; ++t) acc[i][t] = FewStep<T>::mma(w[i], x[t], acc[i][t]);
+                for (int t = 0; t < NT; ++t) acc[i][t] = Step<T>::mma(w[i], x[t], acc[i][t]);
         }
         use = use + 1 == SLOTS ? 0 : use + 1;
     }
@@ -333,11 +316,12 @@ template <typename T> int few_rows_by_size(const void *X, const void *W, int64_t
 }  // namespace
 
 // Whether these kernels take a forward pass: up to 16 rows always, up to 32 where the tile product would have to copy W to whole
-// chunks first or W is small (32 x 14336 x 4096 bf16: 27 us here, 28 there; 32 x 4096 x 28672: 57 here, 51 there).
+// chunks first or W is no more than 24 MB (20 rows, 2048 x 2048: 7.3 us here, 8.9 there; 32 x 1024 x 2816 SwiGLU 7, 11;
+// 32 x 4096 x 4096 14.2, 12.9; 32 x 14336 x 4096 43, 24).
 bool linear_few_rows_serve(int64_t T, int64_t K, int64_t N, int dtype)
 {
     const int64_t size = dtype == OPMX_DTYPE_F32 ? 4 : 2;
-    return T <= 16 || (T <= 32 && (K * size % 16 != 0 || N * K * size < kFewStreamBytes));
+    return T <= 16 || (T <= 32 && (K * size % 16 != 0 || N * K * size < kFewDirectBytes));
 }
 
 int launch_linear_few_rows(const void *X, const void *W, int64_t K, int dtype, const Epilogue &e, hipStream_t s)

@@ -16,7 +16,7 @@
 // What does not exist (rows, columns, k past the end) is loaded from an offset that the descriptor's range check
 // answers with zeros.  The k order of a fragment is the same in both layouts, whatever it is.
 #include "linear_epilogue.h"
-#include "moe_gemm.h"
+#include "linear_step.h"
 
 #include <type_traits>
 
@@ -25,7 +25,6 @@ namespace {
 
 constexpr int kTileBytes = 128;                 // of k per row
 constexpr uint32_t kNowhere = 0x80000000u;      // past every descriptor
-#define OPMX_LDS(p) ((void __attribute__((address_space(3))) *)(p))
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t descriptor(const char *base)
 {
@@ -35,25 +34,6 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t descriptor(const char *base)
     return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void *>((static_cast<uint64_t>(hi) << 32) | lo), 0,
                                              0x7FFFFFFF, 0x00020000);
 }
-
-template <typename T> struct Step;
-template <> struct Step<f16> {
-    using frag = half8_t;
-    static __device__ __forceinline__ float4_t mma(frag p, frag q, float4_t c) { return Mfma<f16>::m16(p, q, c); }
-};
-template <> struct Step<bf16> {
-    using frag = bf16x8_t;
-    static __device__ __forceinline__ float4_t mma(frag p, frag q, float4_t c) { return Mfma<bf16>::m16(p, q, c); }
-};
-template <> struct Step<float> {
-    using frag = float4_t;
-    static __device__ __forceinline__ float4_t mma(frag p, frag q, float4_t c)
-    {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(p[j], q[j], c, 0, 0, 0);
-        return c;
-    }
-};
 
 // How k-major rows are permuted inside a k row of LDS (ROWS values): the index of a unit (32 bytes; fp32: 64) is xored with
 // this.  A transposing read takes, for every half of the wave, one unit of k rows 0 to 3 and 8 to 11 (from a multiple of
@@ -409,14 +389,18 @@ __global__ __launch_bounds__(WM *WN *kWave, 2) void linear_gemm_kernel(Operand P
 //
 // Against eight waves of 128 x 64 the wave tiles read a third less from LDS per operation: with eight, reads and
 // arriving loads together keep LDS busy for all of the 2048 clocks that the matrix units take per k-tile.  One wave
-// per SIMD has to overlap by itself: the 64 MFMAs of a k step (32 values) go in four blocks of 16, and each block
-// reads four of the sixteen fragments of the next step behind its first MFMAs and waits for them at its end.  The
-// accumulators fill the 256 accumulation registers.  A block is one piece of assembly: its order is the issue order,
-// the wait stands where the reads are, and the compiler's own wait in front of transposing reads does not come in.
+// per SIMD has to overlap by itself, so the order of MFMAs, LDS reads and loads is written down, in assembly; the
+// accumulators fill the 256 accumulation registers.  A k-tile is two steps of 32 k values, 64 MFMAs each; while one step is
+// multiplied the fragments of the next are read, and k-tile t + 2 is loaded into the stage of k-tile t once all waves
+// have read all of that.
+//   Both operands along k: every MFMA is a piece of assembly, what stands between is the compiler's.
+//   k over rows of one or both: the fragments come through transposing reads, in front of which the compiler would wait
+//   for all loads.  There a block of 16 MFMAs with the four fragments that it reads, and the wait for them, is one piece.
 //
-// Step 0 of k-tile t reads the fragments of step 1 from the same stage; after it all waves have read all of the stage.
-// Between the steps a wave waits for its loads of k-tile t + 1 (issued a k-tile ago) and for the other waves; step 1
-// then reads the first fragments of k-tile t + 1 from the other stage and loads k-tile t + 2 into this one.
+// bfloat16, 4096 x 28672 outputs over 4096: 742 us, 1300 TFLOP/s (eight waves: 820 us); 4096 x 8192 over 14336 785 us; the
+// gradients of the same 720 to 890 us.  The matrix units work for 68 % of the clocks; k-tiles of MFMAs alone would take
+// 2048 clocks of 2950.  Reads spread over 48 MFMAs instead of 32, loads every third MFMA instead of every fifth, and
+// blocks of 32 MFMAs made no difference or a slower one.
 #define OPMX_WIDE_ROWS(OP)                                                                                            \
     asm volatile("s_nop 1\n\t"                                                                                        \
                  "v_mfma_f32_16x16x32_" OP " %0, %20, %24, %0\n\t"                                                    \
@@ -602,10 +586,9 @@ __global__ __launch_bounds__(256, 1) void linear_gemm_wide_kernel(Operand P, Ope
 
     uint32_t cur = 0, at[4];
     if constexpr (!PK && !QK) {
-        // Rows along k on both sides: fragments are ordinary reads, so every MFMA can be its own piece of assembly and the
-        // compiler's waits are exact.  Step 0 reads the other step's fragments behind its first 32 MFMAs, then the
-        // stage is free and the loads of k-tile t + 2 go out, one behind every third MFMA, until a sixth of the way
-        // into step 1; in its middle k-tile t + 1 must have landed, almost one and a half k-tiles after its loads.
+        // Step 0 reads the other step's fragments behind its first 32 MFMAs.  After the 40th all waves have them: the stage
+        // is free, and the 16 loads of k-tile t + 2 go out behind every fifth MFMA from there on.  In the middle of step 1
+        // (11 of them are out) the loads of k-tile t + 1 must have landed, one and a half k-tiles after they went out.
         const char *p0 = smem + BM * kTileBytes, *q0 = smem;
         const int r = lane & 15, g = lane >> 4;
         const int slot[2] = {(g ^ ((r >> 1) & 7)) << 4, ((4 + g) ^ ((r >> 1) & 7)) << 4};
@@ -635,7 +618,7 @@ __global__ __launch_bounds__(256, 1) void linear_gemm_wide_kernel(Operand P, Ope
 #pragma unroll
             for (int m = 0; m < 64; ++m) {
                 Mfma<T>::m16_acc(pb[m % 8], qb[m / 8], acc[m % 8][m / 8]);
-                                if (m == 32) {
+                if (m == 32) {
                     asm volatile("s_waitcnt vmcnt(11)" ::: "memory");
                     __builtin_amdgcn_s_barrier();
                     asm volatile("" ::: "memory");
@@ -648,35 +631,39 @@ __global__ __launch_bounds__(256, 1) void linear_gemm_wide_kernel(Operand P, Ope
             k_left -= BK;
             cur ^= STAGE;
         }
-    } else
-    for (int kt = 0; kt < nk; ++kt) {
-        rp.template at<0, 1>(cur, at);
-        wide_block<0, 0, 0, PK, 1>(acc, pa, qa, pb, at);
-        rp.template at<4, 1>(cur, at);
-        wide_block<1, 0, 4, PK, 1>(acc, pa, qa, pb, at);
-        rq.template at<0, 1>(cur, at);
-        wide_block<0, 1, 0, QK, 1>(acc, pa, qa, qb, at);
-        rq.template at<4, 1>(cur, at);
-        wide_block<1, 1, 4, QK, 1>(acc, pa, qa, qb, at);
+    } else {
+        // Step 0 (pa, qa) reads the fragments of step 1 from the same stage; then the wave waits for its loads of k-tile t + 1
+        // (issued a k-tile ago) and for the other waves, and step 1 reads the first fragments of k-tile t + 1 from the other
+        // stage while k-tile t + 2 is loaded into this one.
+        for (int kt = 0; kt < nk; ++kt) {
+            rp.template at<0, 1>(cur, at);
+            wide_block<0, 0, 0, PK, 1>(acc, pa, qa, pb, at);
+            rp.template at<4, 1>(cur, at);
+            wide_block<1, 0, 4, PK, 1>(acc, pa, qa, pb, at);
+            rq.template at<0, 1>(cur, at);
+            wide_block<0, 1, 0, QK, 1>(acc, pa, qa, qb, at);
+            rq.template at<4, 1>(cur, at);
+            wide_block<1, 1, 4, QK, 1>(acc, pa, qa, qb, at);
 
-        wait_loads<0>();
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
+            wait_loads<0>();
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
 
-        char *free_stage = smem + cur;
-        cur ^= STAGE;
-        load4(free_stage, I0{});
-        rp.template at<0, 0>(cur, at);
-        wide_block<0, 0, 0, PK, 0>(acc, pb, qb, pa, at);
-        load4(free_stage, I1{});
-        rp.template at<4, 0>(cur, at);
-        wide_block<1, 0, 4, PK, 0>(acc, pb, qb, pa, at);
-        load4(free_stage, I2{});
-        rq.template at<0, 0>(cur, at);
-        wide_block<0, 1, 0, QK, 0>(acc, pb, qb, qa, at);
-        load4(free_stage, I3{});
-        rq.template at<4, 0>(cur, at);
-        wide_block<1, 1, 4, QK, 0>(acc, pb, qb, qa, at);
+            char *free_stage = smem + cur;
+            cur ^= STAGE;
+            load4(free_stage, I0{});
+            rp.template at<0, 0>(cur, at);
+            wide_block<0, 0, 0, PK, 0>(acc, pb, qb, pa, at);
+            load4(free_stage, I1{});
+            rp.template at<4, 0>(cur, at);
+            wide_block<1, 0, 4, PK, 0>(acc, pb, qb, pa, at);
+            load4(free_stage, I2{});
+            rq.template at<0, 0>(cur, at);
+            wide_block<0, 1, 0, QK, 0>(acc, pb, qb, qa, at);
+            load4(free_stage, I3{});
+            rq.template at<4, 0>(cur, at);
+            wide_block<1, 1, 4, QK, 0>(acc, pb, qb, qa, at);
+        }
     }
     // The last MFMAs retire before anything touches an accumulator: the compiler does not know of them.  The empty
     // statements make every use of one come after the wait.
