@@ -3,11 +3,14 @@
 // backward reads the 8-bit input and dY and writes dX.
 //   Y = g a s(beta a),  s the logistic function, X = (a | g)
 //   dg = dY a s(beta a),  da = dY g s(beta a) (1 + beta a (1 - s(beta a)))      at the held a, g
-// All of it is elementwise and bound by memory.  A lane takes 16 bytes of a row, so a block of 32 values lies in
+// All of it is elementwise and bound by memory: [16384, 2 x 14336] bfloat16 moves 1.89 GB forward, in 345 us (5.5 TB/s), and as
+// much backward, in 315 us (6.0 TB/s; a copy of that size reaches 4.9).  A lane takes 16 bytes of a row, so a block of 32 values lies in
 // 4 (16-bit types) or 8 (fp32) neighbouring lanes and its largest magnitude is two or three cross-lane steps.
 // Rows may start at any address: loads and stores of 16 bytes need no alignment on this part, only the
 // last values of a row that fill no chunk go one by one.
 #include "checkpoint8.h"
+
+#include <type_traits>
 
 namespace opmx {
 namespace {
@@ -170,21 +173,26 @@ __global__ __launch_bounds__(256) void swiglu8_backward_kernel(const T *__restri
     const int64_t c = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) * n, left = D - c;
     if (left <= 0) return;
     const int64_t step = static_cast<int64_t>(gridDim.y) * blockDim.y;
-    for (int64_t r = static_cast<int64_t>(blockIdx.y) * blockDim.y + threadIdx.y; r < R; r += step) {
-        const uint32_t ca = codes[r * 2 * blocks + c / kBlock8], cg = codes[(r * 2 + 1) * blocks + c / kBlock8];
-        const Bytes<n> qa = load_bytes<n>(q + r * 2 * D + c, left), qg = load_bytes<n>(q + r * 2 * D + D + c, left);
-        const Chunk<T> dy = load_chunk(dY + r * D + c, left);
-        Chunk<T> da, dg;
+    // `here` values exist: a constant where all do, so that nothing stands between the loads (338 us without, 315 with)
+    auto rows = [&](auto here) {
+        for (int64_t r = static_cast<int64_t>(blockIdx.y) * blockDim.y + threadIdx.y; r < R; r += step) {
+            const uint32_t ca = codes[r * 2 * blocks + c / kBlock8], cg = codes[(r * 2 + 1) * blocks + c / kBlock8];
+            const Bytes<n> qa = load_bytes<n>(q + r * 2 * D + c, here), qg = load_bytes<n>(q + r * 2 * D + D + c, here);
+            const Chunk<T> dy = load_chunk(dY + r * D + c, here);
+            Chunk<T> da, dg;
 #pragma unroll
-        for (int j = 0; j < n; ++j) {
-            const float a = from_steps(qa.v[j], ca), g = from_steps(qg.v[j], cg), d = to_f32(dy.v[j]);
-            const float s = logistic<T>(beta * a);
-            dg.v[j] = from_f32<T>(d * a * s);
-            da.v[j] = from_f32<T>(d * g * (s + beta * a * s * (1.0f - s)));
+            for (int j = 0; j < n; ++j) {
+                const float a = from_steps(qa.v[j], ca), g = from_steps(qg.v[j], cg), d = to_f32(dy.v[j]);
+                const float s = logistic<T>(beta * a);
+                dg.v[j] = from_f32<T>(d * a * s);
+                da.v[j] = from_f32<T>(d * g * (s + beta * a * s * (1.0f - s)));
+            }
+            store_chunk(dX + r * 2 * D + c, da, here);
+            store_chunk(dX + r * 2 * D + D + c, dg, here);
         }
-        store_chunk(dX + r * 2 * D + c, da, left);
-        store_chunk(dX + r * 2 * D + D + c, dg, left);
-    }
+    };
+    if (left >= n) rows(std::integral_constant<int, n>{});
+    else rows(left);
 }
 
 // Blocks of 256 lanes over a strip of a row, or over several rows where rows are short; the lanes of a
