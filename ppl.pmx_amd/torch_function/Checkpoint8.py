@@ -103,6 +103,6 @@ class SwiGLUCheckpoint8(torch.autograd.Function):
 
 
 def swiglu_checkpoint8(X: torch.Tensor, beta: float = 1.0):
-    """``swiglu`` for training: the same output, and the gradient of X taken at X as 8 bits hold it.  Where no
-    gradient is asked for, nothing is kept.  X may be changed in place afterwards: only its 8-bit form is used."""
+    """``swiglu`` for training: the same output (in float16 a value halfway between two may round the other way), and
+    the gradient of X taken at X as 8 bits hold it.  Where no gradient is asked for, it is ``swiglu``, and nothing is kept.  X may be changed in place afterwards: only its 8-bit form is used."""
     return SwiGLUCheckpoint8.apply(X, beta)

@@ -15,7 +15,7 @@ def _dense(t):
 
 class LinearEpilogue(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, X, W, B, residual, in_features, out_features, activation, checkpoint8):
+    def forward(ctx, X, W, B, residual, in_features, out_features, activation, checkpoint8, train):
         name = "linear_epilogue"
         dev = _lib.require_gpu(name, X, W, B, residual)
         if activation not in _lib.ACTIVATIONS:
@@ -39,7 +39,7 @@ class LinearEpilogue(torch.autograd.Function):
             raise TypeError("{}: X, W, B and residual must share one dtype".format(name))
         dt = _lib.dtype_id(W, name)
         T = _rows(lead)
-        need = ctx.needs_input_grad
+        need = ctx.needs_input_grad if train else (False,) * 4
         keep_h = activation != "none" and any(need[:3])
         L = _lib.lib()
         with _lib.on_device(dev):
@@ -69,7 +69,7 @@ class LinearEpilogue(torch.autograd.Function):
     def backward(ctx, dY):
         need = ctx.needs_input_grad
         if not any(need[:3]):
-            return None, None, None, dY, None, None, None, None
+            return None, None, None, dY, None, None, None, None, None
         X, W, H, q, code = ctx.saved_tensors
         T, K, N, dt, act = ctx.sizes
         xshape, dtype, dev = ctx.shapes
@@ -85,7 +85,7 @@ class LinearEpilogue(torch.autograd.Function):
                 _lib.ptr(dYc), _lib.ptr(X), _lib.ptr(q), _lib.ptr(code), _lib.ptr(W), _lib.ptr(H), T, K, N, dt, act,
                 _lib.ptr(dX), _lib.ptr(dW), _lib.ptr(dB), _lib.ptr(ws), ws.numel(), _lib.stream_ptr(dev)),
                 "linear_epilogue backward")
-        return dX, dW, dB, dY if need[3] else None, None, None, None, None
+        return dX, dW, dB, dY if need[3] else None, None, None, None, None, None
 
 
 def linear_epilogue(X: torch.Tensor, W: torch.Tensor, B: torch.Tensor, residual: torch.Tensor, in_features: int,
@@ -95,6 +95,10 @@ def linear_epilogue(X: torch.Tensor, W: torch.Tensor, B: torch.Tensor, residual:
     X [*, in_features], W [out_features, in_features], B [out_features] or None; ``activation`` is none, silu, gelu,
     gelu_tanh or swiglu (as ``swiglu``: first half the gated one, output and residual [*, out_features / 2]).
     Differentiable in X, W, B and residual.  Where an activation needs it, X W^T + B is kept for the backward pass, in
-    4 bytes per value for float32 and in 3 for the 16-bit types.  ``checkpoint8`` keeps X for the gradient of W in 8 bits (``checkpoint8_pack``) instead of
-    as it is; the other gradients do not change."""
-    return LinearEpilogue.apply(X, W, B, residual, in_features, out_features, activation, bool(checkpoint8))
+    4 bytes per value for float32 and in 3 for the 16-bit types (under ``torch.no_grad`` nothing is).  ``checkpoint8``
+    keeps X for the gradient of W in 8 bits (``checkpoint8_pack``) instead of as it is; the other gradients do not
+    change.
+    A backward pass is captured into a graph together with its forward pass, with no eager pass over the same leaves
+    still alive: torch runs a backward pass on its forward pass's stream, which is not being captured."""
+    return LinearEpilogue.apply(X, W, B, residual, in_features, out_features, activation, bool(checkpoint8),
+                                torch.is_grad_enabled())

@@ -157,3 +157,22 @@ def test_a_few_steps_of_descent():
                 w -= 0.01 * g
     for w, old in zip(b.weights, before):
         assert bool(torch.isfinite(w).all()) and not torch.equal(w, old)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_nothing_is_kept_without_gradients(dtype):
+    """Under no_grad, weights that ask for gradients cost no memory beside the output."""
+    OPMX = opmx()
+    T, K, N = 512, 64, 2048
+    x, w = torch.randn(T, K, device=dev(), dtype=dtype), torch.randn(N, K, device=dev(), dtype=dtype, requires_grad=True)
+    kept = []
+    for grads in (False, True):
+        with torch.set_grad_enabled(grads):
+            torch.cuda.synchronize()
+            before = torch.cuda.memory_allocated()
+            y = OPMX.linear_epilogue(x, w, None, None, K, N, "gelu", checkpoint8=True)
+            kept.append(torch.cuda.memory_allocated() - before - y.numel() * y.element_size())
+        if not grads:
+            want = y
+        assert y.requires_grad == grads and torch.equal(y, want)
+    assert kept[0] <= 512 and kept[1] >= T * N            # X W^T, a byte a value at least
