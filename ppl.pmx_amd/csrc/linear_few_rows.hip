@@ -1,10 +1,10 @@
-// Linear with epilogue for few rows of X (decoding: one token up to 32): reading W once at the memory's pace.
+// Linear with epilogue for few rows of X (decoding: one token up to 32, 64 with short rows): reading W once at the memory's pace.
 //
 //   H[t, c] = sum_k X[t, k] W[c, k], then the epilogue
 //
 // A workgroup of eight waves owns 16 RT rows of W (with SwiGLU 16 of each half) and all rows of X over the whole of k:
 // nothing has to be joined by a second launch.  The waves share out k in pieces of 128 bytes of a row and feed the
-// MFMAs straight from global memory, eight pieces in flight per wave; the partial sums meet in LDS and are added in wave
+// MFMAs straight from global memory, one batch of pieces ahead; the partial sums meet in LDS and are added in wave
 // order.  W is the A operand, so a lane holds four neighbouring columns of a row of Y.  X comes from L2: 16 RT rows
 // of W share one reading of it, and a row of X past the last one is the last one again, never stored.
 // Rows of W and X may start anywhere their type allows; the last k values that fill no piece go one by one.
@@ -72,7 +72,7 @@ __global__ __launch_bounds__(kFewWaves *kWave, 2) void few_rows_kernel(const T *
 {
     using frag = typename Step<T>::frag;
     constexpr int n = 16 / sizeof(T), STEP = 4 * n;          // k values of a lane's load, of one MFMA step
-    constexpr int U = NT * RT >= 4 ? 4 : 8;                  // steps in flight
+    constexpr int U = NT * RT >= 4 ? 2 : 4;                  // steps of a batch; two batches are in flight
     constexpr int CB = GATED ? 16 : 16 * RT;                 // columns of Y per workgroup
     __shared__ __attribute__((aligned(16))) float4_t part[kFewWaves][RT][NT][kWave];
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -93,26 +93,49 @@ __global__ __launch_bounds__(kFewWaves *kWave, 2) void few_rows_kernel(const T *
 #pragma unroll
         for (int t = 0; t < NT; ++t) acc[i][t] = float4_t{0.f, 0.f, 0.f, 0.f};
 
-    // steps 2 v and 2 v + 1 (128 bytes of a row) belong to wave v mod 8
+    // steps 2 v and 2 v + 1 (128 bytes of a row) belong to wave v mod 8; they go in batches of U, one batch's loads ahead
     const int steps = static_cast<int>(K / STEP);
+    constexpr int AHEAD = U / 2 * 2 * kFewWaves;             // from a batch to the next
     int s = wave * 2;
-    for (; s + (U / 2 - 1) * 2 * kFewWaves + 1 < steps; s += U / 2 * 2 * kFewWaves) {
-        frag w[U][RT], x[U][NT];
+    auto load = [&](int at, frag (&w)[U][RT], frag (&x)[U][NT]) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int64_t k = static_cast<int64_t>(s + u / 2 * 2 * kFewWaves + u % 2) * STEP;
+            const int64_t k = static_cast<int64_t>(at + u / 2 * 2 * kFewWaves + u % 2) * STEP;
 #pragma unroll
             for (int i = 0; i < RT; ++i) w[u][i] = load_frag<frag, true>(wp[i] + k);
 #pragma unroll
             for (int t = 0; t < NT; ++t) x[u][t] = load_frag<frag, false>(xp[t] + k);
         }
-        __builtin_amdgcn_sched_barrier(0);                   // all of them before the first product
+        __builtin_amdgcn_sched_barrier(0);                   // all of them before the next product
+    };
+    auto multiply = [&](const frag (&w)[U][RT], const frag (&x)[U][NT]) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int i = 0; i < RT; ++i)
 #pragma unroll
                 for (int t = 0; t < NT; ++t) acc[i][t] = Step<T>::mma(w[u][i], x[u][t], acc[i][t]);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    const int last = steps - ((U / 2 - 1) * 2 * kFewWaves + 2);       // where a whole batch may begin at most
+    if (s <= last) {
+        frag wa[U][RT], xa[U][NT], wb[U][RT], xb[U][NT];
+        load(s, wa, xa);
+        for (; s + 2 * AHEAD <= last; s += 2 * AHEAD) {
+            load(s + AHEAD, wb, xb);
+            multiply(wa, xa);
+            load(s + 2 * AHEAD, wa, xa);
+            multiply(wb, xb);
+        }
+        if (s + AHEAD <= last) {
+            load(s + AHEAD, wb, xb);
+            multiply(wa, xa);
+            multiply(wb, xb);
+            s += AHEAD;
+        } else {
+            multiply(wa, xa);
+        }
+        s += AHEAD;
     }
     for (; s < steps; s += 2 * kFewWaves)
         for (int u = 0; u < 2 && s + u < steps; ++u) {
@@ -305,6 +328,7 @@ template <typename T, int NT> int few_rows(const void *X, const void *W, int64_t
 // and two workgroups per CU.  1024 bytes by eight waves, deeper pieces, and workgroups that start k apart were not faster.
 template <typename T> int few_rows_by_size(const void *X, const void *W, int64_t K, const Epilogue &e, hipStream_t s)
 {
+    if (e.rows > 32) return few_rows<T, 4>(X, W, K, e, s);
     if (e.rows > 16) return few_rows<T, 2>(X, W, K, e, s);
     const bool whole = K * sizeof(T) % 16 == 0 && aligned16(X) && aligned16(W);
     if (!whole || e.N * K * static_cast<int64_t>(sizeof(T)) < kFewStreamBytes) return few_rows<T, 1>(X, W, K, e, s);
@@ -317,11 +341,14 @@ template <typename T> int few_rows_by_size(const void *X, const void *W, int64_t
 
 // Whether these kernels take a forward pass: up to 16 rows always, up to 32 where the tile product would have to copy W to whole
 // chunks first or W is no more than 24 MB (20 rows, 2048 x 2048: 7.3 us here, 8.9 there; 32 x 1024 x 2816 SwiGLU 7, 11;
-// 32 x 4096 x 4096 14.2, 12.9; 32 x 14336 x 4096 43, 24).
+// 32 x 4096 x 4096 14.2, 12.9; 32 x 14336 x 4096 43, 24), up to 64 with short rows of W, where every workgroup's own
+// reading of X is short too (64 x 1024 x 1024 float16 7.5, 9.5; 64 x 1024 x 2816 float32 13.8, 15.5; 64 x 2048 x 2048 float16
+// 12.2, 9.7).
 bool linear_few_rows_serve(int64_t T, int64_t K, int64_t N, int dtype)
 {
     const int64_t size = dtype == OPMX_DTYPE_F32 ? 4 : 2;
-    return T <= 16 || (T <= 32 && (K * size % 16 != 0 || N * K * size < kFewDirectBytes));
+    if (T > 32) return T <= 64 && K <= 1024;
+    return T <= 16 || K * size % 16 != 0 || N * K * size < kFewDirectBytes;
 }
 
 int launch_linear_few_rows(const void *X, const void *W, int64_t K, int dtype, const Epilogue &e, hipStream_t s)

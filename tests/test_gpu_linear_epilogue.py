@@ -144,6 +144,14 @@ def test_large_tiles(dtype, act, T, K, N):
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("act,T,K,N", [("swiglu", 3333, 1000, 3600), ("gelu", 3500, 1041, 3335), ("none", 3500, 3600, 1100),
+                                       ("silu", 1550, 3500, 3600)])
+def test_the_largest_tiles(dtype, act, T, K, N):
+    """256 x 256 tiles, which want 16 k-tiles (24 for the gradient of W): forward twice, gradient of X, gradient of W."""
+    check(T, K, N, dtype, act)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_large_tiles_in_both_gradients(dtype):
     check(200, 3500, 3600, dtype, "silu")        # dW [3600, 3500]: k is the 200 rows
     check(3500, 3600, 200, dtype, "none")        # dX [3500, 3600]
