@@ -584,6 +584,9 @@ __global__ __launch_bounds__(256, 1) void linear_gemm_wide_kernel(Operand P, Ope
     fragments<T, BN, PK, 0, 8>(smem + BM * kTileBytes, wn * 8, lane, pa);
     fragments<T, BM, QK, 0, 8>(smem, wm * 8, lane, qa);
 
+    // The wait states between the last MFMA and the first use of an accumulator, at the end of every k-tile: the compiler does
+    // not know of the MFMAs, and copies accumulators as soon as the loop is left, in front of any wait that stands there.
+    auto retire = [] { asm volatile("s_nop 11" ::: "memory"); };
     uint32_t cur = 0, at[4];
     if constexpr (!PK && !QK) {
         // Step 0 reads the other step's fragments behind its first 32 MFMAs.  After the 40th all waves have them: the stage
@@ -626,6 +629,7 @@ __global__ __launch_bounds__(256, 1) void linear_gemm_wide_kernel(Operand P, Ope
                 if (m < 53 && (m - 2) % 5 == 0) load1(5 + (m - 2) / 5);
                 if (m > 32 && m % 2 == 1) read(cur ^ STAGE, 0, (m - 33) / 2, pa, qa);
             }
+            retire();
             lq.next();
             lp.next();
             k_left -= BK;
@@ -663,15 +667,9 @@ __global__ __launch_bounds__(256, 1) void linear_gemm_wide_kernel(Operand P, Ope
             load4(free_stage, I3{});
             rq.template at<4, 0>(cur, at);
             wide_block<1, 1, 4, QK, 0>(acc, pb, qb, qa, at);
+            retire();
         }
     }
-    // The last MFMAs retire before anything touches an accumulator: the compiler does not know of them.  The empty
-    // statements make every use of one come after the wait.
-    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) asm volatile("" : "+a"(acc[j][i]));
     wait_loads<0>();                                     // the epilogue uses the same memory
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
