@@ -76,6 +76,10 @@ def test_large_product_assembly_is_hazard_free(tmp_path):
     assert len(kernels) == 8                        # two types, four layouts
     for name, body in kernels:
         assert findings(body) == (128, []), name
+        # what the counted waits count: 16 loads per k-tile, straight to LDS, and no other access to memory
+        loop = [line.strip() for line in body[body.index("v_mfma"):body.rindex("v_mfma")].split("\n")]
+        loads = [line for line in loop if line.startswith(("buffer_", "global_", "flat_"))]
+        assert len(loads) == 16 and all("lds" in line for line in loads), name
 
 
 def test_the_check_finds_what_it_looks_for():
