@@ -399,8 +399,9 @@ __global__ __launch_bounds__(WM *WN *kWave, 2) void linear_gemm_kernel(Operand P
 //
 // bfloat16, 4096 x 28672 outputs over 4096: 742 us, 1300 TFLOP/s (eight waves: 820 us); 4096 x 8192 over 14336 785 us; the
 // gradients of the same 720 to 890 us.  The matrix units work for 68 % of the clocks; k-tiles of MFMAs alone would take
-// 2048 clocks of 2950.  Reads spread over 48 MFMAs instead of 32, loads every third MFMA instead of every fifth, and
-// blocks of 32 MFMAs made no difference or a slower one.
+// 2048 clocks of 2950.  Reads spread over 48 MFMAs instead of 32, loads every third MFMA instead of every fifth,
+// blocks of 32 MFMAs, and workgroups that load their next tile during the epilogue made no difference or a slower one;
+// 32 x 32 x 16 MFMAs 770 us.
 #define OPMX_WIDE_ROWS(OP)                                                                                            \
     asm volatile("s_nop 1\n\t"                                                                                        \
                  "v_mfma_f32_16x16x32_" OP " %0, %20, %24, %0\n\t"                                                    \
