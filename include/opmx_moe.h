@@ -287,7 +287,8 @@ int opmx_swiglu_checkpoint8_backward(const void *dY, const int8_t *q, const uint
  * X, W, dY start at multiples of 16 bytes where K (dY: N, without an activation) is a multiple of 16 bytes
  * (OPMX_ERR_ALIGNMENT otherwise), the others anywhere their type allows.
  * workspace: opmx_linear_epilogue[_backward]_workspace_bytes(), 256-byte aligned, contents arbitrary, not shared with
- * a call running at the same time (may be NULL where that says 256: nothing is needed).  Results do not vary from call to call.  K < 2^21. */
+ * a call running at the same time (may be NULL where that says 256: nothing is needed).  Results do not vary from call to
+ * call.  K, N < 2^21, T < 2^31. */
 size_t opmx_linear_epilogue_kept_bytes(int64_t T, int64_t N, int dtype);
 size_t opmx_linear_epilogue_workspace_bytes(int64_t T, int64_t K, int64_t N, int dtype, int activation);
 int opmx_linear_epilogue(const void *X, const void *W, const void *B, const void *R, int64_t T, int64_t K, int64_t N,
