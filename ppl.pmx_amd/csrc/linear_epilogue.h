@@ -231,9 +231,9 @@ struct Operand {
     int64_t pitch;
     bool k_major;
 };
-// Tiles of C: 256 x 256 by four waves of 128 x 128 (16-bit types, k in one range); 128 x 128 with two k-tiles in LDS and
-// 64 x 128 with three, each by four waves and two workgroups to a CU.
-enum class Tile { k256, k128, k64 };
+// Tiles of C: 256 x 256 by four waves of 128 x 128 (16-bit types, k in one range); 128 x 128 with two k-tiles in LDS, 64 x 128
+// and (fp32) 32 x 128 with three, each by four waves and two workgroups to a CU.
+enum class Tile { k256, k128, k64, k32 };
 // ranges > 1: k is cut into that many ranges, e.part must hold their sums.
 int launch_linear_gemm(const Operand &P, const Operand &Q, int64_t Kc, int dtype, const Epilogue &e, Tile tile, int ranges,
                        hipStream_t s);

@@ -219,21 +219,26 @@ Cut cut_for(int64_t rows, int64_t ncols, int64_t Kc, bool gated, bool p_rows, bo
     // More tiles than CUs: 128 x 128 (float16, 3000 x 2816 outputs over 2048: 54 us, 64 x 128 55, the gradients 47 and 55).
     // Fewer: 64 x 128 (512 x 1024 over 1024 9 us, 128 x 128 13; 100 x 2048 over 1408 11 and 17), with k in ranges where it is long.
     if (rows > 64 && ceil_div(rows, 128) * columns > 256) return c;
-    c.tile = Tile::k64;
-    const int64_t tiles = ceil_div(rows, 64) * columns;
-    // Microseconds of a k-tile, of one workgroup on a CU and of two (fp32: bound by the matrix units at either), and of
-    // joining r ranges, fitted to the times of 1 to 16 ranges of 17 products with 20 to 2048 rows: the chosen ones are
-    // within 8 % of the best.
-    const double one = f32 ? 1.1 : p_rows ? 0.45 : 0.34, two = f32 ? 2.2 : p_rows ? 0.65 : 0.62;
+    // In fp32, where a tile of half the rows takes little more than half the matrix units' time, also 32 x 128 (512 x 1024
+    // over 1024 18 us, 64 x 128 21; 2048 x 2048 over 2048 150, 135).
+    //
+    // Microseconds of a k-tile, of one workgroup on a CU and of two, and of joining r ranges, fitted to the times of 1 to 16
+    // ranges of 27 products with 20 to 3000 rows: the chosen ones are within 8 % of the best.
     double best = 0;
-    for (int64_t r = 1; r <= 16 && (r == 1 || r * 4 <= nk); ++r) {
-        const int64_t load = ceil_div(tiles * r, 256);
-        const double mb = static_cast<double>(r * rows * width) * 4e-6;
-        const double us = static_cast<double>(ceil_div(nk, r)) * (static_cast<double>(load / 2) * two + static_cast<double>(load % 2) * one) +
-                          (r > 1 ? 3.0 + 0.4 * static_cast<double>(r) + 0.3 * mb : 0.0);
-        if (r == 1 || us < best) {
-            best = us;
-            c.ranges = static_cast<int>(r);
+    for (int half = 0; half < (f32 ? 2 : 1); ++half) {
+        const double one = half ? 0.63 : f32 ? 1.1 : p_rows ? 0.45 : 0.34, two = half ? 1.25 : f32 ? 2.2 : p_rows ? 0.65 : 0.62;
+        const int64_t tiles = ceil_div(rows, half ? 32 : 64) * columns;
+        for (int64_t r = 1; r <= 16 && (r == 1 || r * 4 <= nk); ++r) {
+            const int64_t load = ceil_div(tiles * r, 256);
+            const double mb = static_cast<double>(r * rows * width) * 4e-6;
+            const double us = static_cast<double>(ceil_div(nk, r)) *
+                                  (static_cast<double>(load / 2) * two + static_cast<double>(load % 2) * one) +
+                              (r > 1 ? 3.0 + 0.4 * static_cast<double>(r) + 0.3 * mb : 0.0);
+            if ((half == 0 && r == 1) || us < best) {
+                best = us;
+                c.tile = half ? Tile::k32 : Tile::k64;
+                c.ranges = static_cast<int>(r);
+            }
         }
     }
     if (c.ranges > 1) c.ranges = static_cast<int>(ceil_div(nk, ceil_div(nk, c.ranges)));      // none of them empty

@@ -41,7 +41,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t descriptor(const char *base)
 // halves of the banks apart.
 template <typename T, int ROWS> __device__ __forceinline__ int unit_swizzle(int k)
 {
-    if constexpr (sizeof(T) == 4) return (k >> 2) & 3;
+    if constexpr (sizeof(T) == 4) return (k >> 2) & (ROWS >= 64 ? 3 : 1);      // as many units as a k row has, four at most
     else if constexpr (ROWS * sizeof(T) >= 256) return (k & 3) | ((k >> 3 & 1) << 2);
     else return (k >> 1 & 1) | ((k >> 3 & 1) << 1);
 }
@@ -310,7 +310,7 @@ __global__ __launch_bounds__(WM *WN *kWave, 2) void linear_gemm_kernel(Operand P
     constexpr int STAGE = (BM + BN) * kTileBytes, BK = kTileBytes / sizeof(T);
     constexpr int BNO = GATED ? BN / 2 : BN;
     constexpr int PIECE = WTM < 64 ? WTM : 64;
-    static_assert(WTN == 64 && (TM == 2 || TM == 4), "the epilogue stages pieces of 64 columns");
+    static_assert(WTN == 64 && (TM == 1 || TM == 2 || TM == 4), "the epilogue stages pieces of 64 columns");
     using frag = typename Step<T>::frag;
     extern __shared__ __attribute__((aligned(16))) char smem[];
 
@@ -738,6 +738,9 @@ template <typename T> int by_tile(const Operand &P, const Operand &Q, int64_t Kc
             break;
         case Tile::k128: return by_layout<T, 128, 128, 2, 2, 2>(P, Q, Kc, e, ranges, s);
         case Tile::k64: return by_layout<T, 64, 128, 2, 2, 3>(P, Q, Kc, e, ranges, s);
+        case Tile::k32:
+            if constexpr (sizeof(T) == 4) return by_layout<T, 32, 128, 2, 2, 3>(P, Q, Kc, e, ranges, s);
+            break;
     }
     return OPMX_ERR_UNSUPPORTED;
 }

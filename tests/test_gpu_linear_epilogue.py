@@ -143,6 +143,13 @@ def test_large_tiles(dtype, act, T, K, N):
     check(T, K, N, dtype, act, checkpoint8=act == "swiglu")
 
 
+@pytest.mark.parametrize("act,T,K,N", [("gelu", 257, 1024, 1030), ("swiglu", 130, 1100, 640), ("none", 500, 515, 1027),
+                                       ("silu", 1025, 260, 1020), ("gelu", 97, 2816, 100), ("none", 2100, 300, 2050)])
+def test_float32_in_between(act, T, K, N):
+    """Tiles of 32, 64 and 128 rows, with k in ranges and whole."""
+    check(T, K, N, torch.float32, act, checkpoint8=act == "silu")
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("act,T,K,N", [("swiglu", 3333, 1000, 3600), ("gelu", 3500, 1041, 3335), ("none", 3500, 3600, 1100),
                                        ("silu", 1550, 3500, 3600)])
