@@ -431,6 +431,13 @@ __global__ __launch_bounds__(256) void balance_backward_kernel(const T *__restri
         }
 #define OPMX_DOT(D) dot += other_half<D>(dot)
         OPMX_HALVES(OPMX_DOT);
+        // dot is off by its own rounding and by that of a sum of p that is not quite 1; what is left of the mean of w - dot takes
+        // both away.  Where the w are nearly equal (all experts picked by every token) that is all there is.
+        float rest = 0.0f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) rest += z[i] * (wv[i] - dot);
+#define OPMX_REST(D) rest += other_half<D>(rest)
+        OPMX_HALVES(OPMX_REST);
         if (t >= Ttok) continue;             // (the last trip: nobody needs this lane again)
         T *out = dscores + t * E;
 #pragma unroll
@@ -440,7 +447,7 @@ __global__ __launch_bounds__(256) void balance_backward_kernel(const T *__restri
             T o[N];
 #pragma unroll
             for (int j = 0; j < N; ++j)
-                o[j] = from_f32<T>(keep ? scale * z[c * N + j] * (wv[c * N + j] - dot) : 0.0f);
+                o[j] = from_f32<T>(keep ? scale * z[c * N + j] * ((wv[c * N + j] - dot) - rest) : 0.0f);
             if constexpr (N == 1) out[e0] = o[0];
             else {
                 Vec16<T> q;

@@ -198,3 +198,15 @@ def test_captured_step_replays(T):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, step())), i
+
+
+@pytest.mark.parametrize("E", [2, 3, 8, 31])
+def test_no_gradient_where_every_expert_is_picked(E):
+    """k = E: all w are the same float, the gradient is zero, and what rounding leaves of it is of second order: p has a
+    relative error of 64 * 2^-24, and so has the mean that is taken away."""
+    OPMX = opmx()
+    s = logits(500, E, torch.float32, E).to(dev()).requires_grad_(True)
+    loss, count = OPMX.moe_balance_loss(s, E, E)
+    g, = torch.autograd.grad(loss, s)
+    assert bool((count == 500).all())
+    assert float(g.abs().max()) <= 2 * (64 * 2.0 ** -24) ** 2 / 500
