@@ -371,9 +371,14 @@ __global__ __launch_bounds__(WM *WN *kWave, 2) void linear_gemm_kernel(Operand P
         wait_loads<AHEAD>();                               // this wave's loads of tile kt, and its reads of tile kt - 1
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        load_next();                                       // into the stage that tile kt - 1 was in
         const char *cur = smem + stage * STAGE;
+        // Into the stage that tile kt - 1 was in, when the first products are under way (512 x 1024 over 1024 bfloat16 9.0 us, ahead of
+        // them 9.5; 3000 x 2816 over 2048 float32 365, 378; gradient of X 2048 x 4096 over 14336 bfloat16 208, 223); with two stages
+        // in LDS and the quickest products every moment counts for the loads (3000 x 2816 over 2048 bfloat16 54, ahead 51).
+        constexpr bool ahead = STAGES == 2 && sizeof(T) == 2 && !PK;
+        if constexpr (ahead) load_next();
         multiply(cur, std::integral_constant<int, 0>{});
+        if constexpr (!ahead) load_next();
         multiply(cur, std::integral_constant<int, 1>{});
         stage = stage + 1 == STAGES ? 0 : stage + 1;
     }
