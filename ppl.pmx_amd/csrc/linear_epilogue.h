@@ -59,7 +59,10 @@ template <typename T> __device__ __forceinline__ float slope(int act, float h)
     }
     const bool silu = act == OPMX_ACTIVATION_SILU;
     const float s = logistic_for<T>(silu ? h : 2.0f * kGeluC * (h + kGeluA * h * h * h));
-    const float dx = silu ? 1.0f : 2.0f * kGeluC * (1.0f + 3.0f * kGeluA * h * h);
+    // The factor of the tanh form overflows from |h| = 2e19 on, and infinity times a 1 - s or an s of 0 is NaN.  From |h| = 11 on s is 0
+    // or 1 exactly and any finite factor does: that of 32.
+    const float b = fminf(fabsf(h), 32.0f);
+    const float dx = silu ? 1.0f : 2.0f * kGeluC * (1.0f + 3.0f * kGeluA * b * b);
     return s + h * s * (1.0f - s) * dx;
 }
 

@@ -295,3 +295,38 @@ def test_captured_step_replays(dtype, T, K, N):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, step())), i
+
+
+def diagonal(dtype, rows):
+    """X and a W of ones on the diagonal: H is exactly X, and as large as the type allows."""
+    H = torch.tensor(rows, dtype=torch.float64).to(dtype)
+    return H, torch.eye(H.shape[1]).to(dtype)
+
+
+def large(dtype):
+    top = float(torch.finfo(dtype).max)
+    return [v for v in (0.0, 1.0, 10.5, 31.0, 33.0, 250.0, 6.0e4, 1.0e10, 3.0e18, 1.7e19, 2.0e19, 1.0e20, 1.0e30, 2.0e38)
+            if v <= top] + [top]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
+def test_slopes_of_large_finite_values(dtype, act):
+    """W = 1: H is X, the slopes are those of the formulas, also where h^2 or h^3 is beyond fp32, and every one is finite.
+    Tolerance: the slope's own arithmetic as in backward_tolerances, up to |h| = 12 (further out what it is off by is
+    h e^-12 and less), one rounding of dH and one of dX, which is a product with one term; e^-x in Y is off by |x| F
+    and 0 from x = 88 on."""
+    OPMX = opmx()
+    v = large(dtype)
+    H, W = diagonal(dtype, [v, [-x for x in v]])
+    dY = torch.full_like(H, 0.75)
+    X = H.to(dev()).requires_grad_(True)
+    Y = OPMX.linear_epilogue(X, W.to(dev()), None, None, len(v), len(v), act)
+    dX, = torch.autograd.grad(Y, X, dY.to(dev()))
+    Yr, (f,) = O.act(H.double(), act)
+    assert bool(torch.isfinite(Y).all()) and bool(torch.isfinite(dX).all())
+    u, near = torch.finfo(dtype).eps / 2, H.double().abs().clamp(max=12.0)
+    tiny = torch.finfo(dtype).smallest_normal
+    allow(Y, Yr, (u + 2 * F + F * (16 + 8 * H.double().abs().clamp(max=33.0) ** 2)) * Yr.abs() + tiny, "Y")
+    kept = CURVE[act] * near * (F if dtype == torch.float32 else 2.0 ** -16)
+    allow(dX, f * 0.75, 2.02 * u * f.abs() * 0.75 + 0.75 * (F * (16 + 4 * near) * (1 + near) + kept) + tiny, "dX")
