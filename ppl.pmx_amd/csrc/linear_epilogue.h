@@ -207,7 +207,7 @@ __device__ __forceinline__ void activate8(const Epilogue &e, int64_t row, int64_
     }
     if (GATED) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) h[j] = g[j] * h[j] * logistic_for<T>(h[j]);
+        for (int j = 0; j < 8; ++j) h[j] = g[j] * (h[j] * logistic_for<T>(h[j]));     // (g h alone may overflow where s is 0)
     } else if (e.act != OPMX_ACTIVATION_NONE) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) h[j] = activate<T>(e.act, h[j]);

@@ -74,8 +74,9 @@ __global__ __launch_bounds__(256) void slope_kernel(const T *__restrict__ dY, co
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const float s = logistic_for<T>(a[j]);
-                    h[j] = d[j] * a[j] * s;                                            // of the second half
-                    d[j] = d[j] * g[j] * (s + a[j] * s * (1.0f - s));
+                    // (the factors of d are finite where a and g are; d a and d g alone may overflow where s is 0)
+                    h[j] = d[j] * (a[j] * s);                                          // of the second half
+                    d[j] = d[j] * (g[j] * (s + a[j] * s * (1.0f - s)));
                     sum[0][j] += d[j];
                     sum[1][j] += h[j];
                 }

@@ -330,3 +330,29 @@ def test_slopes_of_large_finite_values(dtype, act):
     allow(Y, Yr, (u + 2 * F + F * (16 + 8 * H.double().abs().clamp(max=33.0) ** 2)) * Yr.abs() + tiny, "Y")
     kept = CURVE[act] * near * (F if dtype == torch.float32 else 2.0 ** -16)
     allow(dX, f * 0.75, 2.02 * u * f.abs() * 0.75 + 0.75 * (F * (16 + 4 * near) * (1 + near) + kept) + tiny, "dX")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_swiglu_of_large_finite_values(dtype):
+    """g a and dY g beyond fp32 where g a s(a) and the gradients are not.  W = 1.  Tolerance: s is off by 8 + |a| ulp (a fast
+    exponential's argument is), three products, the rounding of H in 24 bits, and the roundings of Y, dH and dX; where e^-a is
+    below fp32's range (a <= -88), s is 0 instead of 2^-126 at most."""
+    OPMX = opmx()
+    cases = [(-1e25, 1e25, 1.0), (-3e38, -3e38, 1e30), (-1e20, 3.0, 1e30), (-60.0, 1e38, 1.0), (-60.0, -3e37, 100.0),
+             (-20.0, 1e38, 8.0), (3e38, 0.25, 0.5), (1e20, 1e18, 1.0), (0.5, 2e38, 1.0), (-200.0, 3e38, 1.0), (0.0, 3e38, 1.0)]
+    a, g, d = [torch.tensor(c, dtype=torch.float64)[:, None] for c in zip(*cases)]
+    H, W = diagonal(dtype, torch.cat([a, g], 1).tolist())
+    dY = d.to(dtype)
+    X = H.to(dev()).requires_grad_(True)
+    Y = OPMX.linear_epilogue(X, W.to(dev()), None, None, 2, 2, "swiglu")
+    dX, = torch.autograd.grad(Y, X, dY.to(dev()))
+    Yr, (fa, fg) = O.act(H.double(), "swiglu")
+    a, g = H.double().chunk(2, 1)
+    ref = torch.cat([dY.double() * fa, dY.double() * fg], 1)
+    u, v = torch.finfo(dtype).eps / 2, F if dtype == torch.float32 else 2.0 ** -16
+    own = F * (12 + 2 * a.abs().clamp(max=88.0)) + v * (1 + a.abs().clamp(max=88.0))
+    gone = torch.where(a < -87, 2.0 ** -126 * a.abs().clamp(max=104.0), 0.0)       # past 104, e^-a is below 2^-149
+    tiny = torch.finfo(dtype).smallest_normal
+    assert bool((Yr.abs() < 3e38).all()) and bool((ref.abs() < 3e38).all())       # of the cases above
+    allow(Y, Yr, (own + u) * 1.01 * Yr.abs() + gone * g.abs() + tiny, "Y")
+    allow(dX, ref, (own + 2 * u) * 1.01 * ref.abs() + gone * dY.double().abs() * torch.cat([g.abs(), 1 + 0 * g], 1) + tiny, "dX")
