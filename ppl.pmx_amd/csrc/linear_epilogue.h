@@ -128,7 +128,8 @@ template <typename T> __device__ __forceinline__ void keep8(void *kept, int64_t 
         uint8_t b[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const uint32_t u = __float_as_uint(v[j]) + 0x80u;       // to nearest; infinities and NaNs stay what they are
+            // to nearest, but the last finite values not up to infinity; infinities and NaNs stay what they are
+            const uint32_t bits = __float_as_uint(v[j]), u = (bits & 0x7FFFFFFFu) < 0x7F7FFF80u ? bits + 0x80u : bits;
             a[j] = static_cast<uint16_t>(u >> 16);
             b[j] = static_cast<uint8_t>(u >> 8);
         }

@@ -356,3 +356,18 @@ def test_swiglu_of_large_finite_values(dtype):
     assert bool((Yr.abs() < 3e38).all()) and bool((ref.abs() < 3e38).all())       # of the cases above
     allow(Y, Yr, (own + u) * 1.01 * Yr.abs() + gone * g.abs() + tiny, "Y")
     allow(dX, ref, (own + 2 * u) * 1.01 * ref.abs() + gone * dY.double().abs() * torch.cat([g.abs(), 1 + 0 * g], 1) + tiny, "dX")
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
+def test_the_last_finite_sums_are_kept_finite(act):
+    """X W^T of 2^128 - 2^104, fp32's largest value, out of three bfloat16 terms: Y is an infinity of bfloat16, but the slope is
+    1 (0 on the other side) and so dX = dY (0), exactly: W = 1 for the first feature."""
+    OPMX = opmx()
+    one = [2.0 ** 128 - 2.0 ** 120, 2.0 ** 120 - 2.0 ** 112, 2.0 ** 112 - 2.0 ** 104]
+    X = torch.tensor([one, [-v for v in one]], dtype=torch.float64).to(torch.bfloat16)
+    assert torch.equal(X.double().sum(1), torch.tensor([2.0 ** 128 - 2.0 ** 104, 2.0 ** 104 - 2.0 ** 128], dtype=torch.float64))
+    x = X.to(dev()).requires_grad_(True)
+    Y = OPMX.linear_epilogue(x, torch.ones(1, 3, device=dev(), dtype=torch.bfloat16), None, None, 3, 1, act)
+    dX, = torch.autograd.grad(Y, x, torch.full((2, 1), 0.75, device=dev(), dtype=torch.bfloat16))
+    assert float(Y.detach()[0]) == float("inf") and float(Y.detach()[1]) == 0.0
+    assert torch.equal(dX.cpu(), torch.tensor([[0.75] * 3, [0.0] * 3], dtype=torch.bfloat16))
