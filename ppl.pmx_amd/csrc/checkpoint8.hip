@@ -10,6 +10,7 @@
 // last values of a row that fill no chunk go one by one.
 #include "checkpoint8.h"
 
+#include <cfloat>
 #include <type_traits>
 
 namespace opmx {
@@ -156,7 +157,11 @@ __global__ __launch_bounds__(256) void swiglu8_kernel(const T *__restrict__ X, i
 #pragma unroll
         for (int j = 0; j < n; ++j) {
             const float af = to_f32(a.v[j]);
-            y.v[j] = from_f32<T>(to_f32(g.v[j]) * af * logistic<T>(beta * af));
+            const float gf = to_f32(g.v[j]), s = logistic<T>(beta * af), ga = gf * af;
+            float yf = ga * s;
+            // the plain operator's product, except where g a is beyond fp32 (which it cannot be in float16)
+            if constexpr (!std::is_same<T, f16>::value) yf = fabsf(ga) == INFINITY ? gf * (af * s) : yf;
+            y.v[j] = from_f32<T>(yf);
         }
         store_chunk(Y + r * D + c, y, here);
         pack_chunk(a, here, q + r * 2 * D + c, codes + r * 2 * blocks + c / kBlock8);
@@ -184,8 +189,11 @@ __global__ __launch_bounds__(256) void swiglu8_backward_kernel(const T *__restri
             for (int j = 0; j < n; ++j) {
                 const float a = from_steps(qa.v[j], ca), g = from_steps(qg.v[j], cg), d = to_f32(dy.v[j]);
                 const float s = logistic<T>(beta * a);
-                dg.v[j] = from_f32<T>(d * a * s);
-                da.v[j] = from_f32<T>(d * g * (s + beta * a * s * (1.0f - s)));
+                // The factors of d are finite where a and g are; d a and d g alone may overflow where s is 0.  Where beta a
+                // overflows, s is 0 or 1 and any finite value serves for it.
+                const float ba = fminf(fmaxf(beta * a, -FLT_MAX), FLT_MAX);
+                dg.v[j] = from_f32<T>(d * (a * s));
+                da.v[j] = from_f32<T>(d * (g * (s + ba * s * (1.0f - s))));
             }
             store_chunk(dX + r * 2 * D + c, da, here);
             store_chunk(dX + r * 2 * D + D + c, dg, here);

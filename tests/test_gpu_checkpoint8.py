@@ -230,3 +230,42 @@ def test_swiglu_gradient_against_differences():
         i = col % 45
         scale = dy[:, i].double().abs() * (1 + g[:, i].abs()) * (1 + a[:, i].abs())
         assert bool(((dx[:, col].double().cpu() - want).abs() <= scale * (h * h / 2 + 64 * 2.0 ** -24)).all()), col
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("beta", [1.0, 1e6, -1e6])
+def test_large_finite_values(dtype, beta):
+    """g a, dY g, dY a or beta a beyond fp32 where the output and the gradients are not.  One value per block, whose 8 bits
+    are off by 2^-8 and have gradients of their own.  Tolerance: s is off by 8 + |beta a| ulp, three products and
+    one rounding; where e^-beta a is below fp32's range, s is 0 instead of 2^-126 at most."""
+    OPMX = opmx()
+    cases = [(-1e25, 1e25, 1.0), (-3e38, -3e38, 1e30), (-1e20, 3.0, 1e30), (-60.0, 1e38, 1.0), (-20.0, 1e38, 0.5),
+             (3e38, 0.25, 0.25), (1e20, 1e18, 1.0), (0.5, 1e38, 1.0), (-200.0, 2e38, 1.0), (0.0, 2e38, 1.0), (1e34, 3.0, 0.5),
+             (-1e34, -3.0, 0.5), (1e-5, 1e38, 1.0), (-2e38, 0.0, 0.25)]
+    x = torch.tensor([c[:2] for c in cases], dtype=torch.float64).to(dtype)
+    dy = torch.tensor([c[2:] for c in cases], dtype=torch.float64).to(dtype)
+    xd = x.to(dev()).requires_grad_(True)
+    y = OPMX.swiglu_checkpoint8(xd, beta)
+    dx, = torch.autograd.grad(y, xd, dy.to(dev()))
+    b = torch.tensor(beta, dtype=torch.float32).double()
+    u, f, tiny = half_step(dtype), 2.0 ** -24, torch.finfo(dtype).smallest_normal
+    xa, xg = x.double().chunk(2, -1)
+    ref = O.swiglu(x, b)
+    own = lambda a: f * (12 + 2 * (b * a).abs().clamp(max=88.0))
+    gone = lambda a: torch.where(b * a < -87, 2.0 ** -126 * a.abs(), 0.0)
+    top = float(torch.finfo(dtype).max)
+    fits = ref.abs() < top                                       # (with another beta some are beyond the type)
+    assert int(fits.sum()) >= 9
+    assert_within(y.detach().cpu()[fits], ref[fits], ((own(xa) + u) * 1.01 * ref.abs() + gone(xa) * xg.abs() + tiny)[fits], "Y")
+    a, g = O.swiglu_held(x)
+    d = dy.double()
+    s, ns, ba = O.logistic(b * a), O.logistic(-b * a), (b * a).abs()
+    ref = O.swiglu_backward(a, g, dy, b)
+    terms = torch.cat([(d * g).abs() * (s + ba * s * ns) * own(a) + f * (d * g).abs() * ba.clamp(max=88.0) * s,
+                       (d * a).abs() * s * own(a)], -1)
+    # s next to 1: 1 - s has an ulp of 1 of its own, which ba multiplies while 1 - s is not 0 (ba < 17)
+    terms += torch.cat([f * (d * g).abs() * torch.where(ba < 17, ba, 0 * ba), 0 * d], -1)
+    lost = torch.cat([gone(a) * (1 + ba.clamp(max=104.0)) * (d * g).abs() / a.abs().clamp(min=1e-30), gone(a) * d.abs()], -1)
+    fits = ref.abs() < top
+    assert int(fits.sum()) >= 20
+    assert_within(dx.cpu()[fits], ref[fits], (ref.abs() * u * 1.01 + terms * 1.5 + lost + tiny)[fits], "dX")
