@@ -265,8 +265,9 @@ int opmx_moe_reduce(const void *Y, const void *expert_weights, const int64_t *in
 int opmx_checkpoint8_pack(const void *X, int64_t R, int64_t D, int dtype, int8_t *q, uint8_t *code, void *stream);
 int opmx_checkpoint8_unpack(const int8_t *q, const uint8_t *code, int64_t R, int64_t D, int dtype, void *X, void *stream);
 
-/* SwiGLU for training: opmx_swiglu and, in the same pass, its input in 8 bits; both halves of a row have their
- * own blocks: q [R,2,D], code [R,2,ceil(D/32)].  The backward pass takes the gradient at the held values a, g:
+/* SwiGLU for training: opmx_swiglu (the same bits, but finite also where g a alone is beyond fp32) and, in the same
+ * pass, its input in 8 bits; both halves of a row have their own blocks: q [R,2,D], code [R,2,ceil(D/32)] (both NULL:
+ * nothing is kept).  The backward pass takes the gradient at the held values a, g:
  *   dX[r, D+i] = dY a s(beta a),   dX[r, i] = dY g s(beta a) (1 + beta a (1 - s(beta a))).
  * X, dX [R,2D]; Y, dY [R,D] (dtype); fp32 arithmetic, one rounding. */
 int opmx_swiglu_checkpoint8(const void *X, int64_t R, int64_t D, float beta, int dtype, void *Y, int8_t *q, uint8_t *code,

@@ -376,7 +376,7 @@ int opmx_swiglu_checkpoint8(const void *X, int64_t R, int64_t D, float beta, int
     if (R < 0 || D < 0) return OPMX_ERR_BAD_ARGUMENT;
     if (!dtype_ok(dtype)) return OPMX_ERR_UNSUPPORTED;
     if (R == 0 || D == 0) return OPMX_OK;
-    if (!X || !Y || !q || !code) return OPMX_ERR_BAD_ARGUMENT;
+    if (!X || !Y || (q == nullptr) != (code == nullptr)) return OPMX_ERR_BAD_ARGUMENT;
     return launch_swiglu_checkpoint8(X, R, D, beta, dtype, Y, q, code, st(stream));
 }
 

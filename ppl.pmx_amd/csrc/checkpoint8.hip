@@ -49,6 +49,16 @@ template <typename T> __device__ __forceinline__ void store_chunk(T *p, const Ch
     }
 }
 
+// The same chunk, of which the compiler knows nothing: what a rare branch works out of it is not held in registers before.
+template <typename T> __device__ __forceinline__ Chunk<T> anew(Chunk<T> c)
+{
+    quad q;
+    __builtin_memcpy(&q, &c, 16);
+    asm volatile("" : "+v"(q));
+    __builtin_memcpy(&c, &q, 16);
+    return c;
+}
+
 // n bytes (8 or 4) at an address of any alignment.
 template <int n> struct Bytes {
     signed char v[n];
@@ -142,7 +152,29 @@ template <typename T> __device__ __forceinline__ float logistic(float x)
     else return sigmoidf_(x);
 }
 
-template <typename T>
+// The last product of the output, rounded as the plain operator does.  In float16 its form for whole 16-byte chunks rounds to fp32
+// first and then to the type, its other form once (a value in 16000 differs); which instruction the compiler takes here
+// would depend on what stands around it.
+template <typename T, bool CHUNKS> __device__ __forceinline__ T last_product(float a, float b)
+{
+    if constexpr (!std::is_same<T, f16>::value) {
+        return from_f32<T>(a * b);
+    } else if constexpr (CHUNKS) {
+        float p = a * b;
+        asm("" : "+v"(p));
+        return from_f32<T>(p);
+    } else {
+        uint32_t r;
+        asm("v_fma_mixlo_f16 %0, %1, %2, 0" : "=v"(r) : "v"(a), "v"(b));
+        const uint16_t low = static_cast<uint16_t>(r);
+        T v;
+        __builtin_memcpy(&v, &low, 2);
+        return v;
+    }
+}
+
+// KEEP: q and codes are wanted.  CHUNKS: the plain operator would take this call 16 bytes at a time.
+template <typename T, bool KEEP, bool CHUNKS>
 __global__ __launch_bounds__(256) void swiglu8_kernel(const T *__restrict__ X, int64_t R, int64_t D, int64_t blocks,
                                                       float beta, T *__restrict__ Y, int8_t *__restrict__ q,
                                                       uint8_t *__restrict__ codes)
@@ -154,18 +186,27 @@ __global__ __launch_bounds__(256) void swiglu8_kernel(const T *__restrict__ X, i
         const int64_t r = r0 + threadIdx.y, here = r < R ? left : 0;
         const Chunk<T> a = load_chunk(X + r * 2 * D + c, here), g = load_chunk(X + r * 2 * D + D + c, here);
         Chunk<T> y;
+        float most = 0.0f;
 #pragma unroll
         for (int j = 0; j < n; ++j) {
-            const float af = to_f32(a.v[j]);
-            const float gf = to_f32(g.v[j]), s = logistic<T>(beta * af), ga = gf * af;
-            float yf = ga * s;
-            // the plain operator's product, except where g a is beyond fp32 (which it cannot be in float16)
-            if constexpr (!std::is_same<T, f16>::value) yf = fabsf(ga) == INFINITY ? gf * (af * s) : yf;
-            y.v[j] = from_f32<T>(yf);
+            const float af = to_f32(a.v[j]), ga = to_f32(g.v[j]) * af;
+            most = fmaxf(most, fabsf(ga));
+            y.v[j] = last_product<T, CHUNKS>(ga, logistic<T>(beta * af));
+        }
+        // some g a is beyond fp32 (which it cannot be in float16): there a s first
+        if (!std::is_same<T, f16>::value && most == INFINITY) {
+            const Chunk<T> a2 = anew(a), g2 = anew(g);
+#pragma unroll
+            for (int j = 0; j < n; ++j) {
+                const float af = to_f32(a2.v[j]), gf = to_f32(g2.v[j]), s = logistic<T>(beta * af);
+                if (fabsf(gf * af) == INFINITY) y.v[j] = from_f32<T>(gf * (af * s));
+            }
         }
         store_chunk(Y + r * D + c, y, here);
-        pack_chunk(a, here, q + r * 2 * D + c, codes + r * 2 * blocks + c / kBlock8);
-        pack_chunk(g, here, q + r * 2 * D + D + c, codes + (r * 2 + 1) * blocks + c / kBlock8);
+        if constexpr (KEEP) {
+            pack_chunk(a, here, q + r * 2 * D + c, codes + r * 2 * blocks + c / kBlock8);
+            pack_chunk(g, here, q + r * 2 * D + D + c, codes + (r * 2 + 1) * blocks + c / kBlock8);
+        }
     }
 }
 
@@ -191,7 +232,7 @@ __global__ __launch_bounds__(256) void swiglu8_backward_kernel(const T *__restri
                 const float s = logistic<T>(beta * a);
                 // The factors of d are finite where a and g are; d a and d g alone may overflow where s is 0.  Where beta a
                 // overflows, s is 0 or 1 and any finite value serves for it.
-                const float ba = fminf(fmaxf(beta * a, -FLT_MAX), FLT_MAX);
+                const float ba = __builtin_amdgcn_fmed3f(beta * a, -FLT_MAX, FLT_MAX);
                 dg.v[j] = from_f32<T>(d * (a * s));
                 da.v[j] = from_f32<T>(d * (g * (s + ba * s * (1.0f - s))));
             }
@@ -241,9 +282,19 @@ template <typename T>
 int swiglu8_impl(const void *X, int64_t R, int64_t D, float beta, void *Y, void *q, void *codes, hipStream_t s)
 {
     const Shape g = shape_for<T>(R, D);
-    swiglu8_kernel<T><<<g.grid, g.block, 0, s>>>(static_cast<const T *>(X), R, D, ceil_div(D, kBlock8), beta,
-                                                 static_cast<T *>(Y), static_cast<int8_t *>(q),
-                                                 static_cast<uint8_t *>(codes));
+    auto launch = [&](auto keep, auto chunks) {
+        swiglu8_kernel<T, decltype(keep)::value, decltype(chunks)::value><<<g.grid, g.block, 0, s>>>(
+            static_cast<const T *>(X), R, D, ceil_div(D, kBlock8), beta, static_cast<T *>(Y), static_cast<int8_t *>(q),
+            static_cast<uint8_t *>(codes));
+    };
+    bool chunks = false;
+    if constexpr (std::is_same<T, f16>::value) {
+        chunks = D % Chunk<T>::n == 0 && aligned16(X) && aligned16(Y);
+        if (chunks && q) launch(std::true_type{}, std::true_type{});
+        else if (chunks) launch(std::false_type{}, std::true_type{});
+    }
+    if (!chunks && q) launch(std::true_type{}, std::false_type{});
+    else if (!chunks) launch(std::false_type{}, std::false_type{});
     OPMX_LAUNCH_CHECK();
     return OPMX_OK;
 }

@@ -65,27 +65,25 @@ def _rows(lead):
 
 class SwiGLUCheckpoint8(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, X, beta):
+    def forward(ctx, X, beta, train):
         dev = _lib.require_gpu("swiglu_checkpoint8", X)
         if X.dim() == 0 or X.shape[-1] % 2:
             raise ValueError("swiglu_checkpoint8: last dimension must be even")
         dt = _lib.dtype_id(X, "swiglu_checkpoint8")
         lead, D = tuple(X.shape[:-1]), X.shape[-1] // 2
         R = _rows(lead)
-        L = _lib.lib()
+        # (ctx.needs_input_grad tells what X asks for, also where nothing is recorded)
+        keep = train and ctx.needs_input_grad[0]
         with _lib.on_device(dev):
             Xc = X.detach().contiguous()
             Y = torch.empty(*lead, D, dtype=X.dtype, device=dev)
-            if ctx.needs_input_grad[0]:
-                q = torch.empty(R, 2, D, dtype=torch.int8, device=dev)
-                code = torch.empty(R, 2, _blocks(D), dtype=torch.uint8, device=dev)
-                _lib.check(L.opmx_swiglu_checkpoint8(_lib.ptr(Xc), R, D, float(beta), dt, _lib.ptr(Y), _lib.ptr(q),
-                                                     _lib.ptr(code), _lib.stream_ptr(dev)), "swiglu_checkpoint8")
-                ctx.save_for_backward(q, code)
-                ctx.beta, ctx.dtype, ctx.shape = float(beta), X.dtype, tuple(X.shape)
-            else:
-                _lib.check(L.opmx_swiglu(_lib.ptr(Xc), R, D, float(beta), dt, _lib.ptr(Y), _lib.stream_ptr(dev)),
-                           "swiglu_checkpoint8")
+            q = torch.empty(R, 2, D, dtype=torch.int8, device=dev) if keep else None
+            code = torch.empty(R, 2, _blocks(D), dtype=torch.uint8, device=dev) if keep else None
+            _lib.check(_lib.lib().opmx_swiglu_checkpoint8(_lib.ptr(Xc), R, D, float(beta), dt, _lib.ptr(Y), _lib.ptr(q),
+                                                          _lib.ptr(code), _lib.stream_ptr(dev)), "swiglu_checkpoint8")
+        if keep:
+            ctx.save_for_backward(q, code)
+            ctx.beta, ctx.dtype, ctx.shape = float(beta), X.dtype, tuple(X.shape)
         return Y
 
     @staticmethod
@@ -99,10 +97,11 @@ class SwiGLUCheckpoint8(torch.autograd.Function):
             _lib.check(_lib.lib().opmx_swiglu_checkpoint8_backward(
                 _lib.ptr(dYc), _lib.ptr(q), _lib.ptr(code), q.shape[0], D, ctx.beta,
                 _lib.dtype_id(dX, "swiglu_checkpoint8"), _lib.ptr(dX), _lib.stream_ptr(dev)), "swiglu_checkpoint8")
-        return dX, None
+        return dX, None, None
 
 
 def swiglu_checkpoint8(X: torch.Tensor, beta: float = 1.0):
-    """``swiglu`` for training: the same output (in float16 a value halfway between two may round the other way), and
-    the gradient of X taken at X as 8 bits hold it.  Where no gradient is asked for, it is ``swiglu``, and nothing is kept.  X may be changed in place afterwards: only its 8-bit form is used."""
-    return SwiGLUCheckpoint8.apply(X, beta)
+    """``swiglu`` for training: the same output (and finite also where the product of the halves alone is beyond fp32, which
+    ``swiglu`` makes an infinity or a NaN), and the gradient of X taken at X as 8 bits hold it.  Where no gradient is asked for, or
+    under ``torch.no_grad``, nothing is kept.  X may be changed in place afterwards: only its 8-bit form is used."""
+    return SwiGLUCheckpoint8.apply(X, beta, torch.is_grad_enabled())

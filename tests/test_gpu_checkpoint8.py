@@ -269,3 +269,24 @@ def test_large_finite_values(dtype, beta):
     fits = ref.abs() < top
     assert int(fits.sum()) >= 20
     assert_within(dx.cpu()[fits], ref[fits], (ref.abs() * u * 1.01 + terms * 1.5 + lost + tiny)[fits], "dX")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("R,D", [(2048, 2816), (1500, 1411)])
+def test_nothing_is_kept_without_gradients(dtype, R, D):
+    """Under no_grad, and for an input that asks for no gradient: the plain operator's output bit for bit, as in training,
+    and no memory beside it (the 8 bits would be 4 MB and more)."""
+    OPMX = opmx()
+    x = rows(R, 2 * D, dtype, 6).to(dev())
+    leaf = x.clone().requires_grad_(True)
+    want = OPMX.swiglu(x, 1.25)
+    assert torch.equal(OPMX.swiglu_checkpoint8(leaf, 1.25), want)
+    for grads, arg in ((False, leaf), (False, x), (True, x)):
+        with torch.set_grad_enabled(grads):
+            torch.cuda.synchronize()
+            torch.cuda.reset_peak_memory_stats()
+            before = torch.cuda.memory_allocated()
+            y = OPMX.swiglu_checkpoint8(arg, 1.25)
+            assert torch.cuda.max_memory_allocated() - before <= want.numel() * want.element_size() + (1 << 21)  # (whole blocks)
+        assert not y.requires_grad and torch.equal(y, want)
+        del y

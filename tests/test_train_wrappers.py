@@ -151,3 +151,10 @@ def test_package_refusals():
     g, = torch.autograd.grad(y, leaf, torch.ones_like(y).requires_grad_(True), create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         g.sum().backward()
+
+
+def test_swiglu_checkpoint8_keeps_both_or_nothing():
+    L = _lib.lib()
+    assert L.opmx_swiglu_checkpoint8(ONE, 4, 8, 1.0, 1, ONE, ONE, None, None) == -1
+    assert L.opmx_swiglu_checkpoint8(ONE, 4, 8, 1.0, 1, ONE, None, ONE, None) == -1
+    assert L.opmx_swiglu_checkpoint8(ONE, 0, 8, 1.0, 1, ONE, None, None, None) == 0
