@@ -308,7 +308,7 @@ int opmx_linear_epilogue_backward(const void *dY, const void *X, const int8_t *x
  * workspace: opmx_moe_balance_loss_workspace_bytes(), 16-byte aligned, not shared with a call running at the same time
  * (may be NULL where that says 256: nothing is needed).
  * backward, f held constant:  dscores[t,e] = dloss p[t,e] (w_e - sum_j w_j p[t,j]), 0 for tokens that do not
- * count; dloss: one float on the device.  E and k limits are those of opmx_moe_select. */
+ * count; dloss: one float on the device.  E and k limits are those of opmx_moe_select; T k < 2^31. */
 size_t opmx_moe_balance_loss_workspace_bytes(int64_t T, int E);
 int opmx_moe_balance_loss(const void *scores, const uint8_t *token_mask, int64_t T, int E, int k, int dtype, float *loss,
                           int64_t *expert_count, float *weight, void *workspace, size_t workspace_bytes, void *stream);

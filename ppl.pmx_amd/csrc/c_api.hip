@@ -466,7 +466,7 @@ int opmx_moe_balance_loss(const void *scores, const uint8_t *token_mask, int64_t
 {
     if (T < 0 || E <= 0 || k <= 0 || k > E) return OPMX_ERR_BAD_ARGUMENT;
     if (!dtype_ok(dtype) || E > OPMX_MOE_MAX_EXPERTS || k > OPMX_MOE_MAX_EXPERTS_PER_TOKEN) return OPMX_ERR_UNSUPPORTED;
-    if (T > (int64_t{1} << 31) / k) return OPMX_ERR_UNSUPPORTED;
+    if (T > ((int64_t{1} << 31) - 1) / k) return OPMX_ERR_UNSUPPORTED;        // counts of tokens are 32 bits on the way
     if (!loss || !expert_count || !weight || (T > 0 && !scores)) return OPMX_ERR_BAD_ARGUMENT;
     const size_t need = moe_balance_loss_workspace_bytes(T, E);
     if (need > 256 && (!workspace || workspace_bytes < need)) return OPMX_ERR_WORKSPACE;

@@ -158,3 +158,13 @@ def test_swiglu_checkpoint8_keeps_both_or_nothing():
     assert L.opmx_swiglu_checkpoint8(ONE, 4, 8, 1.0, 1, ONE, ONE, None, None) == -1
     assert L.opmx_swiglu_checkpoint8(ONE, 4, 8, 1.0, 1, ONE, None, ONE, None) == -1
     assert L.opmx_swiglu_checkpoint8(ONE, 0, 8, 1.0, 1, ONE, None, None, None) == 0
+
+
+def test_balance_loss_refuses_counts_past_32_bits():
+    """2^31 tokens in all would be -2^31 in the sums on the way."""
+    L = _lib.lib()
+    T = 1 << 31
+    for k, first in ((1, T), (2, T // 2), (8, T // 8), (7, T // 7 + 1)):
+        need = L.opmx_moe_balance_loss_workspace_bytes(first, 8)
+        assert L.opmx_moe_balance_loss(ONE, None, first, 8, k, 1, ONE, ONE, ONE, ONE, need, None) == -2
+        assert L.opmx_moe_balance_loss(ONE, None, first - 1, 8, k, 1, ONE, ONE, ONE, ONE, need - 1, None) == -3
