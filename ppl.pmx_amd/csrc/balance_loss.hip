@@ -15,13 +15,15 @@
 // 7 for the blocks' sums, backward 44 us, 6.1 TB/s.
 // An expert is picked where its key is not below the k-th; keys of 16-bit scores hold the id too and are
 // distinct, equal fp32 scores at the k-th place are settled by id in a branch few waves take.
-// Sums: fp32 in a lane (a few dozen tokens), 64 bits across blocks, in a fixed order: results do not vary.
+// Sums of p: fp32 over up to kFold tokens of a lane and over the lanes of the block, 64 bits beyond, in a fixed order: results
+// do not vary, and what a sum is off by does not grow with the number of tokens.
 #include "common.h"
 
 namespace opmx {
 namespace {
 
 constexpr int kMaxBlocks = 256;
+constexpr int kFold = 64;       // tokens of a lane whose p are added in fp32
 __host__ __device__ inline int pitch_of(int E) { return (E + 3) / 4 * 4; }      // of a block's sums
 
 // A key orders scores as MoeSelect does: NaN first, -0 equal to +0.  No key is 0 or 2^32 - 1.
@@ -243,98 +245,107 @@ __global__ __launch_bounds__(THREADS) void balance_kernel(const T *__restrict__ 
         cnt[i] = 0;
     }
     int32_t kept = 0;
-    for (int64_t t0 = static_cast<int64_t>(blockIdx.x) * per_block; t0 < Ttok;
-         t0 += static_cast<int64_t>(gridDim.x) * per_block) {
-        const int64_t t = t0 + threadIdx.x / L;
-        const bool keep = t < Ttok && (mask == nullptr || mask[t] != 0);     // the same in the token's L lanes
-        const T *row = scores + (t < Ttok ? t : Ttok - 1) * E;
-        float z[V];
-        uint32_t key[V];
-        load_scores<T, N, V, L, true>(row, E, lane, keep, z, key);
-        uint32_t list[KL];
+    int64_t t0 = static_cast<int64_t>(blockIdx.x) * per_block;
+    const int e = threadIdx.x;
+    double p = 0.0;                              // of expert e, of the block
+    int32_t c = 0, n = 0;
+    while (true) {
+        for (int trip = 0; trip < kFold && t0 < Ttok; ++trip, t0 += static_cast<int64_t>(gridDim.x) * per_block) {
+            const int64_t t = t0 + threadIdx.x / L;
+            const bool keep = t < Ttok && (mask == nullptr || mask[t] != 0);     // the same in the token's L lanes
+            const T *row = scores + (t < Ttok ? t : Ttok - 1) * E;
+            float z[V];
+            uint32_t key[V];
+            load_scores<T, N, V, L, true>(row, E, lane, keep, z, key);
+            uint32_t list[KL];
 #pragma unroll
-        for (int j = 0; j < KL; ++j) list[j] = 0u;
+            for (int j = 0; j < KL; ++j) list[j] = 0u;
 #pragma unroll
-        for (int i = 0; i < V; ++i) insert<KL>(list, key[i]);
+            for (int i = 0; i < V; ++i) insert<KL>(list, key[i]);
 #define OPMX_MERGE(D) merge<KL, D>(list)
-        OPMX_HALVES(OPMX_MERGE);
-        const uint32_t kth = keep ? at<KL>(list, k - 1) : 0xFFFFFFFFu;       // no key of a token that does not count reaches it
-        bool tied = false;
-        if constexpr (!Key<T>::unique) {
-            int picked = 0;
+            OPMX_HALVES(OPMX_MERGE);
+            const uint32_t kth = keep ? at<KL>(list, k - 1) : 0xFFFFFFFFu;       // no key of a token that does not count reaches it
+            bool tied = false;
+            if constexpr (!Key<T>::unique) {
+                int picked = 0;
 #pragma unroll
-            for (int i = 0; i < V; ++i) picked += key[i] >= kth ? 1 : 0;
+                for (int i = 0; i < V; ++i) picked += key[i] >= kth ? 1 : 0;
 #define OPMX_PICKED(D) picked += other_half<D>(picked)
-            OPMX_HALVES(OPMX_PICKED);
-            tied = picked > k;               // more equal ones at the k-th place than are to be picked
-        }
-        if (!__any(tied)) {
+                OPMX_HALVES(OPMX_PICKED);
+                tied = picked > k;               // more equal ones at the k-th place than are to be picked
+            }
+            if (!__any(tied)) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) cnt[i] += key[i] >= kth ? 1 : 0;
-        } else {
-            int above = 0;
+                for (int i = 0; i < V; ++i) cnt[i] += key[i] >= kth ? 1 : 0;
+            } else {
+                int above = 0;
 #pragma unroll
-            for (int i = 0; i < V; ++i) above += key[i] > kth ? 1 : 0;
+                for (int i = 0; i < V; ++i) above += key[i] > kth ? 1 : 0;
 #define OPMX_ABOVE(D) above += other_half<D>(above)
-            OPMX_HALVES(OPMX_ABOVE);
-            const int left = k - above;      // so many of the equal ones are picked, the lowest ids first
-            // ids go up chunk by chunk, and within a chunk lane by lane
-            int before = 0;                  // equal ones in the chunks behind us
+                OPMX_HALVES(OPMX_ABOVE);
+                const int left = k - above;      // so many of the equal ones are picked, the lowest ids first
+                // ids go up chunk by chunk, and within a chunk lane by lane
+                int before = 0;                  // equal ones in the chunks behind us
 #pragma unroll
-            for (int c = 0; c < V / N; ++c) {
-                int mine = 0;
+                for (int c = 0; c < V / N; ++c) {
+                    int mine = 0;
 #pragma unroll
-                for (int j = 0; j < N; ++j) mine += key[c * N + j] == kth ? 1 : 0;
-                int upto = mine, all = mine;
+                    for (int j = 0; j < N; ++j) mine += key[c * N + j] == kth ? 1 : 0;
+                    int upto = mine, all = mine;
 #define OPMX_PREFIX(D) upto += lanes_before<D, L>(upto, lane), all += other_half<D>(all)
-                OPMX_HALVES(OPMX_PREFIX);
-                int rank = before + upto - mine;
+                    OPMX_HALVES(OPMX_PREFIX);
+                    int rank = before + upto - mine;
 #pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    const uint32_t q = key[c * N + j];
-                    cnt[c * N + j] += q > kth || (q == kth && rank < left) ? 1 : 0;
-                    rank += q == kth ? 1 : 0;
+                    for (int j = 0; j < N; ++j) {
+                        const uint32_t q = key[c * N + j];
+                        cnt[c * N + j] += q > kth || (q == kth && rank < left) ? 1 : 0;
+                        rank += q == kth ? 1 : 0;
+                    }
+                    before += all;
                 }
-                before += all;
+            }
+            const float scale = exp_<V, L>(z);
+#pragma unroll
+            for (int i = 0; i < V; ++i) psum[i] = fmaf(z[i], scale, psum[i]);
+            kept += keep && lane == 0 ? 1 : 0;
+        }
+        // over the tokens of the wave, then of the block
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const float ps = sum_mod<L>(psum[i]);
+            const int32_t cs = sum_mod<L>(cnt[i]);
+            psum[i] = 0.0f;
+            cnt[i] = 0;
+            const int id = expert_of<N, L>(i, lane);
+            if (lane_id() < L && id < E) {
+                s_p[wave][id] = ps;
+                s_c[wave][id] = cs;
             }
         }
-        const float scale = exp_<V, L>(z);
+        kept = sum_mod<1>(kept);
+        if (lane_id() == 0) s_n[wave] = kept;
+        kept = 0;
+        __syncthreads();
+        if (e < E) {
+            float part = 0.0f;
 #pragma unroll
-        for (int i = 0; i < V; ++i) psum[i] = fmaf(z[i], scale, psum[i]);
-        kept += keep && lane == 0 ? 1 : 0;
-    }
-    // over the tokens of the wave, then of the block
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        psum[i] = sum_mod<L>(psum[i]);
-        cnt[i] = sum_mod<L>(cnt[i]);
-        const int e = expert_of<N, L>(i, lane);
-        if (lane_id() < L && e < E) {
-            s_p[wave][e] = psum[i];
-            s_c[wave][e] = cnt[i];
+            for (int v = 0; v < WAVES; ++v) {
+                part += s_p[v][e];
+                c += s_c[v][e];
+            }
+            p += part;
         }
-    }
-    kept = sum_mod<1>(kept);
-    if (lane_id() == 0) s_n[wave] = kept;
-    __syncthreads();
-    const int e = threadIdx.x;
-    float p = 0.0f;
-    int32_t c = 0, n = 0;
-    if (e < E) {
 #pragma unroll
-        for (int v = 0; v < WAVES; ++v) {
-            p += s_p[v][e];
-            c += s_c[v][e];
-        }
+        for (int v = 0; v < WAVES; ++v) n += s_n[v];
+        if (t0 >= Ttok) break;
+        __syncthreads();                         // before they are written again
     }
-#pragma unroll
-    for (int v = 0; v < WAVES; ++v) n += s_n[v];
     if (gridDim.x == 1) {
         finish<THREADS>(p, c, n, e, E, k, s_red, loss, counts, w);
         return;
     }
     if (e < pitch_of(E)) {                   // (p and c are 0 past E)
-        part_p[blockIdx.x * pitch_of(E) + e] = p;
+        part_p[blockIdx.x * pitch_of(E) + e] = static_cast<float>(p);
         part_c[blockIdx.x * pitch_of(E) + e] = c;
     }
     if (e == 0) part_n[blockIdx.x] = n;

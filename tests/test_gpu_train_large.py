@@ -97,3 +97,19 @@ def test_balance_loss_with_more_than_2_31_scores():
         dr = p * (w - (p * w).sum())
         tol = 2.0 ** -8 * 1.01 * dr.abs() + 128 * 2.0 ** -24 * p * (w + (p * w).sum())
         assert bool(((ds[r].double() - dr).abs() <= tol).all())
+
+
+def test_long_sums_of_the_balance_loss_stay_exact():
+    """8388608 tokens with k > 8, all with the same scores: 4096 of them in one lane, whose p = 0.0317 is a number that
+    rounds the same way at every addition (4096 of them in a row in fp32 are 1015 2^-24 off).  Tolerance: p is off by 64 2^-24;
+    64 additions at most are in fp32 in a row (1/2 2^-24 each) and the sums of the lanes and blocks are rounded once each."""
+    OPMX = opmx()
+    T, E, k = 1 << 23, 65, 9
+    row = torch.zeros(E)
+    row[1:64:7] = 0.912
+    assert int((row > 0).sum()) == k
+    s = row.to(dev()).expand(T, E).contiguous()
+    loss, count = OPMX.moe_balance_loss(s, E, k)
+    assert torch.equal(count.cpu(), T * (row > 0).long())
+    want = E * float(torch.softmax(row.double(), 0)[row > 0].sum()) / k
+    assert abs(float(loss) - want) <= (64 + 32 + 4) * 2.0 ** -24 * want
