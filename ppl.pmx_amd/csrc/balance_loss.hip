@@ -475,6 +475,8 @@ __global__ __launch_bounds__(256) void balance_backward_kernel(const T *__restri
 // one block per CU are all that the second launch has to add.  L is a constant of the kernels, whose code
 // then has no branches.
 constexpr int kFewExperts = 64, kFewThreads = 256, kManyThreads = 1024;
+constexpr int kFewPicks = 8, kPickThreads = 512;     // more picks: lists of 32 keys leave registers for 8 scores and 8 waves
+constexpr int kPickLanesFew = 8, kPickLanesMany = 32;
 inline int lanes_few(int E) { return E <= 8 ? 1 : E <= 16 ? 2 : E <= 32 ? 4 : 8; }
 inline int lanes_many(int E) { return E <= 128 ? 8 : 16; }
 
@@ -496,9 +498,9 @@ template <typename T, int N, int V, int L, int KL, int THREADS> void forward_lau
 }
 template <typename T, int N> void forward_sums(const Forward &f, hipStream_t s)
 {
-    if (f.k > 8) {                  // lists of 32 keys leave registers for 8 scores only
-        if (f.E <= 64) forward_launch<T, N, 8, 8, 32, 256>(f, s);
-        else forward_launch<T, N, 8, 32, 32, 256>(f, s);
+    if (f.k > kFewPicks) {
+        if (f.E <= kFewExperts) forward_launch<T, N, 8, kPickLanesFew, 32, kPickThreads>(f, s);
+        else forward_launch<T, N, 8, kPickLanesMany, 32, kPickThreads>(f, s);
     } else if (f.E <= kFewExperts) {
         switch (lanes_few(f.E)) {
             case 1: forward_launch<T, N, 8, 1, 8, kFewThreads>(f, s); break;
@@ -513,12 +515,16 @@ template <typename T, int N> void forward_sums(const Forward &f, hipStream_t s)
     }
 }
 
-// One block serves a decoding batch in one launch; beyond that at most one block per CU and a second launch.
-inline int blocks_for(int64_t Ttok, int E)
+// One block serves a decoding batch in one launch; beyond that at most one block per CU and a second launch.  With more
+// picks a block holds fewer tokens at a time, and so there are more of them (4096 tokens, 100 experts, k = 9, fp32: 13 us; as many
+// blocks as for few picks 52); for the tokens of a single block it takes up to 8 trips (64 tokens, 256 experts, k = 32: 22 us).
+inline int blocks_for(int64_t Ttok, int E, int k)
 {
     const bool few = E <= kFewExperts;
-    const int64_t b = ceil_div(Ttok, few ? kFewThreads / lanes_few(E) : kManyThreads / lanes_many(E));
-    return static_cast<int>(b <= 1 ? 1 : (b < kMaxBlocks ? b : kMaxBlocks));
+    const int64_t one = few ? kFewThreads / lanes_few(E) : kManyThreads / lanes_many(E);        // tokens of a block
+    if (Ttok <= one) return 1;
+    const int64_t b = ceil_div(Ttok, k <= kFewPicks ? one : kPickThreads / (few ? kPickLanesFew : kPickLanesMany));
+    return static_cast<int>(b < kMaxBlocks ? b : kMaxBlocks);
 }
 
 template <typename T>
@@ -526,7 +532,7 @@ int forward_impl(const void *scores, const void *mask, int64_t Ttok, int E, int 
                  float *w, hipStream_t s)
 {
     constexpr int n = Vec16<T>::n;
-    Forward f{scores, mask, Ttok, E, k, blocks_for(Ttok, E), static_cast<float *>(ws), nullptr, nullptr, loss, counts, w};
+    Forward f{scores, mask, Ttok, E, k, blocks_for(Ttok, E, k), static_cast<float *>(ws), nullptr, nullptr, loss, counts, w};
     f.pc = reinterpret_cast<int32_t *>(f.pp + f.blocks * pitch_of(E));
     f.pn = f.pc + f.blocks * pitch_of(E);
     if (E % n == 0 && aligned16(scores)) forward_sums<T, n>(f, s);
@@ -585,7 +591,7 @@ int backward_impl(const void *scores, const void *mask, const float *w, const fl
 size_t moe_balance_loss_workspace_bytes(int64_t Ttok, int E)
 {
     if (Ttok <= 0 || E <= 0 || E > OPMX_MOE_MAX_EXPERTS) return 256;
-    const int blocks = blocks_for(Ttok, E);
+    const int few = blocks_for(Ttok, E, kFewPicks), many = blocks_for(Ttok, E, kFewPicks + 1), blocks = few > many ? few : many;
     if (blocks == 1) return 256;             // finishes by itself
     const size_t b = static_cast<size_t>(blocks) * (static_cast<size_t>(pitch_of(E)) * 8 + 4);
     return (b + 255) / 256 * 256 + 256;

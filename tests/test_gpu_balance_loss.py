@@ -210,3 +210,11 @@ def test_no_gradient_where_every_expert_is_picked(E):
     g, = torch.autograd.grad(loss, s)
     assert bool((count == 500).all())
     assert float(g.abs().max()) <= 2 * (64 * 2.0 ** -24) ** 2 / 500
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,E,k", [(64, 256, 32), (65, 256, 32), (129, 128, 9), (4096, 100, 9), (4500, 251, 17), (33, 64, 12),
+                                   (64, 64, 12), (700, 40, 10), (9000, 9, 9), (5000, 16, 16)])
+def test_many_picks_from_one_block_to_all(dtype, T, E, k):
+    check(logits(T, E, dtype, T + k), k, dloss=2.0)
+    check(tie_heavy_scores(T, E, dtype, 7), k, mask=torch.arange(T) % 5 != 1)

@@ -168,3 +168,12 @@ def test_balance_loss_refuses_counts_past_32_bits():
         need = L.opmx_moe_balance_loss_workspace_bytes(first, 8)
         assert L.opmx_moe_balance_loss(ONE, None, first, 8, k, 1, ONE, ONE, ONE, ONE, need, None) == -2
         assert L.opmx_moe_balance_loss(ONE, None, first - 1, 8, k, 1, ONE, ONE, ONE, ONE, need - 1, None) == -3
+
+
+def test_balance_loss_workspace_holds_every_block():
+    """A block's sums are 8 bytes an expert (rows of four) and 4; more than 8 picks take 16 tokens a block at a time (64 up to 64
+    experts), so that 4096 tokens of 100 experts fill 256 blocks."""
+    L = _lib.lib()
+    for T, E, blocks in ((4096, 100, 256), (200, 100, 13), (1 << 20, 256, 256), (4096, 16, 64), (8192, 64, 256)):
+        assert L.opmx_moe_balance_loss_workspace_bytes(T, E) >= blocks * ((E + 3) // 4 * 32 + 4)
+    assert L.opmx_moe_balance_loss_workspace_bytes(64, 256) == 256 == L.opmx_moe_balance_loss_workspace_bytes(32, 8)
