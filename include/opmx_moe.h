@@ -74,6 +74,14 @@ typedef enum opmx_activation {
     OPMX_ACTIVATION_SWIGLU = 4      /* h[D+i] h[i] s(h[i]), D = N/2: Y is [T, N/2] */
 } opmx_activation;
 
+/* What a call of opmx_linear_epilogue_gradients is asked for, for the size of its workspace. */
+typedef enum opmx_linear_gradient {
+    OPMX_LINEAR_DX = 1,
+    OPMX_LINEAR_DW = 2,
+    OPMX_LINEAR_DB = 4,
+    OPMX_LINEAR_X8 = 8              /* X comes in its 8-bit form */
+} opmx_linear_gradient;
+
 /* Limits of the routing kernels. */
 #define OPMX_MOE_MAX_EXPERTS 256
 #define OPMX_MOE_MAX_EXPERTS_PER_TOKEN 32
@@ -281,19 +289,24 @@ int opmx_swiglu_checkpoint8_backward(const void *dY, const int8_t *q, const uint
  * X [T,K], W [N,K], B [N] or NULL, R (residual) [T,M] or NULL, Y [T,M]; M = N, or N/2 with OPMX_ACTIVATION_SWIGLU.
  * H: NULL, or opmx_linear_epilogue_kept_bytes() bytes, 16-byte aligned, that receive H for the backward pass: in float32 as
  * it is, otherwise 24 bits of it (4 or 3 bytes per value; the layout is the library's).
- * backward: from dY [T,M]
+ * gradients: from dY [T,M]
  *   dH = dY * act'(H) (rounded to dtype),  dX = dH W [T,K],  dW = dH^T X [N,K],  dB = sum_t dH [N] (summed unrounded)
  * each of dX, dW, dB may be NULL (not wanted).  dX needs W; dW needs X, or its 8-bit form x_q, x_code (see
  * opmx_checkpoint8_pack; then X is ignored); every activation but NONE needs H.  The gradient of R is dY.
  * X, W, dY start at multiples of 16 bytes where K (dY: N, without an activation) is a multiple of 16 bytes
  * (OPMX_ERR_ALIGNMENT otherwise), the others anywhere their type allows.
- * workspace: opmx_linear_epilogue[_backward]_workspace_bytes(), 256-byte aligned, contents arbitrary, not shared with
- * a call running at the same time (may be NULL where that says 256: nothing is needed).  Results do not vary from call to
- * call.  K, N < 2^21, T < 2^31. */
+ * workspace: opmx_linear_epilogue_workspace_bytes(), opmx_linear_epilogue_gradients_workspace_bytes() of what is asked for (the
+ * opmx_linear_gradient values added up), 256-byte aligned, contents arbitrary, not shared with a call running at the same
+ * time (may be NULL where that says 256: nothing is needed).  opmx_linear_epilogue_backward is the same with a workspace that
+ * holds whatever may be asked for.  Results do not vary from call to call.  K, N < 2^21, T < 2^31. */
 size_t opmx_linear_epilogue_kept_bytes(int64_t T, int64_t N, int dtype);
 size_t opmx_linear_epilogue_workspace_bytes(int64_t T, int64_t K, int64_t N, int dtype, int activation);
 int opmx_linear_epilogue(const void *X, const void *W, const void *B, const void *R, int64_t T, int64_t K, int64_t N,
                          int dtype, int activation, void *Y, void *H, void *workspace, size_t workspace_bytes, void *stream);
+size_t opmx_linear_epilogue_gradients_workspace_bytes(int64_t T, int64_t K, int64_t N, int dtype, int activation, int wanted);
+int opmx_linear_epilogue_gradients(const void *dY, const void *X, const int8_t *x_q, const uint8_t *x_code, const void *W,
+                                   const void *H, int64_t T, int64_t K, int64_t N, int dtype, int activation, void *dX,
+                                   void *dW, void *dB, void *workspace, size_t workspace_bytes, void *stream);
 size_t opmx_linear_epilogue_backward_workspace_bytes(int64_t T, int64_t K, int64_t N, int dtype, int activation);
 int opmx_linear_epilogue_backward(const void *dY, const void *X, const int8_t *x_q, const uint8_t *x_code, const void *W,
                                   const void *H, int64_t T, int64_t K, int64_t N, int dtype, int activation, void *dX,

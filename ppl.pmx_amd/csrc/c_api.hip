@@ -426,15 +426,24 @@ int opmx_linear_epilogue(const void *X, const void *W, const void *B, const void
     return launch_linear_epilogue(X, W, B, R, T, K, N, dtype, activation, Y, H, workspace, st(stream));
 }
 
+constexpr int kAnyGradients = OPMX_LINEAR_DX | OPMX_LINEAR_DW | OPMX_LINEAR_DB | OPMX_LINEAR_X8;
+
 size_t opmx_linear_epilogue_backward_workspace_bytes(int64_t T, int64_t K, int64_t N, int dtype, int activation)
 {
     if (T < 0 || K <= 0 || N <= 0 || !dtype_ok(dtype) || !linear_sizes_ok(T, K, N)) return 256;
-    return linear_epilogue_backward_workspace_bytes(T, K, N, dtype, activation);
+    return linear_epilogue_backward_workspace_bytes(T, K, N, dtype, activation, kAnyGradients);
 }
 
-int opmx_linear_epilogue_backward(const void *dY, const void *X, const int8_t *x_q, const uint8_t *x_code, const void *W,
-                                  const void *H, int64_t T, int64_t K, int64_t N, int dtype, int activation, void *dX,
-                                  void *dW, void *dB, void *workspace, size_t workspace_bytes, void *stream)
+size_t opmx_linear_epilogue_gradients_workspace_bytes(int64_t T, int64_t K, int64_t N, int dtype, int activation, int wanted)
+{
+    if (T < 0 || K <= 0 || N <= 0 || !dtype_ok(dtype) || !linear_sizes_ok(T, K, N)) return 256;
+    return linear_epilogue_backward_workspace_bytes(T, K, N, dtype, activation, T > 0 ? wanted : wanted & ~OPMX_LINEAR_DX);
+}
+
+// whatever: the workspace has to hold whatever may be asked for, not only what is.
+static int linear_gradients(const void *dY, const void *X, const int8_t *x_q, const uint8_t *x_code, const void *W, const void *H,
+                            int64_t T, int64_t K, int64_t N, int dtype, int activation, void *dX, void *dW, void *dB,
+                            void *workspace, size_t workspace_bytes, void *stream, bool whatever)
 {
     if (T < 0 || K < 0 || N < 0 || activation < OPMX_ACTIVATION_NONE || activation > OPMX_ACTIVATION_SWIGLU)
         return OPMX_ERR_BAD_ARGUMENT;
@@ -451,12 +460,29 @@ int opmx_linear_epilogue_backward(const void *dY, const void *X, const int8_t *x
     if (K * size % 16 == 0 && ((dX && !aligned16(W)) || (dW && !x_q && !aligned16(X)))) return OPMX_ERR_ALIGNMENT;
     if (activation == OPMX_ACTIVATION_NONE && N * size % 16 == 0 && !aligned16(dY)) return OPMX_ERR_ALIGNMENT;
     if (H && !aligned16(H)) return OPMX_ERR_ALIGNMENT;
-    const size_t need = linear_epilogue_backward_workspace_bytes(T, K, N, dtype, activation);
+    if (T == 0) dX = nullptr;
+    const int wanted = (dX ? OPMX_LINEAR_DX : 0) | (dW ? OPMX_LINEAR_DW : 0) | (dB ? OPMX_LINEAR_DB : 0) | (x_q ? OPMX_LINEAR_X8 : 0);
+    const size_t need = linear_epilogue_backward_workspace_bytes(T, K, N, dtype, activation, whatever ? kAnyGradients : wanted);
     if (need > 256 && (!workspace || workspace_bytes < need)) return OPMX_ERR_WORKSPACE;
     if (workspace && (reinterpret_cast<uintptr_t>(workspace) & 255u)) return OPMX_ERR_ALIGNMENT;
-    if (T == 0) dX = nullptr;
-    return launch_linear_epilogue_backward(dY, X, x_q, x_code, W, H, T, K, N, dtype, activation, dX, dW, dB, workspace,
+    return launch_linear_epilogue_backward(dY, X, x_q, x_code, W, H, T, K, N, dtype, activation, dX, dW, dB, wanted, workspace,
                                            st(stream));
+}
+
+int opmx_linear_epilogue_gradients(const void *dY, const void *X, const int8_t *x_q, const uint8_t *x_code, const void *W,
+                                   const void *H, int64_t T, int64_t K, int64_t N, int dtype, int activation, void *dX,
+                                   void *dW, void *dB, void *workspace, size_t workspace_bytes, void *stream)
+{
+    return linear_gradients(dY, X, x_q, x_code, W, H, T, K, N, dtype, activation, dX, dW, dB, workspace, workspace_bytes, stream,
+                            false);
+}
+
+int opmx_linear_epilogue_backward(const void *dY, const void *X, const int8_t *x_q, const uint8_t *x_code, const void *W,
+                                  const void *H, int64_t T, int64_t K, int64_t N, int dtype, int activation, void *dX,
+                                  void *dW, void *dB, void *workspace, size_t workspace_bytes, void *stream)
+{
+    return linear_gradients(dY, X, x_q, x_code, W, H, T, K, N, dtype, activation, dX, dW, dB, workspace, workspace_bytes, stream,
+                            true);
 }
 
 size_t opmx_moe_balance_loss_workspace_bytes(int64_t T, int E) { return moe_balance_loss_workspace_bytes(T, E); }

@@ -151,12 +151,13 @@ int launch_swiglu_checkpoint8(const void *X, int64_t R, int64_t D, float beta, i
 int launch_swiglu_checkpoint8_backward(const void *dY, const void *q, const void *codes, int64_t R, int64_t D, float beta,
                                        int dtype, void *dX, hipStream_t s);
 size_t linear_epilogue_workspace_bytes(int64_t T, int64_t K, int64_t N, int dtype, int act);
-size_t linear_epilogue_backward_workspace_bytes(int64_t T, int64_t K, int64_t N, int dtype, int act);
+// wanted: opmx_linear_gradient
+size_t linear_epilogue_backward_workspace_bytes(int64_t T, int64_t K, int64_t N, int dtype, int act, int wanted);
 int launch_linear_epilogue(const void *X, const void *W, const void *B, const void *R, int64_t T, int64_t K, int64_t N,
                            int dtype, int act, void *Y, void *H, void *ws, hipStream_t s);
 int launch_linear_epilogue_backward(const void *dY, const void *X, const void *xq, const void *xcode, const void *W,
                                     const void *H, int64_t T, int64_t K, int64_t N, int dtype, int act, void *dX, void *dW,
-                                    void *dB, void *ws, hipStream_t s);
+                                    void *dB, int wanted, void *ws, hipStream_t s);
 size_t moe_balance_loss_workspace_bytes(int64_t T, int E);
 int launch_moe_balance_loss(const void *scores, const void *mask, int64_t T, int E, int k, int dtype, float *loss,
                             int64_t *counts, float *w, void *ws, hipStream_t s);

@@ -327,23 +327,27 @@ inline int64_t chunk_rows(int64_t Ttok, int64_t ncols)
 struct BackwardPlan {
     size_t dh, x, w, sums, part, total;
     int64_t pitch_n, pitch_k, chunk;
-    bool own_dh, padded;
+    bool own_dh, own_x, own_w;
 };
-BackwardPlan backward_plan(int64_t Ttok, int64_t K, int64_t N, int dtype, int act)
+// wanted: opmx_linear_gradient; only what these need has a place.
+BackwardPlan backward_plan(int64_t Ttok, int64_t K, int64_t N, int dtype, int act, int wanted)
 {
     const int64_t esize = dtype == OPMX_DTYPE_F32 ? 4 : 2, n = 16 / esize;
+    const bool dX = wanted & OPMX_LINEAR_DX, dW = wanted & OPMX_LINEAR_DW, padded = K % n != 0;
     BackwardPlan p{};
     p.pitch_n = up(N, n);
     p.pitch_k = up(K, n);
-    p.padded = K % n != 0;
-    p.own_dh = act != OPMX_ACTIVATION_NONE || N % n != 0;
+    p.own_dh = (act != OPMX_ACTIVATION_NONE || N % n != 0) && (dX || dW);
+    p.own_x = dW && (padded || (wanted & OPMX_LINEAR_X8));          // padded, or unpacked from 8 bits
+    p.own_w = dX && padded;
     p.chunk = chunk_rows(Ttok, act == OPMX_ACTIVATION_SWIGLU ? N / 2 : N);
     p.dh = 0;
     p.x = p.dh + (p.own_dh ? up(Ttok * p.pitch_n * esize, 256) : 0);
-    p.w = p.x + up(Ttok * p.pitch_k * esize, 256);          // padded, or unpacked from 8 bits
-    p.sums = p.w + (p.padded ? up(N * p.pitch_k * esize, 256) : 0);
-    p.part = p.sums + up(ceil_div(Ttok, p.chunk) * N * 4, 256);
-    const size_t a = cut_for(Ttok, K, N, false, true, false, dtype).bytes, b = cut_for(N, K, Ttok, false, true, true, dtype).bytes;
+    p.w = p.x + (p.own_x ? up(Ttok * p.pitch_k * esize, 256) : 0);
+    p.sums = p.w + (p.own_w ? up(N * p.pitch_k * esize, 256) : 0);
+    p.part = p.sums + (wanted & OPMX_LINEAR_DB ? up(ceil_div(Ttok, p.chunk) * N * 4, 256) : 0);
+    const size_t a = dX ? cut_for(Ttok, K, N, false, true, false, dtype).bytes : 0;
+    const size_t b = dW ? cut_for(N, K, Ttok, false, true, true, dtype).bytes : 0;
     p.total = p.part + up(a > b ? a : b, 256);
     return p;
 }
@@ -377,16 +381,15 @@ int forward_impl(const void *X, const void *W, const void *B, const void *R, int
 
 template <typename T>
 int backward_impl(const void *dY, const void *X, const void *xq, const void *xcode, const void *W, const void *H,
-                  int64_t Ttok, int64_t K, int64_t N, int act, void *dX, void *dW, void *dB, char *ws, hipStream_t s)
+                  int64_t Ttok, int64_t K, int64_t N, int act, void *dX, void *dW, void *dB, int wanted, char *ws, hipStream_t s)
 {
-    const BackwardPlan plan = backward_plan(Ttok, K, N, DType<T>::id, act);
+    const BackwardPlan plan = backward_plan(Ttok, K, N, DType<T>::id, act, wanted);
     const bool gated = act == OPMX_ACTIVATION_SWIGLU;
     const int64_t ncols = gated ? N / 2 : N;
     const void *dH = dY;
     int rc = OPMX_OK;
-    const bool want_dh = plan.own_dh && (dX || dW);
-    if (Ttok > 0 && (want_dh || dB)) {
-        T *out = want_dh ? reinterpret_cast<T *>(ws + plan.dh) : nullptr;
+    if (Ttok > 0 && (plan.own_dh || dB)) {
+        T *out = plan.own_dh ? reinterpret_cast<T *>(ws + plan.dh) : nullptr;
         float *sums = dB ? reinterpret_cast<float *>(ws + plan.sums) : nullptr;
         const dim3 grid(static_cast<unsigned>(ceil_div(ncols, kSlopeCols)), static_cast<unsigned>(ceil_div(Ttok, plan.chunk)));
         if (gated)
@@ -405,7 +408,7 @@ int backward_impl(const void *dY, const void *X, const void *xq, const void *xco
     }
     // W and X as the products take them
     int64_t pitch_w = K, pitch_x = K;
-    const bool pad_w = plan.padded && dX, pad_x = plan.padded && dW && !xq && Ttok > 0;
+    const bool pad_w = plan.own_w, pad_x = plan.own_x && !xq && Ttok > 0;
     if (pad_w && pad_x) rc = pad<T>(W, N, ws + plan.w, X, Ttok, ws + plan.x, K, s);
     else if (pad_w) rc = pad<T>(W, N, ws + plan.w, nullptr, 0, nullptr, K, s);
     else if (pad_x) rc = pad<T>(X, Ttok, ws + plan.x, nullptr, 0, nullptr, K, s);
@@ -438,15 +441,16 @@ int backward_impl(const void *dY, const void *X, const void *xq, const void *xco
 
 }  // namespace
 
+// 256 bytes say that none are needed, and that there may be no workspace: whatever is needed is more than that.
+static size_t bytes_for(size_t total) { return total == 0 ? 256 : total < 512 ? 512 : total; }
+
 size_t linear_epilogue_workspace_bytes(int64_t T, int64_t K, int64_t N, int dtype, int act)
 {
-    const size_t b = forward_plan(T, K, N, dtype, act).total;
-    return b > 256 ? b : 256;
+    return bytes_for(forward_plan(T, K, N, dtype, act).total);
 }
-size_t linear_epilogue_backward_workspace_bytes(int64_t T, int64_t K, int64_t N, int dtype, int act)
+size_t linear_epilogue_backward_workspace_bytes(int64_t T, int64_t K, int64_t N, int dtype, int act, int wanted)
 {
-    const size_t b = backward_plan(T, K, N, dtype, act).total;
-    return b > 256 ? b : 256;
+    return bytes_for(backward_plan(T, K, N, dtype, act, wanted).total);
 }
 
 int launch_linear_epilogue(const void *X, const void *W, const void *B, const void *R, int64_t T, int64_t K, int64_t N,
@@ -462,13 +466,13 @@ int launch_linear_epilogue(const void *X, const void *W, const void *B, const vo
 
 int launch_linear_epilogue_backward(const void *dY, const void *X, const void *xq, const void *xcode, const void *W,
                                     const void *H, int64_t T, int64_t K, int64_t N, int dtype, int act, void *dX, void *dW,
-                                    void *dB, void *ws, hipStream_t s)
+                                    void *dB, int wanted, void *ws, hipStream_t s)
 {
     char *w = static_cast<char *>(ws);
     switch (dtype) {
-        case OPMX_DTYPE_F32: return backward_impl<float>(dY, X, xq, xcode, W, H, T, K, N, act, dX, dW, dB, w, s);
-        case OPMX_DTYPE_F16: return backward_impl<f16>(dY, X, xq, xcode, W, H, T, K, N, act, dX, dW, dB, w, s);
-        case OPMX_DTYPE_BF16: return backward_impl<bf16>(dY, X, xq, xcode, W, H, T, K, N, act, dX, dW, dB, w, s);
+        case OPMX_DTYPE_F32: return backward_impl<float>(dY, X, xq, xcode, W, H, T, K, N, act, dX, dW, dB, wanted, w, s);
+        case OPMX_DTYPE_F16: return backward_impl<f16>(dY, X, xq, xcode, W, H, T, K, N, act, dX, dW, dB, wanted, w, s);
+        case OPMX_DTYPE_BF16: return backward_impl<bf16>(dY, X, xq, xcode, W, H, T, K, N, act, dX, dW, dB, wanted, w, s);
     }
     return OPMX_ERR_UNSUPPORTED;
 }

@@ -79,11 +79,13 @@ class LinearEpilogue(torch.autograd.Function):
             dX = torch.empty(xshape, dtype=dtype, device=dev) if need[0] else None
             dW = torch.empty(N, K, dtype=dtype, device=dev) if need[1] else None
             dB = torch.empty(N, dtype=dtype, device=dev) if need[2] else None
-            nbytes = L.opmx_linear_epilogue_backward_workspace_bytes(T, K, N, dt, act)
-            ws = _lib.workspace(nbytes, dev)
-            _lib.check(L.opmx_linear_epilogue_backward(
+            wanted = (_lib.LINEAR_DX * need[0] | _lib.LINEAR_DW * need[1] | _lib.LINEAR_DB * need[2]
+                      | _lib.LINEAR_X8 * (q is not None))
+            nbytes = L.opmx_linear_epilogue_gradients_workspace_bytes(T, K, N, dt, act, wanted)
+            ws = _lib.workspace(nbytes, dev) if nbytes > 256 else None
+            _lib.check(L.opmx_linear_epilogue_gradients(
                 _lib.ptr(dYc), _lib.ptr(X), _lib.ptr(q), _lib.ptr(code), _lib.ptr(W), _lib.ptr(H), T, K, N, dt, act,
-                _lib.ptr(dX), _lib.ptr(dW), _lib.ptr(dB), _lib.ptr(ws), ws.numel(), _lib.stream_ptr(dev)),
+                _lib.ptr(dX), _lib.ptr(dW), _lib.ptr(dB), _lib.ptr(ws), nbytes if ws is not None else 0, _lib.stream_ptr(dev)),
                 "linear_epilogue backward")
         return dX, dW, dB, dY if need[3] else None, None, None, None, None, None
 

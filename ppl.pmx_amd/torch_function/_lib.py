@@ -19,6 +19,7 @@ ABI_VERSION = 1
 
 F32, F16, BF16 = 0, 1, 2
 EPILOGUE_NONE, EPILOGUE_SWIGLU = 0, 1
+LINEAR_DX, LINEAR_DW, LINEAR_DB, LINEAR_X8 = 1, 2, 4, 8
 ACTIVATIONS = {"none": 0, "silu": 1, "gelu": 2, "gelu_tanh": 3, "swiglu": 4}
 MAX_EXPERTS, MAX_EXPERTS_PER_TOKEN = 256, 32
 SELECT_STATIC_SCRATCH_BYTES = 4 << 20
@@ -57,6 +58,9 @@ _SIGNATURES = {
     "opmx_linear_epilogue_kept_bytes": (_sz, [_i64, _i64, _int]),
     "opmx_linear_epilogue_workspace_bytes": (_sz, [_i64, _i64, _i64, _int, _int]),
     "opmx_linear_epilogue": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _int, _vp, _vp, _vp, _sz, _vp]),
+    "opmx_linear_epilogue_gradients_workspace_bytes": (_sz, [_i64, _i64, _i64, _int, _int, _int]),
+    "opmx_linear_epilogue_gradients": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _int, _vp, _vp, _vp,
+                                              _vp, _sz, _vp]),
     "opmx_linear_epilogue_backward_workspace_bytes": (_sz, [_i64, _i64, _i64, _int, _int]),
     "opmx_linear_epilogue_backward": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _int, _vp, _vp, _vp,
                                              _vp, _sz, _vp]),

@@ -371,3 +371,35 @@ def test_the_last_finite_sums_are_kept_finite(act):
     dX, = torch.autograd.grad(Y, x, torch.full((2, 1), 0.75, device=dev(), dtype=torch.bfloat16))
     assert float(Y.detach()[0]) == float("inf") and float(Y.detach()[1]) == 0.0
     assert torch.equal(dX.cpu(), torch.tensor([[0.75] * 3, [0.0] * 3], dtype=torch.bfloat16))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("T,K,N,act", [(40, 72, 56, "silu"), (130, 1001, 515, "none"), (300, 512, 1026, "swiglu"), (64, 4000, 512, "gelu"),
+                                       (5, 33, 7, "none"), (700, 256, 4000, "none")])
+def test_every_set_of_gradients_in_its_own_workspace(dtype, T, K, N, act):
+    """Through the C interface, each in exactly the bytes it asks for: the gradients' bits do not depend on what else is
+    wanted, and nothing behind the workspace is written."""
+    OPMX = opmx()
+    from torch_function import _lib
+    L, d, a, p = _lib.lib(), _lib.dtype_id(torch.empty(0, dtype=dtype), ""), _lib.ACTIVATIONS[act], _lib.ptr
+    X, W, _, _, dY = [None if t is None else t.to(dev()) for t in tensors(T, K, N, dtype, act, False, False)]
+    Y = torch.empty_like(dY)
+    H = torch.empty(L.opmx_linear_epilogue_kept_bytes(T, N, d), dtype=torch.uint8, device=dev())
+    ws = _lib.workspace(L.opmx_linear_epilogue_workspace_bytes(T, K, N, d, a), dev())
+    _lib.check(L.opmx_linear_epilogue(p(X), p(W), None, None, T, K, N, d, a, p(Y), p(H), p(ws), ws.numel(), _lib.stream_ptr(dev())), "")
+    q, code = OPMX.checkpoint8_pack(X)
+    first = {}
+    for wanted in (7, 15, 1, 2, 3, 4, 5, 6, 10, 11, 14):
+        dX, dW, dB = (torch.full((T, K), 9.0, dtype=dtype, device=dev()) if wanted & 1 else None,
+                      torch.full((N, K), 9.0, dtype=dtype, device=dev()) if wanted & 2 else None,
+                      torch.full((N,), 9.0, dtype=dtype, device=dev()) if wanted & 4 else None)
+        need = L.opmx_linear_epilogue_gradients_workspace_bytes(T, K, N, d, a, wanted)
+        ws = torch.full((need + 4096,), 0x5A, dtype=torch.uint8, device=dev())
+        x8 = wanted & 8
+        _lib.check(L.opmx_linear_epilogue_gradients(p(dY), None if x8 else p(X), p(q) if x8 else None, p(code) if x8 else None, p(W),
+                                                    p(H), T, K, N, d, a, p(dX), p(dW), p(dB), p(ws) if need > 256 else None,
+                                                    need if need > 256 else 0, _lib.stream_ptr(dev())), "gradients")
+        assert bool((ws[need:] == 0x5A).all()), wanted
+        for name, got in (("dX", dX), ("dW8" if x8 else "dW", dW), ("dB", dB)):
+            if got is not None:
+                assert bool(torch.isfinite(got).all()) and torch.equal(first.setdefault(name, got), got), (wanted, name)

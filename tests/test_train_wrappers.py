@@ -177,3 +177,59 @@ def test_balance_loss_workspace_holds_every_block():
     for T, E, blocks in ((4096, 100, 256), (200, 100, 13), (1 << 20, 256, 256), (4096, 16, 64), (8192, 64, 256)):
         assert L.opmx_moe_balance_loss_workspace_bytes(T, E) >= blocks * ((E + 3) // 4 * 32 + 4)
     assert L.opmx_moe_balance_loss_workspace_bytes(64, 256) == 256 == L.opmx_moe_balance_loss_workspace_bytes(32, 8)
+
+
+def test_gradients_ask_for_what_they_need():
+    """The workspace holds dH, where it is not dY; X where it is padded or unpacked; W where it is padded; the sums for dB; the
+    sums of k ranges: each only where a wanted gradient takes it."""
+    L = _lib.lib()
+    up = lambda v: -(-v // 256) * 256
+    DX, DW, DB, X8 = 1, 2, 4, 8
+    T, K, N, bf = 8192, 14336, 4096, 2
+    need = lambda act, wanted, T=T, K=K, N=N, dt=bf: L.opmx_linear_epilogue_gradients_workspace_bytes(T, K, N, dt, act, wanted)
+    assert need(0, DX) == need(0, DW) == need(0, DX | DW) == 256                     # many rows: no k ranges
+    assert need(0, DX | X8) == 256 and need(0, DW | X8) == up(T * K * 2)
+    assert need(1, DX) == need(1, DX | DW) == up(T * N * 2)
+    sums = need(0, DB)
+    assert 256 < sums <= up(512 * N * 4) and need(1, DB) == sums
+    assert need(1, DX | DW | DB | X8) == up(T * N * 2) + up(T * K * 2) + sums
+    odd = dict(T=900, K=4001, N=3999)                                               # pitches 4008 and 4000
+    w, x, dh = up(3999 * 4008 * 2), up(900 * 4008 * 2), up(900 * 4000 * 2)
+    assert dh + w <= need(1, DX, **odd) < dh + w + x
+    assert dh + x <= need(1, DW, **odd) < dh + w + x
+    assert need(1, DB, **odd) < dh
+    assert need(0, DX | DW | DB, T=0, K=4001, N=4096) == L.opmx_linear_epilogue_gradients_workspace_bytes(0, 4001, 4096, bf, 0, DW | DB)
+    any_ = L.opmx_linear_epilogue_backward_workspace_bytes
+    for case in ((8192, 14336, 4096, bf, 0), (900, 4001, 3999, 1, 4), (64, 4000, 512, 0, 1), (5, 33, 7, 0, 2), (0, 40, 8, 1, 3)):
+        sizes = [L.opmx_linear_epilogue_gradients_workspace_bytes(*case, w) for w in range(16)]
+        assert max(sizes) == any_(*case)
+    # the call takes exactly that, and the older entry point what may be asked for at most
+    size = need(1, DW, T=64, K=4000, N=512, dt=1)
+    a = [ONE, ONE, None, None, ONE, ONE, 64, 4000, 512, 1, 1, None, ONE, None, ONE]
+    assert L.opmx_linear_epilogue_gradients(*a, size - 1, None) == -3
+    assert L.opmx_linear_epilogue_backward(*a, size, None) == -3
+    a[1], a[2], a[3] = None, ONE, ONE
+    assert L.opmx_linear_epilogue_gradients(*a, size, None) == -3
+
+
+def test_a_workspace_that_is_needed_is_not_called_none():
+    """256 bytes mean that there may be no workspace: the smallest dH, the smallest sums for dB and the smallest padded operand,
+    of 256 bytes and less, are more than that, and without a workspace the call is refused."""
+    L = _lib.lib()
+    DX, DW, DB, X8 = 1, 2, 4, 8
+    for T, K, N, dt, act, wanted in ((1, 64, 64, 1, 0, DB), (1, 64, 64, 1, 0, DX | DW | DB), (3, 100, 36, 0, 0, DB), (1, 64, 64, 1, 1, DX),
+                                     (1, 8, 8, 1, 0, DW | X8), (1, 1, 8, 2, 0, DX), (1, 1, 8, 2, 0, DW), (1, 1, 1, 0, 4, DW)):
+        need = L.opmx_linear_epilogue_gradients_workspace_bytes(T, K, N, dt, act, wanted)
+        assert need >= 512, (T, K, N, dt, act, wanted)
+        if act == 4:
+            continue
+        out = [ONE if wanted & bit else None for bit in (DX, DW, DB)]
+        x8 = ONE if wanted & X8 else None
+        for ws, size in ((None, 0), (None, need), (ONE, need - 1), (ONE, 256)):
+            assert L.opmx_linear_epilogue_gradients(ONE, ONE, x8, x8, ONE, ONE, T, K, N, dt, act, *out, ws, size, None) == -3
+    for T in (0, 1, 17, 33, 65, 130, 1000):
+        for K, N in ((8, 8), (64, 16), (1000, 24), (8192, 64)):
+            for act in range(5):
+                for dt in range(3):
+                    plain = L.opmx_linear_epilogue_gradients_workspace_bytes(T, K, N, dt, act, DB)
+                    assert plain >= 512 if T else plain == 256
