@@ -242,8 +242,8 @@ enum class Tile { k256, k128, k64, k32 };
 int launch_linear_gemm(const Operand &P, const Operand &Q, int64_t Kc, int dtype, const Epilogue &e, Tile tile, int ranges,
                        hipStream_t s);
 
-// The product and its epilogue for few rows of X, from W and X as they are, where it serves.
-bool linear_few_rows_serve(int64_t T, int64_t K, int64_t N, int dtype);
+// The product and its epilogue for up to 64 rows of X, from W and X as they are; and the microseconds that it takes, about.
+double linear_few_rows_us(int64_t T, int64_t K, int64_t N, int dtype, bool gated);
 int launch_linear_few_rows(const void *X, const void *W, int64_t K, int dtype, const Epilogue &e, hipStream_t s);
 
 }  // namespace opmx

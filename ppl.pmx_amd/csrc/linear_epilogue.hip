@@ -10,6 +10,7 @@
 #include "checkpoint8.h"
 #include "linear_epilogue.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace opmx {
@@ -204,6 +205,32 @@ struct Cut {
     int64_t pitch;      // of the ranges' sums
     size_t bytes;       // of the ranges' sums
 };
+// Of the tiles with less than 128 rows.
+//
+// Microseconds of a k-tile, of one workgroup on a CU and of two, and of joining r ranges, fitted to the times of 1 to 16
+// ranges of 27 products with 20 to 3000 rows: the chosen ones are within 8 % of the best.  Returns the chosen one's.
+double short_cut(Cut &c, int64_t rows, int64_t width, int64_t nk, bool p_rows, bool f32)
+{
+    const int64_t columns = ceil_div(width, 128);
+    double best = 0;
+    for (int half = 0; half < (f32 ? 2 : 1); ++half) {
+        const double one = half ? 0.63 : f32 ? 1.1 : p_rows ? 0.45 : 0.34, two = half ? 1.25 : f32 ? 2.2 : p_rows ? 0.65 : 0.62;
+        const int64_t tiles = ceil_div(rows, half ? 32 : 64) * columns;
+        for (int64_t r = 1; r <= 16 && (r == 1 || r * 4 <= nk); ++r) {
+            const int64_t load = ceil_div(tiles * r, 256);
+            const double mb = static_cast<double>(r * rows * width) * 4e-6;
+            const double us = static_cast<double>(ceil_div(nk, r)) *
+                                  (static_cast<double>(load / 2) * two + static_cast<double>(load % 2) * one) +
+                              (r > 1 ? 3.0 + 0.4 * static_cast<double>(r) + 0.3 * mb : 0.0);
+            if ((half == 0 && r == 1) || us < best) {
+                best = us;
+                c.tile = half ? Tile::k32 : Tile::k64;
+                c.ranges = static_cast<int>(r);
+            }
+        }
+    }
+    return best;
+}
 Cut cut_for(int64_t rows, int64_t ncols, int64_t Kc, bool gated, bool p_rows, bool q_rows, int dtype)
 {
     Cut c{Tile::k128, 1, 0, 0};
@@ -222,32 +249,30 @@ Cut cut_for(int64_t rows, int64_t ncols, int64_t Kc, bool gated, bool p_rows, bo
     if (rows > 64 && ceil_div(rows, 128) * columns > 256) return c;
     // In fp32, where a tile of half the rows takes little more than half the matrix units' time, also 32 x 128 (512 x 1024
     // over 1024 18 us, 64 x 128 21; 2048 x 2048 over 2048 150, 135).
-    //
-    // Microseconds of a k-tile, of one workgroup on a CU and of two, and of joining r ranges, fitted to the times of 1 to 16
-    // ranges of 27 products with 20 to 3000 rows: the chosen ones are within 8 % of the best.
-    double best = 0;
-    for (int half = 0; half < (f32 ? 2 : 1); ++half) {
-        const double one = half ? 0.63 : f32 ? 1.1 : p_rows ? 0.45 : 0.34, two = half ? 1.25 : f32 ? 2.2 : p_rows ? 0.65 : 0.62;
-        const int64_t tiles = ceil_div(rows, half ? 32 : 64) * columns;
-        for (int64_t r = 1; r <= 16 && (r == 1 || r * 4 <= nk); ++r) {
-            const int64_t load = ceil_div(tiles * r, 256);
-            const double mb = static_cast<double>(r * rows * width) * 4e-6;
-            const double us = static_cast<double>(ceil_div(nk, r)) *
-                                  (static_cast<double>(load / 2) * two + static_cast<double>(load % 2) * one) +
-                              (r > 1 ? 3.0 + 0.4 * static_cast<double>(r) + 0.3 * mb : 0.0);
-            if ((half == 0 && r == 1) || us < best) {
-                best = us;
-                c.tile = half ? Tile::k32 : Tile::k64;
-                c.ranges = static_cast<int>(r);
-            }
-        }
-    }
+    short_cut(c, rows, width, nk, p_rows, f32);
     if (c.ranges > 1) c.ranges = static_cast<int>(ceil_div(nk, ceil_div(nk, c.ranges)));      // none of them empty
     if (c.ranges > 1) {
         c.pitch = gated ? 2 * up(ncols, 8) : up(ncols, 8);
         c.bytes = static_cast<size_t>(c.ranges) * rows * c.pitch * 4;
     }
     return c;
+}
+
+// Whether a forward pass goes without tiles (linear_few_rows.hip).  Both kinds of kernel are estimated; the tile product's time is
+// that of its workgroups or of reading W, and rows that are not whole chunks are copied first.  Over the 3080 sizes
+// the chosen one takes 0.6 % more than the quicker one in the mean, over 10 % at 85.  Microseconds here and in tiles: 1 x
+// 4096 -> 4096 float16 8.2, 13.8; 20 x 1024 -> 4096 float16 5.4, 9.0; 32 x 4096 -> 1024 float16 14.5, 10.1; 64 x 1024 -> 2816 float32
+// 13.0, 12.8; 64 x 1024 -> 28672 float16 43, 15; 16 x 4095 -> 4096 float32 27, 47; 16 x 14335 -> 1024 float16 88, 31.
+bool few_rows_serve(int64_t Ttok, int64_t K, int64_t N, bool gated, int dtype)
+{
+    if (Ttok > 64) return false;
+    const bool f32 = dtype == OPMX_DTYPE_F32;
+    const int64_t size = f32 ? 4 : 2, width = gated ? 2 * (N / 2) : N;
+    const double mb = static_cast<double>(N * K * size) * 1e-6;
+    Cut c{};
+    const double tiles = 3.7 + 0.9 * short_cut(c, Ttok, width, ceil_div(K, f32 ? 32 : 64), false, f32);
+    const double copies = K * size % 16 == 0 ? 0.0 : 2.5 + mb / 2.4;
+    return linear_few_rows_us(Ttok, K, N, dtype, gated) < std::max(tiles, 4.7 + mb / 4.7) + copies;
 }
 
 template <typename T> int join(const Epilogue &e, int ranges, hipStream_t s)
@@ -307,7 +332,7 @@ ForwardPlan forward_plan(int64_t Ttok, int64_t K, int64_t N, int dtype, int act)
     const int64_t esize = dtype == OPMX_DTYPE_F32 ? 4 : 2, n = 16 / esize, pitch = up(K, n);
     const bool gated = act == OPMX_ACTIVATION_SWIGLU, padded = K % n != 0;
     ForwardPlan p{};
-    if (linear_few_rows_serve(Ttok, K, N, dtype)) return p;
+    if (few_rows_serve(Ttok, K, N, gated, dtype)) return p;
     p.x = 0;
     p.w = p.x + (padded ? up(Ttok * pitch * esize, 256) : 0);
     p.part = p.w + (padded ? up(N * pitch * esize, 256) : 0);
@@ -366,7 +391,7 @@ int forward_impl(const void *X, const void *W, const void *B, const void *R, int
     e.N = N;
     e.ncols = act == OPMX_ACTIVATION_SWIGLU ? N / 2 : N;
     e.act = act;
-    if (linear_few_rows_serve(Ttok, K, N, DType<T>::id)) return launch_linear_few_rows(X, W, K, DType<T>::id, e, s);
+    if (few_rows_serve(Ttok, K, N, act == OPMX_ACTIVATION_SWIGLU, DType<T>::id)) return launch_linear_few_rows(X, W, K, DType<T>::id, e, s);
     const ForwardPlan plan = forward_plan(Ttok, K, N, DType<T>::id, act);
     int64_t pitch = K;
     if (K % n != 0) {

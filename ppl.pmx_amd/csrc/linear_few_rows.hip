@@ -11,13 +11,15 @@
 #include "linear_epilogue.h"
 #include "linear_step.h"
 
+#include <algorithm>
+#include <cmath>
+
 namespace opmx {
 namespace {
 
 constexpr int kFewWaves = 8;
 constexpr int64_t kFewWideColumns = 16384;       // from here on 32 columns per workgroup: 512 workgroups at least
 constexpr int64_t kFewStreamBytes = 8 << 20;     // weights from which on they go through LDS
-constexpr int64_t kFewDirectBytes = 24 << 20;    // weights up to which 17 to 32 rows are few
 
 // 16 bytes at any address; `once`: what the caches need not keep.
 template <typename F, bool ONCE> __device__ __forceinline__ F load_frag(const void *p)
@@ -324,8 +326,8 @@ template <typename T, int NT> int few_rows(const void *X, const void *W, int64_t
     return OPMX_OK;
 }
 
-// Through LDS from kFewStreamBytes of weights on, with at most 16 rows of X (see linear_few_rows_serve): pieces of 512 bytes
-// and two workgroups per CU.  1024 bytes by eight waves, deeper pieces, and workgroups that start k apart were not faster.
+// Through LDS from kFewStreamBytes of weights on, with at most 16 rows of X: pieces of 512 bytes and two workgroups
+// per CU.  1024 bytes by eight waves, deeper pieces, and workgroups that start k apart were not faster.
 template <typename T> int few_rows_by_size(const void *X, const void *W, int64_t K, const Epilogue &e, hipStream_t s)
 {
     if (e.rows > 32) return few_rows<T, 4>(X, W, K, e, s);
@@ -339,16 +341,26 @@ template <typename T> int few_rows_by_size(const void *X, const void *W, int64_t
 
 }  // namespace
 
-// Whether these kernels take a forward pass: up to 16 rows always, up to 32 where the tile product would have to copy W to whole
-// chunks first or W is no more than 24 MB (20 rows, 2048 x 2048: 7.3 us here, 8.9 there; 32 x 1024 x 2816 SwiGLU 7, 11;
-// 32 x 4096 x 4096 14.2, 12.9; 32 x 14336 x 4096 43, 24), up to 64 with short rows of W, where every workgroup's own
-// reading of X is short too (64 x 1024 x 1024 float16 7.5, 9.5; 64 x 1024 x 2816 float32 13.8, 15.5; 64 x 2048 x 2048 float16
-// 12.2, 9.7).
-bool linear_few_rows_serve(int64_t T, int64_t K, int64_t N, int dtype)
+// Fitted, as the tile product's time in linear_epilogue.hip, to both kernels' times at 3080 sizes (1 to 64 rows, K 255 to 14336,
+// N 128 to 28672, float16 and float32, plain and gated, K whole chunks and not, weights out of any cache; bfloat16 is
+// float16): within 15 %, mostly.  A workgroup's time goes with the bytes of a row (kb) and the tiles of W and of X that it
+// multiplies, and the CUs take them in rounds; through LDS it is that or the memory's pace.
+double linear_few_rows_us(int64_t T, int64_t K, int64_t N, int dtype, bool gated)
 {
-    const int64_t size = dtype == OPMX_DTYPE_F32 ? 4 : 2;
-    if (T > 32) return T <= 64 && K <= 1024;
-    return T <= 16 || K * size % 16 != 0 || N * K * size < kFewDirectBytes;
+    const int64_t size = dtype == OPMX_DTYPE_F32 ? 4 : 2, ncols = gated ? N / 2 : N;
+    const double kb = static_cast<double>(K * size) / 1024, mb = static_cast<double>(N * K * size) * 1e-6;
+    const bool whole = K * size % 16 == 0;
+    const int tiles_w = gated ? 2 : 1, tiles_x = T <= 16 ? 1 : T <= 32 ? 2 : 4;
+    const double workgroups = static_cast<double>(ceil_div(ncols, 16));
+    if (T <= 16 && whole && N * K * size >= kFewStreamBytes) {
+        const bool wide = !gated && ncols >= kFewWideColumns;
+        const double us = 3.0 + std::ceil((wide ? workgroups / 2 : workgroups) / 512) * kb * (0.36 * (wide ? 2 : tiles_w) + 0.15);
+        return std::max(us, 3.9 + mb / 5.75);
+    }
+    // rows that start anywhere: 16-byte loads across cache lines, more of them in the 16-bit types
+    const double odd = whole ? 0.0 : size == 2 ? 1.1 * tiles_w - 0.35 * tiles_x + 1.5 * static_cast<double>(T) / 16 : 0.45;
+    const double us = 2.0 + std::ceil(workgroups / 256) * (1.1 + kb * (0.55 * tiles_w + 0.45 * tiles_x + odd));
+    return std::max(us, mb / 3.3);
 }
 
 int launch_linear_few_rows(const void *X, const void *W, int64_t K, int dtype, const Epilogue &e, hipStream_t s)

@@ -403,3 +403,11 @@ def test_every_set_of_gradients_in_its_own_workspace(dtype, T, K, N, act):
         for name, got in (("dX", dX), ("dW8" if x8 else "dW", dW), ("dB", dB)):
             if got is not None:
                 assert bool(torch.isfinite(got).all()) and torch.equal(first.setdefault(name, got), got), (wanted, name)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act,T,K,N", [("none", 16, 14335, 128), ("swiglu", 1, 8191, 130), ("gelu", 32, 4095, 700), ("none", 8, 14336, 128),
+                                       ("silu", 48, 1536, 9000), ("swiglu", 64, 512, 20000), ("none", 40, 501, 4096),
+                                       ("gelu_tanh", 33, 1023, 2100), ("none", 20, 4096, 1024), ("swiglu", 30, 1001, 9000)])
+def test_few_rows_by_either_kernel(dtype, act, T, K, N):
+    check(T, K, N, dtype, act, train=False)

@@ -233,3 +233,19 @@ def test_a_workspace_that_is_needed_is_not_called_none():
                 for dt in range(3):
                     plain = L.opmx_linear_epilogue_gradients_workspace_bytes(T, K, N, dt, act, DB)
                     assert plain >= 512 if T else plain == 256
+
+
+def test_the_quicker_kernel_for_few_rows():
+    """The kernels for few rows need no workspace.  The tile product needs one where it copies rows that are no whole chunks, or
+    cuts k.  Each size with the microseconds of the kernels for few rows and of the tile product."""
+    L = _lib.lib()
+    tiles = [(16, 14335, 128, 1, 0), (8, 14335, 1024, 1, 0), (32, 14335, 1024, 1, 0), (32, 4095, 1024, 1, 0), (20, 8191, 512, 1, 4),
+             (32, 4096, 1024, 1, 0), (20, 4096, 1024, 0, 0), (8, 14336, 128, 1, 0), (64, 14335, 4096, 1, 0), (64, 1001, 28672, 1, 0),
+             (32, 1001, 28672, 2, 0)]    # 88 17, 73 30, 131 30, 40 17, 87 24, 14 10, 25 14, 35 17, 153 54, 80 39, 57 39
+    few = [(64, 501, 4096, 0, 0), (40, 250, 1024, 1, 0), (16, 1001, 4096, 1, 0), (4, 4095, 14336, 0, 0), (32, 4095, 4096, 0, 0),
+           (1, 4096, 28672, 1, 4), (16, 4096, 4096, 2, 0), (20, 1024, 4096, 1, 0), (64, 512, 2816, 1, 0), (64, 1024, 2816, 0, 2)]
+    #      9.6 17, 3.8 7.2, 7.8 17, 73 151, 37 48, 38 50, 9 14, 5.4 9.0, 5.5 6.7, 13.0 12.8
+    for case in tiles:
+        assert L.opmx_linear_epilogue_workspace_bytes(*case) > 256, case
+    for case in few:
+        assert L.opmx_linear_epilogue_workspace_bytes(*case) == 256, case
