@@ -239,8 +239,9 @@ Cut cut_for(int64_t rows, int64_t ncols, int64_t Kc, bool gated, bool p_rows, bo
     const int64_t nk = ceil_div(Kc, f32 ? 32 : 64);
     // The large tile needs most of the 256 CUs busy and k-tiles to spread its start and its end over: against 128 x 128,
     // 4096 x 8192 outputs over 16 k-tiles 76 us and 78, 4096 x 14336 over 4 77 and 57; with k over the rows of both
-    // operands over 16 152 and 141, 4096 x 4096 over 32 66 and 75.
-    if (!f32 && ceil_div(rows, 256) * ceil_div(width, 256) >= 192 && nk >= (q_rows ? 24 : 16)) {
+    // operands over 16 152 and 141, 4096 x 4096 over 32 66 and 75.  And rows for more than half of it: 64 x 49152 over 1024 31 and 20,
+    // 128 x 65536 over 2048 64 and 53, 200 x 65536 over 2048 71 and 84.
+    if (!f32 && rows > 128 && ceil_div(rows, 256) * ceil_div(width, 256) >= 192 && nk >= (q_rows ? 24 : 16)) {
         c.tile = Tile::k256;
         return c;
     }

@@ -411,3 +411,10 @@ def test_every_set_of_gradients_in_its_own_workspace(dtype, T, K, N, act):
                                        ("gelu_tanh", 33, 1023, 2100), ("none", 20, 4096, 1024), ("swiglu", 30, 1001, 9000)])
 def test_few_rows_by_either_kernel(dtype, act, T, K, N):
     check(T, K, N, dtype, act, train=False)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("act,T,N", [("none", 33, 49300), ("swiglu", 128, 49408), ("none", 129, 49300)])
+def test_few_rows_of_many_outputs(dtype, act, T, N):
+    """Up to 128 rows in 128 x 128 or 64 x 128 tiles, above that in the largest."""
+    check(T, 1032, N, dtype, act, train=False)
