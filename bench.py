@@ -66,18 +66,19 @@ MFMA_PEAK_TFLOPS_F32 = 157.3   # dense fp32 MFMA, vendor figure
 # The summaries under profiles/ record them in a line
 #   bench-traffic: workload=<name> forms=<none|swiglu|all> bytes_per_launch=<n> kernel_sources_sha256=<hex>
 # (forms: which fused forms the run used: none, the SwiGLU epilogue alone, or all three as with --fused)
-# together with the hash of the kernel sources the counter run was made with; a line whose hash
-# is not that of the sources in this tree is out of date and is not reported.
+# together with the hash of the kernel sources the counter run was made with: those of the measured layer, as no others have a
+# part in its launches.  A line whose hash is not that of the sources in this tree is out of date and is not reported.
+LAYER_SOURCES = ("activation.hip", "c_api.hip", "common.h", "linear.hip", "moe_gemm.h", "moe_gemm_f32.hip", "moe_gemm_generic.hip",
+                 "moe_gemm_stream.hip", "moe_gemm_tiled.hip", "moe_reduce.hip", "moe_route.h", "moe_select.hip", "rms_norm.hip")
+
+
 def kernel_sources_sha256():
-    import glob
     import hashlib
     h = hashlib.sha256()
-    csrc = os.path.join(ROOT, "ppl.pmx_amd", "csrc")
-    for path in sorted(glob.glob(os.path.join(csrc, "*.hip")) + glob.glob(os.path.join(csrc, "*.h"))):
-        if os.path.basename(path) == "device_ceilings.hip":
-            continue
-        h.update(os.path.basename(path).encode())
-        h.update(open(path, "rb").read())
+    for name in sorted(LAYER_SOURCES):
+        h.update(name.encode())
+        with open(os.path.join(ROOT, "ppl.pmx_amd", "csrc", name), "rb") as f:
+            h.update(f.read())
     return h.hexdigest()
 
 

@@ -17,7 +17,7 @@
 // distinct, equal fp32 scores at the k-th place are settled by id in a branch few waves take.
 // Sums of p: fp32 over up to kFold tokens of a lane and over the lanes of the block, 64 bits beyond, in a fixed order: results
 // do not vary, and what a sum is off by does not grow with the number of tokens.
-#include "common.h"
+#include "train.h"
 
 namespace opmx {
 namespace {

@@ -12,7 +12,7 @@
 // a power of two is exact in bfloat16 as well.  A block with an infinity or a NaN has code 255 and stands for
 // NaN throughout: there is no step for it, and nothing finite may come out of it.
 #pragma once
-#include "common.h"
+#include "train.h"
 
 namespace opmx {
 namespace {

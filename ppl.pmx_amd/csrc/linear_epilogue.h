@@ -2,7 +2,7 @@
 // what happens to eight neighbouring columns of H = X W^T once they are complete.
 //   Y = act(H + B) + R, all in fp32 and rounded once.
 #pragma once
-#include "common.h"
+#include "train.h"
 
 namespace opmx {
 namespace {
