@@ -247,7 +247,17 @@ Cut cut_for(int64_t rows, int64_t ncols, int64_t Kc, bool gated, bool p_rows, bo
     }
     // More tiles than CUs: 128 x 128 (float16, 3000 x 2816 outputs over 2048: 54 us, 64 x 128 55, the gradients 47 and 55).
     // Fewer: 64 x 128 (512 x 1024 over 1024 9 us, 128 x 128 13; 100 x 2048 over 1408 11 and 17), with k in ranges where it is long.
-    if (rows > 64 && ceil_div(rows, 128) * columns > 256) return c;
+    if (rows > 64 && ceil_div(rows, 128) * columns > 256) {
+        // In fp32 the matrix units' time of the last round decides: microseconds of a k-tile, of one and of two workgroups on a CU.
+        // 181 x 19264 over 1600 117 us in 64 x 128 tiles and 203 in 128 x 128, 3000 x 2816 over 2048 329 and 383, 8192 x 1024 over 1024
+        // 149 and 130.  Over 1750 products of 65 to 28672 rows the chosen tile is 1.1 % over the best in the mean and 22 % at most.
+        auto rounds = [](int64_t tiles, double one, double two) {
+            const int64_t load = ceil_div(tiles, 256);
+            return static_cast<double>(load / 2) * two + static_cast<double>(load % 2) * one;
+        };
+        if (f32 && rounds(ceil_div(rows, 64) * columns, 1.15, 2.2) < rounds(ceil_div(rows, 128) * columns, 1.93, 3.87)) c.tile = Tile::k64;
+        return c;
+    }
     // In fp32, where a tile of half the rows takes little more than half the matrix units' time, also 32 x 128 (512 x 1024
     // over 1024 18 us, 64 x 128 21; 2048 x 2048 over 2048 150, 135).
     short_cut(c, rows, width, nk, p_rows, f32);

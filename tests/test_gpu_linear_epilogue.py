@@ -418,3 +418,9 @@ def test_few_rows_by_either_kernel(dtype, act, T, K, N):
 def test_few_rows_of_many_outputs(dtype, act, T, N):
     """Up to 128 rows in 128 x 128 or 64 x 128 tiles, above that in the largest."""
     check(T, 1032, N, dtype, act, train=False)
+
+
+@pytest.mark.parametrize("act,T,K,N", [("swiglu", 181, 333, 19264), ("none", 4500, 100, 1024), ("gelu", 1200, 520, 2400)])
+def test_float32_past_one_round_of_tiles(act, T, K, N):
+    """More 128 x 128 tiles than CUs: those or 64 x 128, whichever fills its last round better."""
+    check(T, K, N, torch.float32, act)
