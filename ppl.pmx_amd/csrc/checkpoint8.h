@@ -7,8 +7,9 @@
 // never beyond the type's largest exponent -- the step is 2^max(e - 6, -126), a value x is held as the whole
 // number round-half-even(x / step) in [-127, 127], and the block's code is the step's biased exponent, one
 // byte.  Dividing by the step, rounding and multiplying back are exact in fp32, so every kernel agrees on
-// every bit; |x - held(x)| <= step / 2 <= m / 127.5 (only values beyond 127.5 steps at the very top of the
-// type's range, where the step may not grow, are off by up to one step).  A whole number of 7 bits times
+// every bit; |x - held(x)| <= max(m / 127.5, 2^-127): half a step, except that values beyond 127.5 steps at the very top
+// of the type's range, where the step may not grow, are off by up to one, which is no more of m; and 2^-127 is
+// half of the smallest step, so that a block below it is held as zeros.  A whole number of 7 bits times
 // a power of two is exact in bfloat16 as well.  A block with an infinity or a NaN has code 255 and stands for
 // NaN throughout: there is no step for it, and nothing finite may come out of it.
 #pragma once

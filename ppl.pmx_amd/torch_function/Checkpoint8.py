@@ -2,8 +2,8 @@
 the reference, which only runs forward; not ONNX nodes).
 
 Blocks of 32 values of the last dimension share a power-of-two step and hold whole numbers in [-127, 127]:
-8.25 bits per value instead of 16 or 32, at most 1/127.5 of the block's largest magnitude off
-(``include/opmx_moe.h`` has the definition).  A block with an infinity or a NaN stands for NaN throughout.
+8.25 bits per value instead of 16 or 32, off by at most 1/127.5 of the block's largest magnitude or 2^-127, whichever is
+more (``include/opmx_moe.h`` has the definition).  A block with an infinity or a NaN stands for NaN throughout.
 """
 import torch
 from torch.autograd.function import once_differentiable

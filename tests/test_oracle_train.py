@@ -73,3 +73,17 @@ def test_balance_loss_by_hand_and_by_differences():
     assert abs(float(direct) - float(loss)) < 1e-12
     g, = torch.autograd.grad(direct, z)
     assert torch.allclose(O.balance_loss_backward(z.detach(), w, 1.0, mask), g, atol=1e-14)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_8_bits_at_both_ends_of_the_range(dtype):
+    """1/127.5 of the block's largest magnitude also where the step may not grow any more; 2^-127 where it may not shrink."""
+    info = torch.finfo(dtype)
+    top = torch.tensor([info.max, info.max * 0.998, info.max * 0.996, info.max / 2, info.max / 250, -info.max * 0.99], dtype=torch.float64)
+    low = torch.tensor([2.0 ** -119, 2.0 ** -120, 2.0 ** -126, 0.4 * 2.0 ** -126, 2.0 ** -127, 1.4 * 2.0 ** -133], dtype=torch.float64)
+    for values in (top, low, low[3:]):
+        x = values.to(dtype)[None]
+        err, m = (O.held8(x) - x.double()).abs().max(), x.double().abs().max()
+        assert float(err) <= max(float(m) / 127.5, 2.0 ** -127)
+    x = torch.tensor([[0.4 * 2.0 ** -126]])
+    assert float(O.held8(x)) == 0.0                                  # all of it, and still within 2^-127
