@@ -291,6 +291,8 @@ int opmx_swiglu_checkpoint8_backward(const void *dY, const int8_t *q, const uint
  * it is, otherwise 24 bits of it (4 or 3 bytes per value; the layout is the library's).
  * gradients: from dY [T,M]
  *   dH = dY * act'(H) (rounded to dtype),  dX = dH W [T,K],  dW = dH^T X [N,K],  dB = sum_t dH [N] (summed unrounded)
+ * (in float16 a dH past 65504, under a loss scale for instance, is an infinity, and so are the row of dX and the rows of
+ * dW that it goes into, also where they would fit),
  * each of dX, dW, dB may be NULL (not wanted).  dX needs W; dW needs X, or its 8-bit form x_q, x_code (see
  * opmx_checkpoint8_pack; then X is ignored); every activation but NONE needs H.  The gradient of R is dY.
  * X, W, dY start at multiples of 16 bytes where K (dY: N, without an activation) is a multiple of 16 bytes

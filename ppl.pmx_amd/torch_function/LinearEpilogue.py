@@ -97,7 +97,10 @@ def linear_epilogue(X: torch.Tensor, W: torch.Tensor, B: torch.Tensor, residual:
     X [*, in_features], W [out_features, in_features], B [out_features] or None; ``activation`` is none, silu, gelu,
     gelu_tanh or swiglu (as ``swiglu``: first half the gated one, output and residual [*, out_features / 2]).
     Differentiable in X, W, B and residual.  Where an activation needs it, X W^T + B is kept for the backward pass, in
-    4 bytes per value for float32 and in 3 for the 16-bit types (under ``torch.no_grad`` nothing is).  ``checkpoint8``
+    4 bytes per value for float32 and in 3 for the 16-bit types (under ``torch.no_grad`` nothing is).  For the gradients of X and W
+    the gradient of X W^T + B is rounded to the tensors' type, as the matrix units take it: in float16 one past 65504 becomes an
+    infinity there.  X, W and the gradient of the output are copied first where they are not contiguous or do not start at
+    a multiple of 16 bytes.  ``checkpoint8``
     keeps X for the gradient of W in 8 bits (``checkpoint8_pack``) instead of as it is; the other gradients do not
     change.
     A backward pass is captured into a graph together with its forward pass, with no eager pass over the same leaves

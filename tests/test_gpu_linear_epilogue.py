@@ -424,3 +424,37 @@ def test_few_rows_of_many_outputs(dtype, act, T, N):
 def test_float32_past_one_round_of_tiles(act, T, K, N):
     """More 128 x 128 tiles than CUs: those or 64 x 128, whichever fills its last round better."""
     check(T, K, N, torch.float32, act)
+
+
+@pytest.mark.parametrize("checkpoint8", [False, True])
+def test_a_dh_beyond_float16_is_an_infinity(checkpoint8):
+    """dH is rounded to the type for the products: where dY act'(H) is past 65504, the row of dX and the rows of dW that it goes
+    into are infinities or NaN, as a loss scale that is too large has to show, and no others.  dB is summed unrounded."""
+    OPMX = opmx()
+    T, K, N = 70, 64, 48
+    X, W, B, _, dY = [None if t is None else t.to(dev()) for t in tensors(T, K, N, torch.float16, "swiglu", True, False)]
+    W = W.clone()
+    W[:N // 2] *= 0.1
+    with torch.no_grad():
+        B[24 + 3] = 300.0                                            # g of column 3 in every row
+    leaves = [t.clone().requires_grad_(True) for t in (X, W, B)]
+    run = lambda d: torch.autograd.grad(OPMX.linear_epilogue(*leaves, None, K, N, "swiglu", checkpoint8=checkpoint8), leaves, d)
+    dY = dY.clone()
+    dY[:, 3] = 0.25
+    clean = run(dY)
+    big = dY.clone()
+    big[5, 3], big[6, 3] = 3000.0, -3832.0                           # dH = 8e5 and -8e5
+    _, H = O.linear_epilogue(X.cpu(), W.cpu(), B.cpu(), None, "swiglu")
+    fa, fg = O.act(H, "swiglu")[1]
+    dH = torch.cat([fa * big.cpu().double(), fg * big.cpu().double()], 1)
+    over = dH.abs() > 65520
+    assert sorted(over.nonzero().tolist()) == [[5, 3], [6, 3]]
+    dX, dW, dB = run(big)
+    rows, cols = torch.ones(T, dtype=torch.bool), torch.ones(N, dtype=torch.bool)
+    rows[[5, 6]] = False
+    cols[[3, 27]] = False                                            # (27: the other half's gradient is finite, but another)
+    assert not bool(torch.isfinite(dX[~rows]).any()) and not bool(torch.isfinite(dW[3]).any())
+    assert torch.equal(dX[rows], clean[0][rows]) and torch.equal(dW[cols], clean[1][cols])
+    assert bool(torch.isfinite(dW[27]).all()) and bool(torch.isfinite(dB).all())
+    # H in 24 bits moves the slope by 2^-17 |H|, |H| < 1 in these two rows: 8e5 2^-17 each, and as much again for the arithmetic
+    assert abs(float(dB[3]) - float(dH[:, 3].sum())) <= 2 * 2 * 8.1e5 * 2.0 ** -17 + 4096 * 2.0 ** -11
