@@ -3,8 +3,9 @@
 // backward reads the 8-bit input and dY and writes dX.
 //   Y = g a s(beta a),  s the logistic function, X = (a | g)
 //   dg = dY a s(beta a),  da = dY g s(beta a) (1 + beta a (1 - s(beta a)))      at the held a, g
-// All of it is elementwise and bound by memory: [16384, 2 x 14336] bfloat16 moves 1.89 GB forward, in 345 us (5.5 TB/s), and as
-// much backward, in 315 us (6.0 TB/s; a copy of that size reaches 4.9).  A lane takes 16 bytes of a row, so a block of 32 values lies in
+// All of it is elementwise and bound by memory: [16384, 2 x 14336] bfloat16 moves 1.89 GB forward, in 343 us (5.5 TB/s), and as
+// much backward, in 318 us (5.9 TB/s; a copy of that size reaches 4.9), from a replayed graph; pack and unpack of
+// [16384, 14336] 134 and 126 us (5.3 and 5.7 TB/s).  A lane takes 16 bytes of a row, so a block of 32 values lies in
 // 4 (16-bit types) or 8 (fp32) neighbouring lanes and its largest magnitude is two or three cross-lane steps.
 // Rows may start at any address: loads and stores of 16 bytes need no alignment on this part, only the
 // last values of a row that fill no chunk go one by one.
@@ -219,7 +220,7 @@ __global__ __launch_bounds__(256) void swiglu8_backward_kernel(const T *__restri
     const int64_t c = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) * n, left = D - c;
     if (left <= 0) return;
     const int64_t step = static_cast<int64_t>(gridDim.y) * blockDim.y;
-    // `here` values exist: a constant where all do, so that nothing stands between the loads (338 us without, 315 with)
+    // `here` values exist: a constant where all do, so that nothing stands between the loads (7 % slower without)
     auto rows = [&](auto here) {
         for (int64_t r = static_cast<int64_t>(blockIdx.y) * blockDim.y + threadIdx.y; r < R; r += step) {
             const uint32_t ca = codes[r * 2 * blocks + c / kBlock8], cg = codes[(r * 2 + 1) * blocks + c / kBlock8];

@@ -23,8 +23,8 @@ constexpr float kInvSqrt2Pi = 0.39894228040143268f;
 
 // Phi(h) for GELU, and e^(-h^2 / 2), which the slope needs as well.  With z = |h| / sqrt 2, erfc(z) = e^(-z^2) t S(t) where
 // t = 1 / (1 + 0.4 z) and S is smooth: a polynomial of degree 8 fitted to scipy's erfcx for z <= 14 (beyond,
-// e^(-z^2) is 0 in fp32) is within 9e-8 of it, relatively, on both sides: Phi keeps its digits where it is small.
-// In fp32 the whole is within 4e-7 (1 + h^2 / 4).  The library's erfc costs four times the instructions, in an epilogue
+// e^(-z^2) is 0 in fp32) is within 1.13e-7 of it, relatively, on both sides: Phi keeps its digits where it is small.
+// In fp32 the whole is within 7e-7 (1 + h^2 / 4).  The library's erfc costs four times the instructions, in an epilogue
 // whose time no matrix instruction hides.
 __device__ __forceinline__ float normal_cdf(float h, float &bell)
 {

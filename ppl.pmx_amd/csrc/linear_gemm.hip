@@ -402,8 +402,8 @@ __global__ __launch_bounds__(WM *WN *kWave, 2) void linear_gemm_kernel(Operand P
 //   k over rows of one or both: the fragments come through transposing reads, in front of which the compiler would wait
 //   for all loads.  There a block of 16 MFMAs with the four fragments that it reads, and the wait for them, is one piece.
 //
-// bfloat16, 4096 x 28672 outputs over 4096: 742 us, 1300 TFLOP/s (eight waves: 820 us); 4096 x 8192 over 14336 785 us; the
-// gradients of the same 720 to 890 us.  The matrix units work for 68 % of the clocks; k-tiles of MFMAs alone would take
+// bfloat16, 4096 x 28672 outputs over 4096: 725 us, 1327 TFLOP/s (eight waves: 820 us), its gradients 723 and 766; 8192 x 4096
+// over 14336 with a residual 728 us, its gradients 771 and 773 (medians; the clocks under this load differ by 10 % from box to box).  The matrix units work for 68 % of the clocks; k-tiles of MFMAs alone would take
 // 2048 clocks of 2950.  Reads spread over 48 MFMAs instead of 32, loads every third MFMA instead of every fifth,
 // blocks of 32 MFMAs, and workgroups that load their next tile during the epilogue made no difference or a slower one;
 // 32 x 32 x 16 MFMAs 770 us.

@@ -7,7 +7,7 @@ signatures (``torch_function/__init__.py:15,17-20,29-30,37-38`` of OpenPPL/ppl.p
 the seven operators of the MoE layer and the RMSNorm pair in front of it, plus fused forms that
 are not ONNX nodes (gate/up GEMM with SwiGLU, router gate with MoeSelect, and MoeSelect as an
 index that the gate/up GEMM reads the tokens through, without the expanded copy), and operators with
-gradients, for training beside the layer: a linear with bias, activation and residual in its epilogue,
+gradients, for training beside the layer, which itself only runs forward: a linear with bias, activation and residual in its epilogue,
 SwiGLU and activations kept in 8 bits, and the router's balance loss.
 """
 from .Checkpoint8 import checkpoint8_pack, checkpoint8_unpack, swiglu_checkpoint8
