@@ -403,10 +403,10 @@ __global__ __launch_bounds__(WM *WN *kWave, 2) void linear_gemm_kernel(Operand P
 //   for all loads.  There a block of 16 MFMAs with the four fragments that it reads, and the wait for them, is one piece.
 //
 // bfloat16, 4096 x 28672 outputs over 4096: 725 us, 1327 TFLOP/s (eight waves: 820 us), its gradients 723 and 766; 8192 x 4096
-// over 14336 with a residual 728 us, its gradients 771 and 773 (medians; the clocks under this load differ by 10 % from box to box).  The matrix units work for 68 % of the clocks; k-tiles of MFMAs alone would take
-// 2048 clocks of 2950.  Reads spread over 48 MFMAs instead of 32, loads every third MFMA instead of every fifth,
-// blocks of 32 MFMAs, and workgroups that load their next tile during the epilogue made no difference or a slower one;
-// 32 x 32 x 16 MFMAs 770 us.
+// over 14336 with a residual 728 us, its gradients 771 and 773 (medians; the clocks under this load differ by 10 % from call to
+// call).  The matrix units work for 68 % of the clocks; k-tiles of MFMAs alone would take 2048 clocks of 2950.  Reads spread
+// over 48 MFMAs instead of 32, loads every third MFMA instead of every fifth, blocks of 32 MFMAs, and workgroups that
+// load their next tile during the epilogue made no difference or a slower one; 32 x 32 x 16 MFMAs 4 % slower.
 #define OPMX_WIDE_ROWS(OP)                                                                                            \
     asm volatile("s_nop 1\n\t"                                                                                        \
                  "v_mfma_f32_16x16x32_" OP " %0, %20, %24, %0\n\t"                                                    \
